@@ -15,7 +15,7 @@ from typing import Any, Optional
 
 import torch
 
-from . import reference as R
+from . import paged, reference as R
 from .gates import GateSpec
 from .srw_ref import SRWResult, prepare_pool_ref, srw_pool_ref
 
@@ -82,6 +82,22 @@ class ReferenceBackend:
 
     def diversity(self, tensors):
         return R.pool_diversity(tensors)
+
+    # ---- paged key/value cache -----------------------------------------
+    @torch.no_grad()
+    def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
+        paged.write(k, v, k_pages, v_pages, table, lengths, starts, k_scale, v_scale)
+
+    @torch.no_grad()
+    def paged_read(self, k_pages, v_pages, table, lengths, max_len, k_scale=None, v_scale=None,
+                   dtype=torch.float32):
+        return paged.read(k_pages, v_pages, table, lengths, max_len, k_scale, v_scale, dtype)
+
+    @torch.no_grad()
+    def paged_attention(self, q, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None, *,
+                        max_new=None, window=None, sinks=0, scale=None):
+        return paged.attention(q, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, max_new=max_new,
+                               window=window, sinks=sinks, scale=scale)
 
     # ---- SRW pool op ---------------------------------------------------
     def prepare_pool(self, emb, read, write, spec: GateSpec, pctx: Optional[ParallelCtx] = None):

@@ -1188,6 +1188,8 @@ Tensor grad_sq_norm(std::vector<Tensor> grads) {
 
 }  // namespace
 
+void register_paged(py::module_& m);   // bindings_paged.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm", &gemm);
   m.def("srw_fwd_gate", &srw_fwd_gate);
@@ -1240,4 +1242,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("small_allreduce", &small_allreduce);
   m.def("zero_reduce", &zero_reduce);
   m.def("zero_adam_scatter", &zero_adam_scatter);
+  register_paged(m);
 }

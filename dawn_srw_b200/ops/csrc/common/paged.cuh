@@ -1,0 +1,128 @@
+// Device-side view of a paged key/value cache: which sequence a packed row belongs to, where a
+// position lives, and 8-bit codes as bf16.
+#pragma once
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "../dsb_api_paged.h"
+
+namespace dsb {
+namespace paged {
+
+constexpr int kStatusBadPage = 4;   // a table entry or a length outside the cache
+
+enum Kind { kBf16 = 0, kE4m3 = 1, kInt8 = 2 };
+
+struct View {
+  DsbPaged c;
+  int shift;                        // log2(page)
+};
+
+inline View make_view(const DsbPaged* c) {
+  View w;
+  w.c = *c;
+  w.shift = 0;
+  while ((1 << w.shift) < c->page) ++w.shift;
+  return w;
+}
+
+// What the launchers refuse (the kernels' vector accesses and shifts rely on it).
+inline bool bad_cache(const DsbPaged* c) {
+  if (c->kind < 0 || c->kind > 2 || c->dh < 16 || c->dh > 128 || c->dh % 16 != 0) return true;
+  if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1)) != 0) return true;
+  if (c->H <= 0 || c->n_pages < 0 || c->B < 0 || c->width < 0 || c->N < 0) return true;
+  if (c->starts == nullptr && c->N != c->B) return true;
+  if (c->kind != kBf16 && (c->k_scale == nullptr || c->v_scale == nullptr)) return true;
+  return ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) != 0;
+}
+
+struct Rows { int first, count; };  // packed rows of a sequence
+
+__device__ __forceinline__ Rows seq_rows(const View& w, int b) {
+  if (w.c.starts == nullptr) return {b, 1};
+  const int a = min(max(w.c.starts[b], 0), w.c.N), e = min(max(w.c.starts[b + 1], a), w.c.N);
+  return {a, e - a};
+}
+
+// Positions of sequence b: what the table can hold at most.
+__device__ __forceinline__ int seq_length(const View& w, int b) {
+  const int len = w.c.lengths[b];
+  const long long cap = static_cast<long long>(w.c.width) << w.shift;
+  if (len > cap) {
+    atomicExch(w.c.status, kStatusBadPage);
+    return static_cast<int>(cap);
+  }
+  return max(len, 0);
+}
+
+// The sequence that packed row t belongs to, or -1 (rows before the first or behind the last one).
+__device__ __forceinline__ int seq_of_row(const View& w, int t) {
+  if (w.c.starts == nullptr) return t;
+  int lo = 0, hi = w.c.B;                          // the last b with starts[b] <= t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (w.c.starts[mid + 1] <= t) lo = mid + 1; else hi = mid;
+  }
+  return lo < w.c.B && w.c.starts[lo] <= t ? lo : -1;
+}
+
+// Page of position `pos` of sequence b, or -1 where the table names none of the pool.
+__device__ __forceinline__ int page_of(const View& w, int b, int pos) {
+  const int id = w.c.table[static_cast<size_t>(b) * w.c.width + (pos >> w.shift)];
+  if (static_cast<unsigned>(id) >= static_cast<unsigned>(w.c.n_pages)) {
+    atomicExch(w.c.status, kStatusBadPage);
+    return -1;
+  }
+  return id;
+}
+
+// Index of (page, head, slot of pos) among the rows of the pool: times dh for elements.
+__device__ __forceinline__ size_t slot_row(const View& w, int page, int h, int pos) {
+  return ((static_cast<size_t>(page) * w.c.H + h) << w.shift) + (pos & (w.c.page - 1));
+}
+
+// Four 8-bit codes -> four bf16 (two registers), exactly, without a conversion instruction.
+// int8: 128 + (low seven bits) and 128 or 256 (by the sign bit) are bf16 values whose bits are the code's
+// own; their difference is the number.  e4m3: exponent and fraction moved into bf16's places read as the
+// value times 2^-120 (the biases differ by 120, subnormals included), so one product puts it right.  The
+// NaN codes 0x7f, 0xff, which no write here makes, read as +-480.
+template <int KIND>
+__device__ __forceinline__ uint2 codes_to_bf16(uint32_t x) {
+  uint2 r = {__byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342)};
+  auto one = [](uint32_t p) -> uint32_t {
+    if (KIND == kInt8) {
+      const uint32_t a = (p & 0x007f007fu) | 0x43004300u, b = (p & 0x00800080u) | 0x43004300u;
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&b));
+      return *reinterpret_cast<const uint32_t*>(&d);
+    }
+    const uint32_t a = ((p & 0x007f007fu) << 4) | ((p & 0x00800080u) << 8), s = 0x7b807b80u;   // 2^120 twice
+    const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&s));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  };
+  r.x = one(r.x);
+  r.y = one(r.y);
+  return r;
+}
+
+// Eight elements at `row * dh + col` of a pool as four registers of bf16 pairs.
+template <int KIND>
+__device__ __forceinline__ uint4 load8(const void* pool, size_t elem) {
+  if (KIND == kBf16) return __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + elem));
+  const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + elem));
+  const uint2 a = codes_to_bf16<KIND>(c.x), b = codes_to_bf16<KIND>(c.y);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+__device__ __forceinline__ void bf16x8_to_f32(const uint4& u, float* f) {
+  const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(r[i] << 16);
+    f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+  }
+}
+
+}  // namespace paged
+}  // namespace dsb

@@ -1,0 +1,319 @@
+// Paged key/value cache: rows into pages (rounded to the pages' type on the way), pages back to dense
+// tensors, attention of new tokens over pages.  Types, layouts and bounds: dsb_api_paged.h.
+#include <cuda_fp8.h>
+
+#include "common/paged.cuh"
+#include "common/ptx.cuh"
+
+namespace dsb {
+namespace paged {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLeast = 7.888609e-31f;      // 2^-100: a row without a larger value is stored as zeros
+
+// Lanes that share a row: eight elements each, a power of two of them.
+__host__ __device__ constexpr int lanes_per_row(int dh) {
+  return dh <= 16 ? 2 : dh <= 32 ? 4 : dh <= 64 ? 8 : 16;
+}
+
+struct Eight { float f[8]; };
+
+template <bool SRC_BF16>
+__device__ __forceinline__ Eight load_src(const void* p, size_t at) {
+  Eight e;
+  if (SRC_BF16) {
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at)), e.f);
+  } else {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    *reinterpret_cast<float4*>(e.f) = __ldg(q);
+    *reinterpret_cast<float4*>(e.f + 4) = __ldg(q + 1);
+  }
+  return e;
+}
+
+// One row's share of eight elements into a pool.  8-bit kinds take the row's largest magnitude as bits, so that
+// NaN and infinity, which sort above every number, are seen: such a row is stored as zeros with a NaN scale.
+//   e4m3: scale = the smallest power of two with largest / scale <= 448: x / scale is exact and the code is the
+//         only rounding.  int8: scale = largest / 127, code = rint(x * (127 / largest)).
+template <int KIND, int LPR>
+__device__ __forceinline__ void store_row(void* pool, float* scales, size_t row, int dh, int lane, const Eight& e) {
+  const int col = 8 * lane;
+  const bool on = col < dh;
+  if (KIND == kBf16) {
+    if (on)
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(pool) + row * dh + col) =
+          make_uint4(pack_bf16x2(e.f[0], e.f[1]), pack_bf16x2(e.f[2], e.f[3]), pack_bf16x2(e.f[4], e.f[5]),
+                     pack_bf16x2(e.f[6], e.f[7]));
+    return;
+  }
+  uint32_t top = 0;
+  if (on) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(e.f[i]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int x = 1; x < LPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+  const float amax = __uint_as_float(top);
+  const bool odd = top >= 0x7f800000u, some = !odd && amax >= kLeast;
+  float scale = 1.f, inv = 1.f;
+  if (some) {
+    if (KIND == kE4m3) {
+      const uint32_t s = (top >> 23) - ((top & 0x7fffffu) <= 0x600000u ? 8u : 7u);   // biased exponent
+      scale = __uint_as_float(s << 23);
+      inv = __uint_as_float((254u - s) << 23);
+    } else {
+      scale = __fdiv_rn(amax, 127.f);
+      inv = __fdiv_rn(127.f, amax);
+    }
+  }
+  uint32_t w[2] = {0u, 0u};
+  if (!odd) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float a = e.f[i] * inv, b = e.f[i + 1] * inv;
+      uint32_t c;
+      if (KIND == kE4m3)
+        c = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+      else
+        c = (static_cast<uint32_t>(__float2int_rn(a)) & 0xffu) | ((static_cast<uint32_t>(__float2int_rn(b)) & 0xffu) << 8);
+      w[i >> 2] |= c << (8 * (i & 2));
+    }
+  }
+  if (on) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pool) + row * dh + col) = make_uint2(w[0], w[1]);
+  if (lane == 0) scales[row] = odd ? __uint_as_float(0x7fc00000u) : scale;
+}
+
+// A group of LPR lanes per (new token, head): its key and its value.
+template <int KIND, bool SRC_BF16, int LPR>
+__global__ void __launch_bounds__(kThreads) paged_write_kernel(const View w, const void* __restrict__ k,
+                                                               const void* __restrict__ v, long long k_st, long long k_sh,
+                                                               long long v_st, long long v_sh) {
+  const long long g = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) / LPR;
+  const int lane = threadIdx.x % LPR, col = 8 * lane;
+  const long long rows = static_cast<long long>(w.c.N) * w.c.H;
+  int t = -1, h = 0, page = -1, pos = -1;
+  if (g < rows) {
+    t = static_cast<int>(g / w.c.H);
+    h = static_cast<int>(g - static_cast<long long>(t) * w.c.H);
+    const int b = seq_of_row(w, t);
+    if (b >= 0) {
+      const Rows r = seq_rows(w, b);
+      const int len = seq_length(w, b);
+      pos = len - r.count + (t - r.first);
+      if (pos >= 0 && pos < len) page = page_of(w, b, pos);
+    }
+  }
+  const bool on = page >= 0 && col < w.c.dh;
+  Eight ek, ev;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ek.f[i] = ev.f[i] = 0.f;
+  if (on) {
+    ek = load_src<SRC_BF16>(k, static_cast<size_t>(t) * k_st + static_cast<size_t>(h) * k_sh + col);
+    ev = load_src<SRC_BF16>(v, static_cast<size_t>(t) * v_st + static_cast<size_t>(h) * v_sh + col);
+  }
+  // every lane takes part in the shuffles; a group without a page stores nothing
+  const size_t row = page >= 0 ? slot_row(w, page, h, pos) : 0;
+  const int dh = page >= 0 ? w.c.dh : 0;
+  if (KIND == kBf16) {
+    store_row<KIND, LPR>(w.c.k, nullptr, row, dh, lane, ek);
+    store_row<KIND, LPR>(w.c.v, nullptr, row, dh, lane, ev);
+  } else {
+    store_row<KIND, LPR>(w.c.k, w.c.k_scale, row, dh, page >= 0 ? lane : 99, ek);
+    store_row<KIND, LPR>(w.c.v, w.c.v_scale, row, dh, page >= 0 ? lane : 99, ev);
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ Eight read8(const void* pool, const float* scales, size_t row, int dh, int col) {
+  Eight e;
+  if (KIND == kBf16) {
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + row * dh + col)), e.f);
+    return e;
+  }
+  const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + row * dh + col));
+  const float s = __ldg(scales + row);
+  bf16x8_to_f32(make_uint4(codes_to_bf16<KIND>(c.x).x, codes_to_bf16<KIND>(c.x).y, codes_to_bf16<KIND>(c.y).x,
+                           codes_to_bf16<KIND>(c.y).y), e.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e.f[i] *= s;
+  return e;
+}
+
+template <bool DST_BF16>
+__device__ __forceinline__ void write8(void* p, size_t at, const Eight& e) {
+  if (DST_BF16) {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) =
+        make_uint4(pack_bf16x2(e.f[0], e.f[1]), pack_bf16x2(e.f[2], e.f[3]), pack_bf16x2(e.f[4], e.f[5]),
+                   pack_bf16x2(e.f[6], e.f[7]));
+  } else {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    q[0] = *reinterpret_cast<const float4*>(e.f);
+    q[1] = *reinterpret_cast<const float4*>(e.f + 4);
+  }
+}
+
+// A group of LPR lanes per (sequence, head, position): blockIdx.x = sequence and head, blockIdx.y = positions.
+template <int KIND, bool DST_BF16, int LPR>
+__global__ void __launch_bounds__(kThreads) paged_read_kernel(const View w, void* __restrict__ k, void* __restrict__ v,
+                                                              int max_len) {
+  const int b = blockIdx.x / w.c.H, h = blockIdx.x - b * w.c.H;
+  const int col = 8 * (threadIdx.x % LPR), len = min(seq_length(w, b), max_len);
+  if (col >= w.c.dh) return;
+  for (long long p = blockIdx.y * (kThreads / LPR) + threadIdx.x / LPR; p < max_len;
+       p += static_cast<long long>(gridDim.y) * (kThreads / LPR)) {
+    const int pos = static_cast<int>(p);
+    Eight ek, ev;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ek.f[i] = ev.f[i] = 0.f;
+    const int page = pos < len ? page_of(w, b, pos) : -1;
+    if (page >= 0) {
+      const size_t row = slot_row(w, page, h, pos);
+      ek = read8<KIND>(w.c.k, w.c.k_scale, row, w.c.dh, col);
+      ev = read8<KIND>(w.c.v, w.c.v_scale, row, w.c.dh, col);
+    }
+    const size_t at = (static_cast<size_t>(blockIdx.x) * max_len + pos) * w.c.dh + col;
+    write8<DST_BF16>(k, at, ek);
+    write8<DST_BF16>(v, at, ev);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// One warp per (row, query head): positions in turn, a lane per four elements of the head.
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) paged_attention_simple_kernel(const View w, const __nv_bfloat16* __restrict__ q,
+                                                                          long long q_st, long long q_sh,
+                                                                          __nv_bfloat16* __restrict__ out, int Hq,
+                                                                          int window, int sinks, float scale) {
+  const long long g = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31, dh = w.c.dh;
+  if (g >= static_cast<long long>(w.c.N) * Hq) return;
+  const int t = static_cast<int>(g / Hq), hq = static_cast<int>(g - static_cast<long long>(t) * Hq);
+  const int h = hq / (Hq / w.c.H), b = seq_of_row(w, t), c0 = 8 * (lane & 15);
+  const bool on = c0 < dh && lane < 16;
+  float m = -3.0e38f, l = 0.f, o[8], qf[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = qf[i] = 0.f;
+  if (on) bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(q + t * q_st + hq * q_sh + c0)), qf);
+  if (b >= 0) {
+    const Rows r = seq_rows(w, b);
+    const int last = seq_length(w, b) - r.count + (t - r.first);
+    for (int j = 0; j <= last; ++j) {
+      if (window > 0 && j <= last - window && j >= sinks) continue;
+      const int page = page_of(w, b, j);
+      if (page < 0) continue;
+      const size_t row = slot_row(w, page, h, j);
+      Eight k, v;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
+      if (on) {
+        k = read8<KIND>(w.c.k, w.c.k_scale, row, dh, c0);
+        v = read8<KIND>(w.c.v, w.c.v_scale, row, dh, c0);
+      }
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(qf[i], k.f[i], s);
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      s *= scale;
+      const float mn = fmaxf(m, s), f = __expf(m - mn), e = __expf(s - mn);
+      l = fmaf(l, f, e);
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], f, e * v.f[i]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (on) {
+    Eight e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e.f[i] = o[i] * inv;
+    write8<true>(out, (static_cast<size_t>(t) * Hq + hq) * dh + c0, e);
+  }
+}
+
+template <int KIND, bool SRC_BF16>
+int launch_write(const View& w, const void* k, const void* v, long long k_st, long long k_sh, long long v_st,
+                 long long v_sh, cudaStream_t stream) {
+  const int lpr = lanes_per_row(w.c.dh);
+  const long long groups = static_cast<long long>(w.c.N) * w.c.H;
+  const long long blocks = (groups * lpr + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffLL) return 932;
+  const unsigned n = static_cast<unsigned>(blocks);
+#define DSB_WRITE(L) paged_write_kernel<KIND, SRC_BF16, L><<<n, kThreads, 0, stream>>>(w, k, v, k_st, k_sh, v_st, v_sh)
+  if (lpr == 2) DSB_WRITE(2);
+  else if (lpr == 4) DSB_WRITE(4);
+  else if (lpr == 8) DSB_WRITE(8);
+  else DSB_WRITE(16);
+#undef DSB_WRITE
+  return cudaGetLastError() == cudaSuccess ? 0 : 933;
+}
+
+template <int KIND, bool DST_BF16>
+int launch_read(const View& w, void* k, void* v, int max_len, cudaStream_t stream) {
+  const int lpr = lanes_per_row(w.c.dh), per = kThreads / lpr;
+  const long long bh = static_cast<long long>(w.c.B) * w.c.H;
+  if (bh > 0x7fffffffLL) return 935;
+  long long y = (static_cast<long long>(max_len) + per - 1) / per;
+  if (y > 65535) y = 65535;
+  const dim3 grid(static_cast<unsigned>(bh), static_cast<unsigned>(y));
+#define DSB_READ(L) paged_read_kernel<KIND, DST_BF16, L><<<grid, kThreads, 0, stream>>>(w, k, v, max_len)
+  if (lpr == 2) DSB_READ(2);
+  else if (lpr == 4) DSB_READ(4);
+  else if (lpr == 8) DSB_READ(8);
+  else DSB_READ(16);
+#undef DSB_READ
+  return cudaGetLastError() == cudaSuccess ? 0 : 936;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace dsb
+
+using namespace dsb::paged;
+
+extern "C" int dsb_paged_write(const DsbPaged* c, const void* k, const void* v, int src_bf16, long long k_st,
+                               long long k_sh, long long v_st, long long v_sh, cudaStream_t stream) {
+  if (bad_cache(c)) return 930;
+  const int step = src_bf16 ? 8 : 4;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0 || k_st % step || k_sh % step ||
+      v_st % step || v_sh % step)
+    return 931;
+  if (c->N == 0 || c->B == 0) return 0;
+  const View w = make_view(c);
+#define DSB_KIND(K)                                                                     \
+  (src_bf16 ? launch_write<K, true>(w, k, v, k_st, k_sh, v_st, v_sh, stream)            \
+            : launch_write<K, false>(w, k, v, k_st, k_sh, v_st, v_sh, stream))
+  if (c->kind == kBf16) return DSB_KIND(kBf16);
+  if (c->kind == kE4m3) return DSB_KIND(kE4m3);
+  return DSB_KIND(kInt8);
+#undef DSB_KIND
+}
+
+extern "C" int dsb_paged_read(const DsbPaged* c, void* k, void* v, int dst_bf16, int max_len, cudaStream_t stream) {
+  if (bad_cache(c) || max_len < 0) return 934;
+  if (c->B == 0 || max_len == 0) return 0;
+  const View w = make_view(c);
+#define DSB_KIND(K) (dst_bf16 ? launch_read<K, true>(w, k, v, max_len, stream) : launch_read<K, false>(w, k, v, max_len, stream))
+  if (c->kind == kBf16) return DSB_KIND(kBf16);
+  if (c->kind == kE4m3) return DSB_KIND(kE4m3);
+  return DSB_KIND(kInt8);
+#undef DSB_KIND
+}
+
+extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
+                                   int window, int sinks, float scale, cudaStream_t stream) {
+  if (bad_cache(c) || Hq <= 0 || Hq % c->H != 0 || window < 0 || sinks < 0) return 940;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8) return 941;
+  if (c->N == 0) return 0;
+  const View w = make_view(c);
+  const long long blocks = (static_cast<long long>(c->N) * Hq * 32 + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffffLL) return 942;
+  const unsigned n = static_cast<unsigned>(blocks);
+  const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
+  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
+  if (c->kind == kBf16) paged_attention_simple_kernel<kBf16><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
+  else if (c->kind == kE4m3) paged_attention_simple_kernel<kE4m3><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
+  else paged_attention_simple_kernel<kInt8><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
+  return cudaGetLastError() == cudaSuccess ? 0 : 943;
+}

@@ -78,7 +78,8 @@ def check_status(device=None) -> None:
         if code != 0:
             st.zero_()
             raise RuntimeError(f"dawn_srw_b200 kernel reported status {code} on cuda:{key} "
-                               "(1 = barrier wait timed out, 3 = peer wait timed out)")
+                               "(1 = barrier wait timed out, 3 = peer wait timed out, "
+                               "4 = a length or a table entry outside the paged cache)")
 
 
 _PENDING = {}
@@ -100,7 +101,8 @@ def check_status_deferred() -> None:
                 st.zero_()
                 _PENDING.pop(key, None)
                 raise RuntimeError(f"dawn_srw_b200 kernel reported status {code} on cuda:{key} "
-                                   "(1 = barrier wait timed out, 3 = peer wait timed out)")
+                                   "(1 = barrier wait timed out, 3 = peer wait timed out, "
+                                   "4 = a length or a table entry outside the paged cache)")
             host_buf = host
         else:
             host_buf = torch.zeros(1, dtype=torch.int32).pin_memory()
@@ -109,6 +111,11 @@ def check_status_deferred() -> None:
             ev = torch.cuda.Event()
             ev.record()
         _PENDING[key] = (ev, host_buf)
+
+
+def _paged_status(pages):
+    """Status word for the pages' device; of CPU pages a stand-in (the binding refuses them after all else)."""
+    return status_word(pages.device) if pages.is_cuda else torch.zeros(1, dtype=torch.int32)
 
 
 def _gate_list(spec: GateSpec) -> List[float]:
@@ -973,6 +980,39 @@ class CudaBackend:
         f = lambda t: t.float().contiguous()
         count_launches(2)
         return ext().prompt_attention(f(q), f(k), f(v), cache_k, cache_v, B, S, status_word(q.device))
+
+    # ---- paged key/value cache (layouts, types and bounds: ops/paged.py) ----
+    @torch.no_grad()
+    def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
+        """Keys and values [N, H, dh] (fp32 or bf16) of new tokens into their pages, rounded to the pages'
+        type.  One launch; rows of no sequence, and positions whose table entry names no page, are left
+        out (the latter sets the status word)."""
+        count_launches(1)
+        ext().paged_write(k, v, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, _paged_status(k_pages))
+
+    @torch.no_grad()
+    def paged_read(self, k_pages, v_pages, table, lengths, max_len: int, k_scale=None, v_scale=None,
+                   dtype=torch.float32):
+        """Pages back to dense k, v [B, H, max_len, dh], zeros at and behind a sequence's length."""
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("paged cache: dtype must be float32 or bfloat16")
+        count_launches(1)
+        return tuple(ext().paged_read(k_pages, v_pages, table, lengths, int(max_len), k_scale, v_scale,
+                                      dtype == torch.bfloat16, _paged_status(k_pages)))
+
+    @torch.no_grad()
+    def paged_attention(self, q, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None, *,
+                        max_new: Optional[int] = None, window: Optional[int] = None, sinks: int = 0,
+                        scale: Optional[float] = None):
+        """Attention of the new tokens q [N, Hq, dh] over the pages of their sequences (their own keys and
+        values are written before): every key at or before the token's position, with ``window`` the last
+        ``window`` of them and the first ``sinks`` positions only.  ``Hq`` is a multiple of the pages'
+        heads; ``max_new``, the largest number of new tokens of a sequence if the caller knows it, only
+        chooses the kernel.  Returns [N, Hq, dh] in bf16 (as ``attention``); zeros for a row that sees no
+        key or belongs to no sequence."""
+        count_launches(1)
+        return ext().paged_attention(q, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, max_new,
+                                     window, sinks, scale, _paged_status(k_pages))
 
     def embed(self, ids, tok, pos):
         if tok.shape[1] % 4 != 0 or tok.dtype != torch.float32:
