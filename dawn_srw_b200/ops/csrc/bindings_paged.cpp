@@ -43,8 +43,8 @@ DsbPaged view(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTe
     c.v_scale = vs->data_ptr<float>();
   }
   REFUSE_UNLESS(table.dim() == 2 && table.scalar_type() == torch::kInt32 && table.is_contiguous() &&
-                    table.size(1) <= (0x7fffffffLL / page) - 1,
-                "table must be a contiguous int32 [sequences, pages]");
+                    table.size(1) <= (1 << 30) / page,
+                "table must be a contiguous int32 [sequences, pages] of at most 2^30 positions each");
   const int64_t B = table.size(0);
   REFUSE_UNLESS(lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == torch::kInt32 &&
                     lengths.is_contiguous(),
@@ -57,7 +57,7 @@ DsbPaged view(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTe
   } else {
     REFUSE_UNLESS(N == B, "without starts every sequence has one new token: ", N, " rows for ", B, " sequences");
   }
-  REFUSE_UNLESS(N <= 0x7fffffffLL && B <= 0x7fffffffLL - 1, "too many rows");
+  REFUSE_UNLESS(N <= (1 << 30) && B <= 65535, "more than 65535 sequences, or too many rows");
   REFUSE_UNLESS(v.device() == k.device() && table.device() == k.device() && lengths.device() == k.device(),
                 "pages, table and lengths must be on one device");
   REFUSE_UNLESS(k.is_cuda(), "the kernels need CUDA tensors");
@@ -142,10 +142,14 @@ Tensor paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, cons
   Tensor out = torch::empty({q.size(0), Hq, q.size(2)}, kp.options().dtype(torch::kBFloat16));
   const int64_t top = 0x7fffffffLL;
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
+  const int hint = static_cast<int>(std::min<int64_t>(max_new.has_value() ? *max_new : starts.has_value() ? q.size(0) : 1, top));
+  const int64_t bytes = dsb_paged_attention_workspace(&c, static_cast<int>(Hq), hint);
+  Tensor ws;                    // of this call alone: captured graphs and streams share nothing
+  if (bytes > 0) ws = torch::empty({bytes}, kp.options().dtype(torch::kUInt8));
   const int rc = dsb_paged_attention(&c, qr.data_ptr(), qr.stride(0), qr.stride(1), out.data_ptr(), static_cast<int>(Hq),
-                                     window.has_value() ? static_cast<int>(std::min(*window, top)) : 0,
+                                     hint, window.has_value() ? static_cast<int>(std::min(*window, top)) : 0,
                                      static_cast<int>(std::min(sinks, top)), static_cast<float>(s),
-                                     at::cuda::getCurrentCUDAStream().stream());
+                                     bytes > 0 ? ws.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "dsb_paged_attention failed with code ", rc);
   return out;
 }

@@ -11,6 +11,8 @@ namespace paged {
 
 constexpr int kStatusBadPage = 4;   // a table entry or a length outside the cache
 
+constexpr int kMostPositions = 1 << 30;   // of a sequence, and packed rows: sums of two stay in 32 bits
+
 enum Kind { kBf16 = 0, kE4m3 = 1, kInt8 = 2 };
 
 struct View {
@@ -31,6 +33,7 @@ inline bool bad_cache(const DsbPaged* c) {
   if (c->kind < 0 || c->kind > 2 || c->dh < 16 || c->dh > 128 || c->dh % 16 != 0) return true;
   if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1)) != 0) return true;
   if (c->H <= 0 || c->n_pages < 0 || c->B < 0 || c->width < 0 || c->N < 0) return true;
+  if (c->N > kMostPositions || static_cast<long long>(c->width) * c->page > kMostPositions) return true;
   if (c->starts == nullptr && c->N != c->B) return true;
   if (c->kind != kBf16 && (c->k_scale == nullptr || c->v_scale == nullptr)) return true;
   return ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) != 0;

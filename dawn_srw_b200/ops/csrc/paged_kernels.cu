@@ -178,60 +178,6 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const View w, void
   }
 }
 
-// ---------------------------------------------------------------------------
-// One warp per (row, query head): positions in turn, a lane per four elements of the head.
-template <int KIND>
-__global__ void __launch_bounds__(kThreads) paged_attention_simple_kernel(const View w, const __nv_bfloat16* __restrict__ q,
-                                                                          long long q_st, long long q_sh,
-                                                                          __nv_bfloat16* __restrict__ out, int Hq,
-                                                                          int window, int sinks, float scale) {
-  const long long g = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31, dh = w.c.dh;
-  if (g >= static_cast<long long>(w.c.N) * Hq) return;
-  const int t = static_cast<int>(g / Hq), hq = static_cast<int>(g - static_cast<long long>(t) * Hq);
-  const int h = hq / (Hq / w.c.H), b = seq_of_row(w, t), c0 = 8 * (lane & 15);
-  const bool on = c0 < dh && lane < 16;
-  float m = -3.0e38f, l = 0.f, o[8], qf[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = qf[i] = 0.f;
-  if (on) bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(q + t * q_st + hq * q_sh + c0)), qf);
-  if (b >= 0) {
-    const Rows r = seq_rows(w, b);
-    const int last = seq_length(w, b) - r.count + (t - r.first);
-    for (int j = 0; j <= last; ++j) {
-      if (window > 0 && j <= last - window && j >= sinks) continue;
-      const int page = page_of(w, b, j);
-      if (page < 0) continue;
-      const size_t row = slot_row(w, page, h, j);
-      Eight k, v;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k.f[i] = v.f[i] = 0.f;
-      if (on) {
-        k = read8<KIND>(w.c.k, w.c.k_scale, row, dh, c0);
-        v = read8<KIND>(w.c.v, w.c.v_scale, row, dh, c0);
-      }
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(qf[i], k.f[i], s);
-#pragma unroll
-      for (int x = 1; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= scale;
-      const float mn = fmaxf(m, s), f = __expf(m - mn), e = __expf(s - mn);
-      l = fmaf(l, f, e);
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], f, e * v.f[i]);
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (on) {
-    Eight e;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.f[i] = o[i] * inv;
-    write8<true>(out, (static_cast<size_t>(t) * Hq + hq) * dh + c0, e);
-  }
-}
-
 template <int KIND, bool SRC_BF16>
 int launch_write(const View& w, const void* k, const void* v, long long k_st, long long k_sh, long long v_st,
                  long long v_sh, cudaStream_t stream) {
@@ -299,21 +245,4 @@ extern "C" int dsb_paged_read(const DsbPaged* c, void* k, void* v, int dst_bf16,
   if (c->kind == kE4m3) return DSB_KIND(kE4m3);
   return DSB_KIND(kInt8);
 #undef DSB_KIND
-}
-
-extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
-                                   int window, int sinks, float scale, cudaStream_t stream) {
-  if (bad_cache(c) || Hq <= 0 || Hq % c->H != 0 || window < 0 || sinks < 0) return 940;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8) return 941;
-  if (c->N == 0) return 0;
-  const View w = make_view(c);
-  const long long blocks = (static_cast<long long>(c->N) * Hq * 32 + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return 942;
-  const unsigned n = static_cast<unsigned>(blocks);
-  const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
-  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
-  if (c->kind == kBf16) paged_attention_simple_kernel<kBf16><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
-  else if (c->kind == kE4m3) paged_attention_simple_kernel<kE4m3><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
-  else paged_attention_simple_kernel<kInt8><<<n, kThreads, 0, stream>>>(w, qb, q_st, q_sh, ob, Hq, window, sinks, scale);
-  return cudaGetLastError() == cudaSuccess ? 0 : 943;
 }
