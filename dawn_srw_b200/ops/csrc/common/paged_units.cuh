@@ -25,6 +25,7 @@ struct Unit {
   int len, n, first;                // length, new tokens, first packed row of the sequence
   int rows;                         // rows of this tile
   int lo, hi, s_end;
+  int lo_all, hi_all;               // [lo_all, hi_all): positions that every row of the tile sees (may be none)
   int st, skip, tiles;              // tile t of the unit is position tile t (t < st) or t + skip
 };
 
@@ -42,6 +43,8 @@ __device__ __forceinline__ void unit_range(const AttnParams& p, Unit& u) {
   u.lo = max(0, p_lo - p.window + 1);             // p_lo >= -N, N and window at most 2^30: no overflow
   u.lo = min(u.lo, u.hi);
   u.s_end = min(p.sinks, u.lo);
+  u.lo_all = max(0, p_hi - p.window + 1);
+  u.hi_all = p_lo + 1;
   u.st = (u.s_end + TP - 1) / TP;
   const int t_lo = max(u.lo / TP, u.st), t_hi = (u.hi + TP - 1) / TP;
   u.skip = t_lo - u.st;

@@ -1,19 +1,18 @@
 // Attention of a few query rows per key/value head (single tokens, drafted ones) over a paged cache.
 //
-// A warp streams tiles of positions straight from global memory into matrix-instruction fragments:
-//   S^T [positions, rows] = K Q^T        m16n8k16, K the M side: eight rows fill the N side, so that one row costs
-//                                        the same as eight and a tile's scores need no shared memory;
-//   O^T [dh, rows]       += V^T P^T      V^T the M side; the transposed P comes from movmatrix, the transposed V
-//                                        from pairs of rows interleaved with byte permutes.
-// Any order of the contraction will do as long as both operands have it, so a lane takes eight neighbouring
-// elements of a row (16 bytes of bf16, 8 of codes) where the fragment wants pairs 2t, 2t+1, 2t+8, 2t+9; 8-bit codes
-// become bf16 in registers, exactly, their scales go to the scores and the weights in fp32.  The running maximum and
-// sum of the softmax stay in registers.
+// Each warp streams tiles of positions through a ring of its own in shared memory (16-byte asynchronous copies; the
+// sixteen positions of a head in a page are contiguous) and multiplies with m16n8k16 instructions:
+//   S^T [positions, rows] = K Q^T        K the M side: eight rows fill the N side, so that one row costs what eight do
+//                                        and the scores of a tile stay in registers;
+//   O^T [dh, rows]       += V^T P^T      V^T the M side, by transposing ldmatrix; P is transposed by movmatrix.
+// 8-bit codes go through ldmatrix as pairs and become bf16 in registers, exactly; any order of the contraction will
+// do as long as both operands have it, so a lane's queries are those of the four neighbouring codes it gets.  Scales
+// of positions go to the scores and the weights in fp32.  Running maximum and sum stay in registers.
 //
-// Two ways to share the work (kSplit): short caches take one block per unit, its warps interleaved over the tiles
-// and merged in shared memory: one launch.  Long ones take as many warps as the GPU holds, each with an equal run of
-// consecutive tiles of all units; a unit that several warps share is left in pieces, which a second kernel adds up in
-// order.  The lengths are read on the device, so a captured call follows them.
+// Two ways to share the work: short caches take one block per unit, its warps interleaved over the tiles and merged
+// in shared memory: one launch.  Long ones take as many warps as the GPU holds, each with an equal run of consecutive
+// tiles of all units; a unit that several warps share is left in pieces, which a second kernel adds up in order.  The
+// lengths are read on the device, so a captured call follows them.
 #include "common/paged_units.cuh"
 #include "common/ptx.cuh"
 
@@ -41,55 +40,64 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Eight elements of a row as they lie in memory.
-template <int KIND> struct Raw { uint2 v; };
-template <> struct Raw<kBf16> { uint4 v; };
+__device__ __forceinline__ void ldmatrix(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes to shared memory; zeros where `on` is false (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// The four codes that ldmatrix gives a lane, as bf16: neighbours (K), or of two positions by column (V transposed).
 template <int KIND>
-__device__ __forceinline__ void clear(Raw<KIND>& r) { r.v = make_uint2(0u, 0u); }
-template <>
-__device__ __forceinline__ void clear<kBf16>(Raw<kBf16>& r) { r.v = make_uint4(0u, 0u, 0u, 0u); }
-
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-template <int KIND>
-__device__ __forceinline__ Raw<KIND> load_raw(const void* pool, size_t elem) {
-  Raw<KIND> r;
-  r.v = ldg8(static_cast<const uint8_t*>(pool) + elem);
-  return r;
-}
-template <>
-__device__ __forceinline__ Raw<kBf16> load_raw<kBf16>(const void* pool, size_t elem) {
-  Raw<kBf16> r;
-  r.v = ldg16(static_cast<const __nv_bfloat16*>(pool) + elem);
-  return r;
-}
-template <int KIND>
-__device__ __forceinline__ void words(const Raw<KIND>& r, uint32_t* o) {
-  const uint2 a = codes_to_bf16<KIND>(r.v.x), b = codes_to_bf16<KIND>(r.v.y);
-  o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
-}
-template <>
-__device__ __forceinline__ void words<kBf16>(const Raw<kBf16>& r, uint32_t* o) {
-  o[0] = r.v.x; o[1] = r.v.y; o[2] = r.v.z; o[3] = r.v.w;
+__device__ __forceinline__ uint32_t pair_to_bf16(uint32_t p) {
+  if (KIND == kInt8) {
+    const uint32_t a = (p & 0x007f007fu) | 0x43004300u, b = (p & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+  const uint32_t a = ((p & 0x007f007fu) << 4) | ((p & 0x00800080u) << 8), s = 0x7b807b80u;   // 2^120 twice
+  const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&s));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// One warp's state for a unit: NT tiles of eight rows.  Lane (g, t) = (lane / 4, lane % 4) holds rows 2t and 2t+1 of
-// a tile and, of O^T, the eight elements 64 jj + 8 g ..; its queries are row g's.
-template <int KIND, int DC, int NT, int MT>
+// Shared memory of a warp: kStages tiles of keys, values and scales.  Rows are an odd number of 16-byte words
+// apart, so that the eight rows of an ldmatrix fall on different banks.
+template <int KIND, int KD>
+struct Ring {
+  static constexpr int kMT = KIND == kBf16 && KD > 4 ? 1 : 2;           // sixteens of positions in a tile
+  static constexpr int kTP = 16 * kMT;
+  static constexpr int kElem = KIND == kBf16 ? 2 : 1;
+  static constexpr int kRowMost = ((KD * kElem) | 1) * 16;
+  static constexpr int kScale = 2 * kTP * kRowMost;                     // scales behind the rows
+  static constexpr int kStage = kScale + (KIND == kBf16 ? 0 : 2 * kTP * 4);
+  // twelve warps fit an SM with a ring of 18.9 KB each
+  static constexpr int kStages = 4 * kStage <= 18944 ? 4 : 3 * kStage <= 18944 ? 3 : 2;
+  static constexpr int kBytes = kStages * kStage;
+  static_assert(kBytes <= 18944, "three blocks of four warps have to fit an SM");
+};
+
+// One warp's state for a unit: NT tiles of eight rows.  Lane (g, t) = (lane / 4, lane % 4) holds rows 2t and 2t + 1
+// of a tile and of O^T the columns column(c, 0), column(c, 1) of sixteen c; its queries are row g's.
+template <int KIND, int KD, int NT>
 struct Warp {
-  static constexpr int kRows = 8 * NT, kTP = 16 * MT, kJ = (DC + 1) / 2;
-  uint32_t q[NT][DC][4];
-  float o[NT][kJ][4][4];
+  using R = Ring<KIND, KD>;
+  static constexpr int kRows = 8 * NT, kTP = R::kTP, kMT = R::kMT;
+  uint32_t q[NT][KD][2];
+  float o[NT][KD][4];
   float m[NT][2], l[NT][2];
+
+  static __device__ __forceinline__ int column(int c, int e, int g) {
+    return KIND == kBf16 ? 16 * c + 8 * e + g : 16 * c + 2 * g + e;
+  }
 
   __device__ __forceinline__ void begin(const AttnParams& p, const Unit& u, int g, int t) {
 #pragma unroll
@@ -99,25 +107,29 @@ struct Warp {
       const __nv_bfloat16* row = p.q;
       if (live) row += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
 #pragma unroll
-      for (int j = 0; j < DC; ++j) {
-        const int col = 32 * j + 8 * t;
-        const uint4 v = live && col < p.w.c.dh ? __ldg(reinterpret_cast<const uint4*>(row + col)) : make_uint4(0u, 0u, 0u, 0u);
-        q[nt][j][0] = v.x; q[nt][j][1] = v.y; q[nt][j][2] = v.z; q[nt][j][3] = v.w;
+      for (int k = 0; k < KD; ++k) {
+        const bool on = live && 16 * k < p.w.c.dh;
+        if (KIND == kBf16) {
+          q[nt][k][0] = on ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * k + 2 * t)) : 0u;
+          q[nt][k][1] = on ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * k + 8 + 2 * t)) : 0u;
+        } else {
+          const uint2 v = on ? __ldg(reinterpret_cast<const uint2*>(row + 16 * k + 4 * t)) : make_uint2(0u, 0u);
+          q[nt][k][0] = v.x;
+          q[nt][k][1] = v.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][k][e] = 0.f;
       }
       m[nt][0] = m[nt][1] = kFloor;
       l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-      for (int jj = 0; jj < kJ; ++jj)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][jj][c][e] = 0.f;
     }
   }
 
-  // Tiles t0, t0 + step, .. below t1 of the unit.
-  __device__ void run(const AttnParams& p, const Unit& u, int t0, int t1, int step, int lane) {
+  // Tiles t0, t0 + step, .. below t1 of the unit; ring: this warp's shared memory.
+  __device__ void run(const AttnParams& p, const Unit& u, int t0, int t1, int step, int lane, uint32_t ring) {
     const int g = lane >> 2, t = lane & 3, dh = p.w.c.dh, shift = p.w.shift;
+    const int wpr = dh * R::kElem >> 4, row_b = (wpr | 1) << 4;          // 16-byte words of a row, bytes between rows
+    const int steps = dh >> 4, per_word = 65536 / wpr + 1;
     int pos_of[NT][2];                                   // positions of this lane's rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -127,11 +139,12 @@ struct Warp {
         pos_of[nt][e] = r < u.rows ? u.len - u.n + (u.rt * kRows + r) / p.G : -1;
       }
     const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
-    // lane i < MT: the page of the tile's i-th sixteen positions, -1 where no row sees any of them
+    auto place = [&](int tile) { return (tile < u.st ? tile : tile + u.skip) * kTP; };
+    // lane i < kMT: the page of the tile's i-th sixteen positions, -1 where no row sees any of them
     auto page_ids = [&](int tile) {
       int id = -1;
-      const int x = (tile < u.st ? tile : tile + u.skip) * kTP + 16 * lane;
-      if (lane < MT && tile < t1 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
+      const int x = place(tile) + 16 * lane;
+      if (lane < kMT && tile < t1 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
         id = __ldg(table + (x >> shift));
         if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
           atomicExch(p.w.c.status, kStatusBadPage);
@@ -140,78 +153,146 @@ struct Warp {
       }
       return id;
     };
-    int ids = page_ids(t0);
-    for (int tile = t0; tile < t1; tile += step) {
-      const int x0 = (tile < u.st ? tile : tile + u.skip) * kTP;
-      Raw<KIND> kr[MT][2][DC], vr[MT][4][kJ];
-      float ks[MT][2], vs[MT][2];
-      uint32_t live = 0;                                 // bit 2 mt + e: position x0 + 16 mt + 8 e + g may be seen
+    uint32_t absent[R::kStages];                         // bit mt: the sixteen positions have no page
+    auto issue = [&](int tile, int slot, int ids) {
+      uint32_t gone = 0;
+      if (tile < t1) {
+        const int x0 = place(tile);
+        const uint32_t kdst = ring + slot * R::kStage, vdst = kdst + kTP * row_b;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int id = __shfl_sync(0xffffffffu, ids, mt), x = x0 + 16 * mt;
-        const size_t base = ((static_cast<size_t>(max(id, 0)) * p.w.c.H + u.h) << shift) + (x & (p.w.c.page - 1));
-        auto seen = [&](int i) { return id >= 0 && x + i < u.hi && (x + i >= u.lo || x + i < u.s_end); };
+        for (int mt = 0; mt < kMT; ++mt) {
+          const int id = __shfl_sync(0xffffffffu, ids, mt), x = x0 + 16 * mt;
+          gone |= static_cast<uint32_t>(id < 0) << mt;
+          const size_t base = ((static_cast<size_t>(max(id, 0)) * p.w.c.H + u.h) << shift) + (x & (p.w.c.page - 1));
+          const char* ks = static_cast<const char*>(p.w.c.k) + base * dh * R::kElem;
+          const char* vs = static_cast<const char*>(p.w.c.v) + base * dh * R::kElem;
+          const bool all = id >= 0 && x + 16 <= u.hi && x >= u.lo;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool on = seen(g + 8 * e);
-          live |= static_cast<uint32_t>(on) << (2 * mt + e);
-#pragma unroll
-          for (int j = 0; j < DC; ++j) {
-            clear(kr[mt][e][j]);
-            if (on && 32 * j + 8 * t < dh) kr[mt][e][j] = load_raw<KIND>(p.w.c.k, (base + g + 8 * e) * dh + 32 * j + 8 * t);
+          for (int c = 0; c < (16 * KD * R::kElem + 31) / 32; ++c) {
+            const int i = lane + 32 * c;
+            if (i >= 16 * wpr) break;
+            const int row = (i * per_word) >> 16;        // i / wpr: exact for i < 256, wpr <= 16
+            const uint32_t off = (16 * mt + row) * row_b + ((i - row * wpr) << 4);
+            const bool on = all || (id >= 0 && x + row < u.hi && (x + row >= u.lo || x + row < u.s_end));
+            copy16(kdst + off, ks + 16 * i, on);
+            copy16(vdst + off, vs + 16 * i, on);
           }
-          ks[mt][e] = vs[mt][e] = 1.f;
-          if (KIND != kBf16 && on) {
-            ks[mt][e] = __ldg(p.w.c.k_scale + base + g + 8 * e);
-            vs[mt][e] = __ldg(p.w.c.v_scale + base + g + 8 * e);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {                    // positions 2t, 2t+1, 2t+8, 2t+9: the fragment's own order
-          const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-          const bool on = seen(row);
-#pragma unroll
-          for (int jj = 0; jj < kJ; ++jj) {
-            clear(vr[mt][i][jj]);
-            if (on && 64 * jj + 8 * g < dh) vr[mt][i][jj] = load_raw<KIND>(p.w.c.v, (base + row) * dh + 64 * jj + 8 * g);
+          if (KIND != kBf16 && lane < 8) {
+            const float* src = (lane < 4 ? p.w.c.k_scale : p.w.c.v_scale) + base + 4 * (lane & 3);
+            copy16(ring + slot * R::kStage + R::kScale + ((lane < 4 ? 0 : kTP) + 16 * mt + 4 * (lane & 3)) * 4, src, id >= 0);
           }
         }
       }
-      ids = page_ids(tile + step);                       // one tile ahead of the loads that need them
+      copies_commit();
+      return gone;
+    };
+    // S - 1 tiles ahead of the one in work; page ids one tile ahead of the copies that need them
+    int next = t0, ids = page_ids(t0);
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) {
+      const int now = ids;
+      ids = page_ids(next + step);
+      absent[i] = issue(next, i, now);
+      next += step;
+    }
+    // rows of an ldmatrix: K: positions (lane & 7) + 8 (bit 3), words by bit 4; V: positions by bit 4 (bf16) or 3
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_word = lane >> 4;
+    const int v_row = (lane & 7) + (KIND == kBf16 ? (lane >> 4) * 8 : ((lane >> 3) & 1) * 8);
+    const int v_word = KIND == kBf16 ? (lane >> 3) & 1 : lane >> 4;
+    int slot = 0;
+    for (int tile = t0; tile < t1; tile += step) {
+      copies_wait<R::kStages - 2>();
+      __syncwarp();
+      const uint32_t gone = absent[0];
+      {
+        const int now = ids;
+        ids = page_ids(next + step);
+        const uint32_t more = issue(next, slot == 0 ? R::kStages - 1 : slot - 1, now);
+        next += step;
+#pragma unroll
+        for (int i = 0; i + 2 < R::kStages; ++i) absent[i] = absent[i + 1];
+        absent[R::kStages - 2] = more;
+      }
+      const int x0 = place(tile);
+      const uint32_t kst = ring + slot * R::kStage, vst = kst + kTP * row_b;
+      const uint32_t sst = kst + R::kScale;
       // ---- scores
-      float s[NT][MT][4];
+      float s[NT][kMT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
+        for (int mt = 0; mt < kMT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt) {
+        const uint32_t at = kst + (16 * mt + k_row) * row_b + 16 * k_word;
+        if (KIND == kBf16) {
 #pragma unroll
-        for (int j = 0; j < DC; ++j) {
-          uint32_t a[4], b[4];
-          words<KIND>(kr[mt][0][j], a);
-          words<KIND>(kr[mt][1][j], b);
+          for (int k = 0; k < KD; ++k) {
+            if (k < steps) {
+              uint32_t a[4];
+              ldmatrix(at + 32 * k, a);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816(s[nt][mt], a[0], b[0], a[1], b[1], q[nt][j][0], q[nt][j][1]);
-            mma16816(s[nt][mt], a[2], b[2], a[3], b[3], q[nt][j][2], q[nt][j][3]);
+              for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][mt], a[0], a[1], a[2], a[3], q[nt][k][0], q[nt][k][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KD; k += 2) {
+            if (k < steps) {
+              uint32_t a[4];
+              ldmatrix(at + 16 * k, a);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (k + e < KD && k + e < steps) {
+                  const uint2 lo = codes_to_bf16<KIND>(a[2 * e]), hi = codes_to_bf16<KIND>(a[2 * e + 1]);
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816(s[nt][mt], lo.x, hi.x, lo.y, hi.y, q[nt][k + e][0], q[nt][k + e][1]);
+                }
+              }
+            }
           }
         }
+      }
       // ---- weights: s[.][.][c] is position g + 8 (c / 2), row 2t + c % 2
-      uint32_t pt[NT][MT][2];
+      float ks[kMT][2], vs[kMT][2];
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          ks[mt][e] = p.scale_log2;
+          vs[mt][e] = 1.f;
+          if (KIND != kBf16) {
+            float a, b;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(sst + (16 * mt + 8 * e + g) * 4) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(sst + (kTP + 16 * mt + 8 * e + g) * 4) : "memory");
+            ks[mt][e] *= a;
+            vs[mt][e] = b;
+          }
+        }
+      const bool open = gone == 0u && x0 >= u.lo_all && x0 + kTP <= u.hi_all;     // every row sees every position
+      uint32_t pt[NT][kMT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float top[2] = {kFloor, kFloor};
-        uint32_t vis = 0;
+        uint32_t vis = 0xffffffffu;
+        if (!open) {
+          vis = 0;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+          for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int x = x0 + 16 * mt + g + 8 * (c >> 1), pr = pos_of[nt][c & 1];
+              const bool on = ((gone >> mt) & 1u) == 0u && x <= pr && (x > pr - p.window || x < p.sinks);
+              vis |= static_cast<uint32_t>(on) << (4 * mt + c);
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int x = x0 + 16 * mt + g + 8 * (c >> 1), pr = pos_of[nt][c & 1];
-            const bool on = ((live >> (2 * mt + (c >> 1))) & 1u) && x <= pr && (x > pr - p.window || x < p.sinks);
-            vis |= static_cast<uint32_t>(on) << (4 * mt + c);
-            s[nt][mt][c] *= p.scale_log2 * ks[mt][c >> 1];
-            if (on) top[c & 1] = fmaxf(top[c & 1], s[nt][mt][c]);
+            s[nt][mt][c] *= ks[mt][c >> 1];
+            if ((vis >> (4 * mt + c)) & 1u) top[c & 1] = fmaxf(top[c & 1], s[nt][mt][c]);
           }
         float f[2];
 #pragma unroll
@@ -225,20 +306,18 @@ struct Warp {
         }
         if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-          for (int jj = 0; jj < kJ; ++jj)
+          for (int c = 0; c < KD; ++c)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][jj][c][e] *= f[e & 1];
+            for (int e = 0; e < 4; ++e) o[nt][c][e] *= f[e & 1];
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < kMT; ++mt) {
           float w[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             w[c] = (vis >> (4 * mt + c)) & 1u ? exp2_fast(s[nt][mt][c] - m[nt][c & 1]) : 0.f;
             l[nt][c & 1] += w[c];
-            if (KIND != kBf16) w[c] = w[c] > 0.f ? w[c] * vs[mt][c >> 1] : w[c];
+            if (KIND != kBf16) w[c] = (vis >> (4 * mt + c)) & 1u ? w[c] * vs[mt][c >> 1] : 0.f;
           }
           // the one rounding of a weight (to bf16, with its position's scale): 2^-8 at most
           pt[nt][mt][0] = transpose8x8(pack_bf16x2(w[0], w[1]));
@@ -247,21 +326,43 @@ struct Warp {
       }
       // ---- O^T += V^T P^T
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt) {
+        const uint32_t at = vst + (16 * mt + v_row) * row_b + 16 * v_word;
+        if (KIND == kBf16) {
 #pragma unroll
-        for (int jj = 0; jj < kJ; ++jj) {
-          uint32_t r[4][4];
+          for (int c = 0; c < KD; ++c) {
+            if (c < steps) {
+              uint32_t a[4];
+              ldmatrix_t(at + 32 * c, a);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) words<KIND>(vr[mt][i][jj], r[i]);
+              for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][c], a[0], a[1], a[2], a[3], pt[nt][mt][0], pt[nt][mt][1]);
+            }
+          }
+        } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t a0 = __byte_perm(r[0][c], r[1][c], 0x5410), a1 = __byte_perm(r[0][c], r[1][c], 0x7632);
-            const uint32_t a2 = __byte_perm(r[2][c], r[3][c], 0x5410), a3 = __byte_perm(r[2][c], r[3][c], 0x7632);
+          for (int c = 0; c < KD; c += 2) {
+            if (c < steps) {
+              uint32_t a[4];
+              ldmatrix_t(at + 16 * c, a);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][jj][c], a0, a1, a2, a3, pt[nt][mt][0], pt[nt][mt][1]);
+              for (int e = 0; e < 2; ++e) {
+                if (c + e < KD && c + e < steps) {
+                  const uint32_t a0 = pair_to_bf16<KIND>(__byte_perm(a[2 * e], 0u, 0x4240)),
+                                 a1 = pair_to_bf16<KIND>(__byte_perm(a[2 * e], 0u, 0x4341)),
+                                 a2 = pair_to_bf16<KIND>(__byte_perm(a[2 * e + 1], 0u, 0x4240)),
+                                 a3 = pair_to_bf16<KIND>(__byte_perm(a[2 * e + 1], 0u, 0x4341));
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][c + e], a0, a1, a2, a3, pt[nt][mt][0], pt[nt][mt][1]);
+                }
+              }
+            }
           }
         }
+      }
+      slot = slot + 1 == R::kStages ? 0 : slot + 1;
     }
+    copies_wait<0>();
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -269,33 +370,21 @@ struct Warp {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
   }
-
-  // This lane's eight elements (from column 64 jj + 8 g) of row 8 nt + 2 t + e.
-  __device__ __forceinline__ void eight(int nt, int jj, int e, float* f) const {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      f[2 * c] = o[nt][jj][c][e];
-      f[2 * c + 1] = o[nt][jj][c][2 + e];
-    }
-  }
 };
 
 __device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) {
   return p.out + (static_cast<size_t>(u.first + row / p.G) * p.Hq + u.h * p.G + row % p.G) * p.w.c.dh;
 }
 
-__device__ __forceinline__ uint4 pack8(const float* f, float s) {
-  return make_uint4(pack_bf16x2(f[0] * s, f[1] * s), pack_bf16x2(f[2] * s, f[3] * s), pack_bf16x2(f[4] * s, f[5] * s),
-                    pack_bf16x2(f[6] * s, f[7] * s));
-}
-
 // One block per unit: grid (row tiles, heads, sequences); more row tiles than the grid has are taken in turn.
-template <int KIND, int DC, int NT, int MT>
-__global__ void __launch_bounds__(32 * kWarps) paged_few_block_kernel(const AttnParams p) {
-  using W = Warp<KIND, DC, NT, MT>;
-  __shared__ float s_o[kWarps][W::kRows][16 * 8 + 4];
+template <int KIND, int KD, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const AttnParams p) {
+  using W = Warp<KIND, KD, NT>;
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_ml[kWarps][W::kRows][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
+  const int ld = dh + 4;                               // of a row of O: the merge's rows fall on different banks
+  float* s_o = reinterpret_cast<float*>(smem);         // [kWarps][kRows][ld], over the rings once they are read
   if (blockIdx.x == 0 && blockIdx.y == 0) zero_other_rows(p, blockIdx.z * blockDim.x + threadIdx.x, gridDim.z * blockDim.x);
   Unit u;
   unit_sequence(p, u, blockIdx.z);
@@ -305,43 +394,45 @@ __global__ void __launch_bounds__(32 * kWarps) paged_few_block_kernel(const Attn
     unit_range<W::kRows, W::kTP>(p, u);
     W s;
     s.begin(p, u, g, t);
-    s.run(p, u, warp, u.tiles, kWarps, lane);
-    __syncthreads();                                   // the last unit's readers are done
+    s.run(p, u, warp, u.tiles, kWarps, lane, smem_u32(smem) + warp * W::R::kBytes);
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t + e;
 #pragma unroll
-        for (int jj = 0; jj < W::kJ; ++jj) {
-          float f[8];
-          s.eight(nt, jj, e, f);
-          float4* d = reinterpret_cast<float4*>(&s_o[warp][r][64 * jj + 8 * g]);
-          d[0] = make_float4(f[0], f[1], f[2], f[3]);
-          d[1] = make_float4(f[4], f[5], f[6], f[7]);
-        }
+        for (int c = 0; c < KD; ++c)
+          if (16 * c < dh) {
+            s_o[(warp * W::kRows + r) * ld + W::column(c, 0, g)] = s.o[nt][c][e];
+            s_o[(warp * W::kRows + r) * ld + W::column(c, 1, g)] = s.o[nt][c][2 + e];
+          }
         if (g == 0) {
           s_ml[warp][r][0] = s.m[nt][e];
           s_ml[warp][r][1] = s.l[nt][e];
         }
       }
     __syncthreads();
-    for (int i = threadIdx.x; i < u.rows * (dh / 8); i += blockDim.x) {
-      const int r = i / (dh / 8), c = 8 * (i - r * (dh / 8));
-      float top = kFloor, sum = 0.f, f[8];
+    for (int i = threadIdx.x; i < u.rows * (dh / 4); i += blockDim.x) {
+      const int r = i / (dh / 4), c = 4 * (i - r * (dh / 4));
+      float top = kFloor, sum = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][r][0]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = 0.f;
-#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float x = exp2_fast(s_ml[w][r][0] - top);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * W::kRows + r) * ld + c);
         sum = fmaf(x, s_ml[w][r][1], sum);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = fmaf(x, s_o[w][r][c + k], f[k]);
+        f[0] = fmaf(x, v.x, f[0]);
+        f[1] = fmaf(x, v.y, f[1]);
+        f[2] = fmaf(x, v.z, f[2]);
+        f[3] = fmaf(x, v.w, f[3]);
       }
-      *reinterpret_cast<uint4*>(out_row(p, u, u.rt * W::kRows + r) + c) = pack8(f, sum > 0.f ? 1.f / sum : 0.f);
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
+          make_uint2(pack_bf16x2(f[0] * inv, f[1] * inv), pack_bf16x2(f[2] * inv, f[3] * inv));
     }
+    __syncthreads();                                   // before the next unit's copies
   }
 }
 
@@ -396,9 +487,11 @@ constexpr int kLeastTiles = 2;
 // Equal runs of tiles for every warp.  Piece 2 i + 1 of worker i: a unit that begins in its run and ends in a later
 // one; piece 2 i: a unit that began in an earlier run.  meta[i] = {unit of piece 2 i + 1 or -1 .., rows | 1 << 16 if
 // piece 2 i ends its unit}.
-template <int KIND, int DC, int NT, int MT>
-__global__ void __launch_bounds__(32 * kWarps) paged_few_run_kernel(const AttnParams p) {
-  using W = Warp<KIND, DC, NT, MT>;
+template <int KIND, int KD, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const AttnParams p) {
+  using W = Warp<KIND, KD, NT>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * W::R::kBytes;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
   const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
   zero_other_rows(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
@@ -430,7 +523,7 @@ __global__ void __launch_bounds__(32 * kWarps) paged_few_run_kernel(const AttnPa
       const int t1 = static_cast<int>(min(static_cast<long long>(u.tiles), t0 + left));
       W s;
       s.begin(p, u, g, t);
-      s.run(p, u, t0, t1, 1, lane);
+      s.run(p, u, t0, t1, 1, lane, ring);
       const bool whole = t0 == 0 && t1 == u.tiles;
       float* piece = p.part + (2 * static_cast<size_t>(worker) + (t0 == 0 ? 1 : 0)) * piece_floats<W::kRows>(dh);
       if (!whole) {
@@ -450,20 +543,18 @@ __global__ void __launch_bounds__(32 * kWarps) paged_few_run_kernel(const AttnPa
           if (r >= u.rows) continue;
           const float inv = s.l[nt][e] > 0.f ? 1.f / s.l[nt][e] : 0.f;
           if (!whole && g == 0) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(s.m[nt][e], s.l[nt][e]);
+          float* row = piece + 2 * W::kRows + r * dh;
+          __nv_bfloat16* dst = out_row(p, u, u.rt * W::kRows + r);
 #pragma unroll
-          for (int jj = 0; jj < W::kJ; ++jj) {
-            const int c = 64 * jj + 8 * g;
-            if (c >= dh) continue;
-            float f[8];
-            s.eight(nt, jj, e, f);
-            if (whole) {
-              *reinterpret_cast<uint4*>(out_row(p, u, u.rt * W::kRows + r) + c) = pack8(f, inv);
-            } else {
-              float4* d = reinterpret_cast<float4*>(piece + 2 * W::kRows + r * dh + c);
-              d[0] = make_float4(f[0], f[1], f[2], f[3]);
-              d[1] = make_float4(f[4], f[5], f[6], f[7]);
+          for (int c = 0; c < KD; ++c)
+            if (16 * c < dh) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float f = s.o[nt][c][2 * x + e];
+                if (whole) dst[W::column(c, x, g)] = __float2bfloat16(f * inv);
+                else row[W::column(c, x, g)] = f;
+              }
             }
-          }
         }
       at += t1 - t0;
       if (at >= run.end) break;
@@ -558,23 +649,30 @@ int device_sms() {
   return n > 0 ? n : 148;
 }
 
-constexpr int kBlocksPerSm = 2;
+constexpr int kBlocksPerSm = 3;
 
 int few_workers() { return device_sms() * kBlocksPerSm * kWarps; }
 
 // Short caches: a block per unit.
 bool by_blocks(const DsbPaged* c) { return static_cast<long long>(c->width) * c->page <= 1024; }
 
-template <int KIND, int DC, int NT>
+template <typename F>
+int with_smem(F* kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? 0 : 944;
+}
+
+template <int KIND, int KD, int NT>
 int launch(AttnParams& p, int max_rt, cudaStream_t stream) {
-  // positions of a tile: what 128 registers of keys and values hold
-  constexpr int MT = NT == 2 ? (KIND == kBf16 ? 1 : 2) : (DC > 2 ? (KIND == kBf16 ? 2 : 4) : 4);
+  using W = Warp<KIND, KD, NT>;
+  constexpr int bytes = kWarps * (W::R::kBytes > W::kRows * (16 * KD + 4) * 4 ? W::R::kBytes : W::kRows * (16 * KD + 4) * 4);
   if (by_blocks(&p.w.c)) {
+    if (with_smem(paged_few_block_kernel<KIND, KD, NT>, bytes)) return 944;
     const dim3 grid(max_rt, p.w.c.H, p.w.c.B);
-    paged_few_block_kernel<KIND, DC, NT, MT><<<grid, 32 * kWarps, 0, stream>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : 944;
+    paged_few_block_kernel<KIND, KD, NT><<<grid, 32 * kWarps, bytes, stream>>>(p);
+    return cudaGetLastError() == cudaSuccess ? 0 : 945;
   }
-  paged_few_run_kernel<KIND, DC, NT, MT><<<p.workers / kWarps, 32 * kWarps, 0, stream>>>(p);
+  if (with_smem(paged_few_run_kernel<KIND, KD, NT>, bytes)) return 944;
+  paged_few_run_kernel<KIND, KD, NT><<<p.workers / kWarps, 32 * kWarps, bytes, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 945;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.workers);
@@ -588,13 +686,14 @@ int launch(AttnParams& p, int max_rt, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, paged_merge_kernel<8 * NT>, p) == cudaSuccess ? 0 : 946;
 }
 
+// Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.
 template <int KIND, int NT>
 int launch_dim(AttnParams& p, int max_rt, cudaStream_t stream) {
-  const int dc = (p.w.c.dh + 31) / 32;
-  if (dc == 1) return launch<KIND, 1, NT>(p, max_rt, stream);
-  if (dc == 2) return launch<KIND, 2, NT>(p, max_rt, stream);
-  if (dc == 3) return launch<KIND, 3, NT>(p, max_rt, stream);
-  return launch<KIND, 4, NT>(p, max_rt, stream);
+  const int dh = p.w.c.dh;
+  if (dh <= 32) return launch<KIND, 2, NT>(p, max_rt, stream);
+  if (dh <= 64) return launch<KIND, 4, NT>(p, max_rt, stream);
+  if (dh <= 80) return launch<KIND, 5, NT>(p, max_rt, stream);
+  return launch<KIND, 8, NT>(p, max_rt, stream);
 }
 
 template <int KIND>
