@@ -5,14 +5,18 @@
 //   S^T [positions, rows] = K Q^T        K the M side: eight rows fill the N side, so that one row costs what eight do
 //                                        and the scores of a tile stay in registers;
 //   O^T [dh, rows]       += V^T P^T      V^T the M side, by transposing ldmatrix; P is transposed by movmatrix.
-// 8-bit codes go through ldmatrix as pairs and become bf16 in registers, exactly; any order of the contraction will
-// do as long as both operands have it, so a lane's queries are those of the four neighbouring codes it gets.  Scales
-// of positions go to the scores and the weights in fp32.  Running maximum and sum stay in registers.
+// 8-bit codes go through ldmatrix as pairs and become fp16 in registers, exactly (an instruction for two e4m3 codes;
+// two and a half for two int8 ones); any order of the contraction will do as long as both operands have it, so a
+// lane's queries are those of the four neighbouring codes it gets.  Queries, bf16, become fp16 by a power of two for
+// each row that brings the largest to [128, 256): exact down to 2^-22 of it, off by 2^-33 of it below.  The keys'
+// scales go to the scores in fp32, the values' to the exponents (see below).  Running maximum and sum stay in registers.
 //
 // Two ways to share the work: short caches take one block per unit, its warps interleaved over the tiles and merged
 // in shared memory: one launch.  Long ones take as many warps as the GPU holds, each with an equal run of consecutive
 // tiles of all units; a unit that several warps share is left in pieces, which a second kernel adds up in order.  The
 // lengths are read on the device, so a captured call follows them.
+#include <cuda_fp16.h>
+
 #include "common/paged_units.cuh"
 #include "common/ptx.cuh"
 
@@ -22,12 +26,19 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr float kFloor = -3.0e38f;     // below every score
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
 
+template <bool F16>
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -56,17 +67,35 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// The four codes that ldmatrix gives a lane, as bf16: neighbours (K), or of two positions by column (V transposed).
-template <int KIND>
-__device__ __forceinline__ uint32_t pair_to_bf16(uint32_t p) {
+// Four codes as two registers of fp16 pairs: bytes 0, 1 and 2, 3 (K: neighbours of a row), or, crossed, 0, 2 and 1, 3
+// (V: ldmatrix transposed pairs of columns, a register holds two columns of two positions).  int8: 0x6400 + u is the
+// fp16 number 1024 + u, u = code + 128.
+template <int KIND, bool CROSSED>
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t x) {
+  uint2 r;
   if (KIND == kInt8) {
-    const uint32_t a = (p & 0x007f007fu) | 0x43004300u, b = (p & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&d);
+    x ^= 0x80808080u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, CROSSED ? 0x4240 : 0x4140), b = __byte_perm(x, 0x64646464u, CROSSED ? 0x4341 : 0x4342);
+    const uint32_t off = 0x64806480u;                    // 1152 twice
+    const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
+    r.x = *reinterpret_cast<const uint32_t*>(&u);
+    r.y = *reinterpret_cast<const uint32_t*>(&v);
+    return r;
   }
-  const uint32_t a = ((p & 0x007f007fu) << 4) | ((p & 0x00800080u) << 8), s = 0x7b807b80u;   // 2^120 twice
-  const __nv_bfloat162 d = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&s));
-  return *reinterpret_cast<const uint32_t*>(&d);
+  if (CROSSED) x = __byte_perm(x, 0u, 0x3120);
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
+      : "=r"(r.x), "=r"(r.y) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Shared memory of a warp: kStages tiles of keys, values and scales.  Rows are an odd number of 16-byte words
@@ -91,9 +120,11 @@ template <int KIND, int KD, int NT>
 struct Warp {
   using R = Ring<KIND, KD>;
   static constexpr int kRows = 8 * NT, kTP = R::kTP, kMT = R::kMT;
+  static constexpr bool kF16 = KIND != kBf16;
   uint32_t q[NT][KD][2];
   float o[NT][KD][4];
   float m[NT][2], l[NT][2];
+  float f[NT][2];                    // scores to exponents of two: scale * log2(e) over the row's power of two
 
   static __device__ __forceinline__ int column(int c, int e, int g) {
     return KIND == kBf16 ? 16 * c + 8 * e + g : 16 * c + 2 * g + e;
@@ -106,19 +137,38 @@ struct Warp {
       const bool live = 8 * nt + g < u.rows;
       const __nv_bfloat16* row = p.q;
       if (live) row += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
+      uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
         const bool on = live && 16 * k < p.w.c.dh;
-        if (KIND == kBf16) {
+        if (!kF16) {
           q[nt][k][0] = on ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * k + 2 * t)) : 0u;
           q[nt][k][1] = on ? __ldg(reinterpret_cast<const uint32_t*>(row + 16 * k + 8 + 2 * t)) : 0u;
         } else {
           const uint2 v = on ? __ldg(reinterpret_cast<const uint2*>(row + 16 * k + 4 * t)) : make_uint2(0u, 0u);
           q[nt][k][0] = v.x;
           q[nt][k][1] = v.y;
+          top = max(top, max(max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu)));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][k][e] = 0.f;
+      }
+      f[nt][0] = f[nt][1] = p.scale_log2;
+      if (kF16) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponent of the row's largest value to that of 128; rows of zeros, tiny ones and non-numbers as they are
+        const uint32_t e = top >> 7;
+        const bool as_is = e < 16u || e == 255u;
+        const float up = as_is ? 1.f : __uint_as_float((127u + 134u - e) << 23);
+        const float down = as_is ? 1.f : __uint_as_float((e - 7u) << 23);
+#pragma unroll
+        for (int k = 0; k < KD; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            q[nt][k][x] = pack_f16x2(__uint_as_float(q[nt][k][x] << 16) * up, __uint_as_float(q[nt][k][x] & 0xffff0000u) * up);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) f[nt][x] *= __shfl_sync(0xffffffffu, down, 4 * (2 * t + x));
       }
       m[nt][0] = m[nt][1] = kFloor;
       l[nt][0] = l[nt][1] = 0.f;
@@ -153,6 +203,15 @@ struct Warp {
       }
       return id;
     };
+    // the 16-byte words of sixteen positions that this lane copies: their row, and their place in shared memory
+    constexpr int kCopies = (16 * KD * R::kElem + 31) / 32;
+    uint32_t copy_row[kCopies], copy_dst[kCopies];
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const int i = lane + 32 * c;
+      copy_row[c] = i < 16 * wpr ? (i * per_word) >> 16 : 99;            // i / wpr: exact for i < 256, wpr <= 16
+      copy_dst[c] = copy_row[c] * row_b + ((i - copy_row[c] * wpr) << 4);
+    }
     uint32_t absent[R::kStages];                         // bit mt: the sixteen positions have no page
     auto issue = [&](int tile, int slot, int ids) {
       uint32_t gone = 0;
@@ -168,14 +227,13 @@ struct Warp {
           const char* vs = static_cast<const char*>(p.w.c.v) + base * dh * R::kElem;
           const bool all = id >= 0 && x + 16 <= u.hi && x >= u.lo;
 #pragma unroll
-          for (int c = 0; c < (16 * KD * R::kElem + 31) / 32; ++c) {
-            const int i = lane + 32 * c;
-            if (i >= 16 * wpr) break;
-            const int row = (i * per_word) >> 16;        // i / wpr: exact for i < 256, wpr <= 16
-            const uint32_t off = (16 * mt + row) * row_b + ((i - row * wpr) << 4);
-            const bool on = all || (id >= 0 && x + row < u.hi && (x + row >= u.lo || x + row < u.s_end));
-            copy16(kdst + off, ks + 16 * i, on);
-            copy16(vdst + off, vs + 16 * i, on);
+          for (int c = 0; c < kCopies; ++c) {
+            if (copy_row[c] >= 16u) continue;
+            const uint32_t off = 16 * mt * row_b + copy_dst[c];
+            const int y = x + static_cast<int>(copy_row[c]);
+            const bool on = all || (id >= 0 && y < u.hi && (y >= u.lo || y < u.s_end));
+            copy16(kdst + off, ks + 16 * lane + 512 * c, on);
+            copy16(vdst + off, vs + 16 * lane + 512 * c, on);
           }
           if (KIND != kBf16 && lane < 8) {
             const float* src = (lane < 4 ? p.w.c.k_scale : p.w.c.v_scale) + base + 4 * (lane & 3);
@@ -232,7 +290,7 @@ struct Warp {
               uint32_t a[4];
               ldmatrix(at + 32 * k, a);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][mt], a[0], a[1], a[2], a[3], q[nt][k][0], q[nt][k][1]);
+              for (int nt = 0; nt < NT; ++nt) mma16816<false>(s[nt][mt], a[0], a[1], a[2], a[3], q[nt][k][0], q[nt][k][1]);
             }
           }
         } else {
@@ -244,32 +302,33 @@ struct Warp {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 if (k + e < KD && k + e < steps) {
-                  const uint2 lo = codes_to_bf16<KIND>(a[2 * e]), hi = codes_to_bf16<KIND>(a[2 * e + 1]);
+                  const uint2 lo = codes_to_f16<KIND, false>(a[2 * e]), hi = codes_to_f16<KIND, false>(a[2 * e + 1]);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt)
-                    mma16816(s[nt][mt], lo.x, hi.x, lo.y, hi.y, q[nt][k + e][0], q[nt][k + e][1]);
+                    mma16816<true>(s[nt][mt], lo.x, hi.x, lo.y, hi.y, q[nt][k + e][0], q[nt][k + e][1]);
                 }
               }
             }
           }
         }
       }
-      // ---- weights: s[.][.][c] is position g + 8 (c / 2), row 2t + c % 2
-      float ks[kMT][2], vs[kMT][2];
+      // ---- weights: s[.][.][c] is position g + 8 (c / 2), row 2t + c % 2.  With scales v of the values the running
+      // maximum is that of score + log2 v, so that a weight times its scale, 2^14 at most, is an fp16 number: 2^-11
+      // off at most, or 2^-39 of the largest; the sum takes the scale out again.  A scale of zero counts as 2^-126.
+      float ks[kMT][2], lv[kMT][2], rv[kMT][2];
+      if (kF16) {
 #pragma unroll
-      for (int mt = 0; mt < kMT; ++mt)
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          ks[mt][e] = p.scale_log2;
-          vs[mt][e] = 1.f;
-          if (KIND != kBf16) {
-            float a, b;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(sst + (16 * mt + 8 * e + g) * 4) : "memory");
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(sst + (kTP + 16 * mt + 8 * e + g) * 4) : "memory");
-            ks[mt][e] *= a;
-            vs[mt][e] = b;
+          for (int e = 0; e < 2; ++e) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks[mt][e]) : "r"(sst + (16 * mt + 8 * e + g) * 4) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sst + (kTP + 16 * mt + 8 * e + g) * 4) : "memory");
+            v = v < kLeastScale ? kLeastScale : v;       // keeps NaN
+            lv[mt][e] = log2_fast(v);
+            rv[mt][e] = __fdividef(1.f, v);
           }
-        }
+      }
       const bool open = gone == 0u && x0 >= u.lo_all && x0 + kTP <= u.hi_all;     // every row sees every position
       uint32_t pt[NT][kMT][2];
 #pragma unroll
@@ -291,37 +350,37 @@ struct Warp {
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[nt][mt][c] *= ks[mt][c >> 1];
+            s[nt][mt][c] = kF16 ? fmaf(s[nt][mt][c], ks[mt][c >> 1] * f[nt][c & 1], lv[mt][c >> 1]) : s[nt][mt][c] * f[nt][c & 1];
             if ((vis >> (4 * mt + c)) & 1u) top[c & 1] = fmaxf(top[c & 1], s[nt][mt][c]);
           }
-        float f[2];
+        float d[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
           top[e] = fmaxf(top[e], m[nt][e]);
-          f[e] = exp2_fast(m[nt][e] - top[e]);
+          d[e] = exp2_fast(m[nt][e] - top[e]);
           m[nt][e] = top[e];
-          l[nt][e] *= f[e];
+          l[nt][e] *= d[e];
         }
-        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+        if (__any_sync(0xffffffffu, d[0] != 1.f || d[1] != 1.f)) {
 #pragma unroll
           for (int c = 0; c < KD; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][c][e] *= f[e & 1];
+            for (int e = 0; e < 4; ++e) o[nt][c][e] *= d[e & 1];
         }
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt) {
           float w[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            w[c] = (vis >> (4 * mt + c)) & 1u ? exp2_fast(s[nt][mt][c] - m[nt][c & 1]) : 0.f;
-            l[nt][c & 1] += w[c];
-            if (KIND != kBf16) w[c] = (vis >> (4 * mt + c)) & 1u ? w[c] * vs[mt][c >> 1] : 0.f;
+            w[c] = (vis >> (4 * mt + c)) & 1u ? exp2_fast(s[nt][mt][c] - m[nt][c & 1] + (kF16 ? 14.f : 0.f)) : 0.f;
+            if (kF16) l[nt][c & 1] = (vis >> (4 * mt + c)) & 1u ? fmaf(w[c], rv[mt][c >> 1], l[nt][c & 1]) : l[nt][c & 1];
+            else l[nt][c & 1] += w[c];
           }
-          // the one rounding of a weight (to bf16, with its position's scale): 2^-8 at most
-          pt[nt][mt][0] = transpose8x8(pack_bf16x2(w[0], w[1]));
-          pt[nt][mt][1] = transpose8x8(pack_bf16x2(w[2], w[3]));
+          // the one rounding of a weight: to bf16, 2^-8 at most, or to fp16 as above
+          pt[nt][mt][0] = transpose8x8(kF16 ? pack_f16x2(w[0], w[1]) : pack_bf16x2(w[0], w[1]));
+          pt[nt][mt][1] = transpose8x8(kF16 ? pack_f16x2(w[2], w[3]) : pack_bf16x2(w[2], w[3]));
         }
       }
       // ---- O^T += V^T P^T
@@ -335,7 +394,7 @@ struct Warp {
               uint32_t a[4];
               ldmatrix_t(at + 32 * c, a);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][c], a[0], a[1], a[2], a[3], pt[nt][mt][0], pt[nt][mt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][c], a[0], a[1], a[2], a[3], pt[nt][mt][0], pt[nt][mt][1]);
             }
           }
         } else {
@@ -347,12 +406,10 @@ struct Warp {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 if (c + e < KD && c + e < steps) {
-                  const uint32_t a0 = pair_to_bf16<KIND>(__byte_perm(a[2 * e], 0u, 0x4240)),
-                                 a1 = pair_to_bf16<KIND>(__byte_perm(a[2 * e], 0u, 0x4341)),
-                                 a2 = pair_to_bf16<KIND>(__byte_perm(a[2 * e + 1], 0u, 0x4240)),
-                                 a3 = pair_to_bf16<KIND>(__byte_perm(a[2 * e + 1], 0u, 0x4341));
+                  const uint2 lo = codes_to_f16<KIND, true>(a[2 * e]), hi = codes_to_f16<KIND, true>(a[2 * e + 1]);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][c + e], a0, a1, a2, a3, pt[nt][mt][0], pt[nt][mt][1]);
+                  for (int nt = 0; nt < NT; ++nt)
+                    mma16816<true>(o[nt][c + e], lo.x, lo.y, hi.x, hi.y, pt[nt][mt][0], pt[nt][mt][1]);
                 }
               }
             }
@@ -428,7 +485,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const A
         f[2] = fmaf(x, v.z, f[2]);
         f[3] = fmaf(x, v.w, f[3]);
       }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
           make_uint2(pack_bf16x2(f[0] * inv, f[1] * inv), pack_bf16x2(f[2] * inv, f[3] * inv));
     }
@@ -482,7 +539,7 @@ __device__ __forceinline__ Run share(const AttnParams& p, int lane, long long wo
 template <int ROWS>
 __host__ __device__ constexpr int piece_floats(int dh) { return ROWS * (dh + 2); }
 
-constexpr int kLeastTiles = 2;
+constexpr int kLeastTiles = 8;
 
 // Equal runs of tiles for every warp.  Piece 2 i + 1 of worker i: a unit that begins in its run and ends in a later
 // one; piece 2 i: a unit that began in an earlier run.  meta[i] = {unit of piece 2 i + 1 or -1 .., rows | 1 << 16 if
@@ -541,7 +598,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
         for (int e = 0; e < 2; ++e) {
           const int r = 8 * nt + 2 * t + e;
           if (r >= u.rows) continue;
-          const float inv = s.l[nt][e] > 0.f ? 1.f / s.l[nt][e] : 0.f;
+          const float inv = s.l[nt][e] == 0.f ? 0.f : 1.f / s.l[nt][e];
           if (!whole && g == 0) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(s.m[nt][e], s.l[nt][e]);
           float* row = piece + 2 * W::kRows + r * dh;
           __nv_bfloat16* dst = out_row(p, u, u.rt * W::kRows + r);
@@ -576,15 +633,19 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
   if (lane == 0) p.meta[worker] = meta;
 }
 
-constexpr int kMergeThreads = 128;
+constexpr int kMergeThreads = 256;
+constexpr int kMergeChunk = 64;        // pieces whose weights are at hand at a time
 
-// One block per worker whose last unit goes on in later runs: its piece and theirs, in order.
+// One block per worker whose last unit goes on in later runs: its piece and theirs, in order.  A few threads would
+// wait for one piece after the other, so groups of threads take every n-th piece each.
 template <int ROWS>
 __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float s_w[ROWS];
+  __shared__ float s_w[kMergeChunk][ROWS];
+  __shared__ float s_top[ROWS], s_inv[ROWS];
+  __shared__ __align__(16) float4 s_sum[kMergeThreads];
   __shared__ int s_last;
-  const int i = blockIdx.x, dh = p.w.c.dh;
+  const int i = blockIdx.x, dh = p.w.c.dh, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4 meta = p.meta[i];
   if (meta.x < 0) return;
   Unit u;
@@ -592,23 +653,21 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnPa
   u.h = meta.y;
   u.rt = meta.z;
   unit_range<ROWS, 16>(p, u);
-  if (threadIdx.x < 32) {                              // the worker that ends the unit
+  if (tid < 32) {                                      // the worker that ends the unit
     int j = i + 1;
     for (;; j += 32) {
-      const int k = j + static_cast<int>(threadIdx.x);
+      const int k = j + tid;
       const unsigned end = __ballot_sync(0xffffffffu, k >= p.workers || p.meta[k].w != 0);
       if (end != 0u) {
         j += __ffs(end) - 1;
         break;
       }
     }
-    if (threadIdx.x == 0) s_last = min(j, p.workers - 1);
+    if (tid == 0) s_last = min(j, p.workers - 1);
   }
   __syncthreads();
   const int last = s_last, stride = piece_floats<ROWS>(dh);
   auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __shared__ float s_top[ROWS];
   for (int r = warp; r < u.rows; r += kMergeThreads / 32) {
     float top = kFloor;
     for (int j = i + lane; j <= last; j += 32) top = fmaxf(top, piece(j)[2 * r]);
@@ -620,25 +679,59 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnPa
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     if (lane == 0) {
       s_top[r] = top;
-      s_w[r] = sum > 0.f ? 1.f / sum : 0.f;
+      s_inv[r] = sum == 0.f ? 0.f : 1.f / sum;
     }
   }
-  __syncthreads();
-  for (int k = threadIdx.x; k < u.rows * (dh / 4); k += kMergeThreads) {
-    const int r = k / (dh / 4), c = 4 * (k - r * (dh / 4));
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int j = i; j <= last; ++j) {
-      const float* d = piece(j);
-      const float x = exp2_fast(d[2 * r] - s_top[r]);
-      const float4 o = *reinterpret_cast<const float4*>(d + 2 * ROWS + r * dh + c);
-      a.x = fmaf(x, o.x, a.x);
-      a.y = fmaf(x, o.y, a.y);
-      a.z = fmaf(x, o.z, a.z);
-      a.w = fmaf(x, o.w, a.w);
+  const int tasks = u.rows * (dh / 4);                 // float4s of the unit
+  const int groups = tasks >= kMergeThreads ? 1 : kMergeThreads / tasks;
+  const int grp = groups == 1 ? 0 : tid / tasks, at = groups == 1 ? tid : tid - grp * tasks;
+  const int rounds = groups == 1 ? (tasks + kMergeThreads - 1) / kMergeThreads : 1;
+  constexpr int kRounds = (ROWS * 32 + kMergeThreads - 1) / kMergeThreads;
+  float4 a[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = i; j0 <= last; j0 += kMergeChunk) {
+    const int n = min(kMergeChunk, last + 1 - j0);
+    __syncthreads();
+    for (int x = tid; x < n * u.rows; x += kMergeThreads) {
+      const int j = x / u.rows, r = x - j * u.rows;
+      s_w[j][r] = exp2_fast(piece(j0 + j)[2 * r] - s_top[r]);
     }
-    *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r) + c) =
-        make_uint2(pack_bf16x2(a.x * s_w[r], a.y * s_w[r]), pack_bf16x2(a.z * s_w[r], a.w * s_w[r]));
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
+      if (k < rounds && task < tasks && grp < groups) {
+#pragma unroll 8
+        for (int j = grp; j < n; j += groups) {
+          const float w = s_w[j][r];
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(piece(j0 + j) + 2 * ROWS + r * dh + c));
+          a[k].x = fmaf(w, o.x, a[k].x);
+          a[k].y = fmaf(w, o.y, a[k].y);
+          a[k].z = fmaf(w, o.z, a[k].z);
+          a[k].w = fmaf(w, o.w, a[k].w);
+        }
+      }
+    }
+  }
+  if (groups > 1) {
+    s_sum[tid] = a[0];
+    __syncthreads();
+    if (grp != 0) return;
+    for (int x = 1; x < groups; ++x) {
+      const float4 o = s_sum[at + x * tasks];
+      a[0].x += o.x;
+      a[0].y += o.y;
+      a[0].z += o.z;
+      a[0].w += o.w;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
+    if (k < rounds && task < tasks)
+      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r) + c) =
+          make_uint2(pack_bf16x2(a[k].x * s_inv[r], a[k].y * s_inv[r]), pack_bf16x2(a[k].z * s_inv[r], a[k].w * s_inv[r]));
   }
 }
 
