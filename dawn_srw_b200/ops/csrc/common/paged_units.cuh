@@ -1,10 +1,53 @@
 // Attention over pages, cut into units: a unit is a (sequence, key/value head, tile of query rows), its work the
 // tiles of positions that its rows see.  Query rows of a head are (new token, query head of the group), tokens first.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "paged.cuh"
+#include "ptx.cuh"
 
 namespace dsb {
 namespace paged {
+
+constexpr float kFloor = -3.0e38f;               // below every score
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Four codes as two registers of fp16 pairs: bytes 0, 1 and 2, 3 (K: neighbours of a row), or, crossed, 0, 2 and 1, 3
+// (V: ldmatrix transposed pairs of columns, a register holds two columns of two positions).  int8: 0x6400 + u is the
+// fp16 number 1024 + u, u = code + 128.
+template <int KIND, bool CROSSED>
+__device__ __forceinline__ uint2 codes_to_f16(uint32_t x) {
+  uint2 r;
+  if (KIND == kInt8) {
+    x ^= 0x80808080u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, CROSSED ? 0x4240 : 0x4140), b = __byte_perm(x, 0x64646464u, CROSSED ? 0x4341 : 0x4342);
+    const uint32_t off = 0x64806480u;                    // 1152 twice
+    const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
+    r.x = *reinterpret_cast<const uint32_t*>(&u);
+    r.y = *reinterpret_cast<const uint32_t*>(&v);
+    return r;
+  }
+  if (CROSSED) x = __byte_perm(x, 0u, 0x3120);
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
+      : "=r"(r.x), "=r"(r.y) : "r"(x));
+  return r;
+}
 
 struct AttnParams {
   View w;
@@ -85,6 +128,254 @@ __device__ __forceinline__ void zero_other_rows(const AttnParams& p, int worker,
     if (row >= a) row += e - a;
     reinterpret_cast<uint4*>(p.out)[row * per + i % per] = make_uint4(0u, 0u, 0u, 0u);
   }
+}
+
+__device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) {
+  return p.out + (static_cast<size_t>(u.first + row / p.G) * p.Hq + u.h * p.G + row % p.G) * p.w.c.dh;
+}
+
+// Where a worker's run of tiles begins, among all tiles of all units in order (sequence, head, row tile).
+struct Run { long long begin, end, total; };
+
+// Equal runs of the warps: worker i of n takes tiles [i T / n, (i + 1) T / n).
+template <int ROWS, int TP>
+__device__ __forceinline__ Run share(const AttnParams& p, int lane, long long worker, int least, int& b, long long& before) {
+  const int B = p.w.c.B;
+  long long total = 0;
+  for (int i = 0; i < B; i += 32) {
+    long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    total += x;
+  }
+  const long long most = total / least;
+  const long long n = most < 1 ? 1 : most < p.workers ? most : p.workers;
+  Run r = {0, 0, total};
+  if (worker >= n) return r;
+  r.begin = worker * total / n;
+  r.end = (worker + 1) * total / n;
+  b = 0;
+  before = 0;
+  for (int i = 0; i < B; i += 32) {                    // the sequence that holds tile r.begin
+    const long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
+    long long c = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, c, d);
+      if (lane >= d) c += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + c > r.begin);
+    if (past != 0u) {
+      const int k = __ffs(past) - 1;
+      b = i + k;
+      before += __shfl_sync(0xffffffffu, c - x, k);
+      return r;
+    }
+    before += __shfl_sync(0xffffffffu, c, 31);
+  }
+  return r;
+}
+
+// A piece of a unit in the workspace: per row maximum and sum, then O.
+template <int ROWS>
+__host__ __device__ constexpr int piece_floats(int dh) { return ROWS * (dh + 2); }
+
+// A worker's segments: what of each unit lies in its run.
+template <int ROWS, int TP>
+struct Segments {
+  Unit u;
+  int nrt, t0, t1;                  // row tiles of the sequence; tiles [t0, t1) of the unit
+  long long at, end;
+
+  __device__ __forceinline__ bool on() const { return at < end; }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == u.tiles; }
+  __device__ __forceinline__ int slot() const { return t0 == 0 ? 1 : 0; }        // of the worker's two pieces
+
+  // Of a unit that other workers share: where it begins (x, y, z), or that it ends here (w).
+  __device__ __forceinline__ void note(int4& meta) const {
+    if (whole()) return;
+    if (t0 == 0) {
+      meta.x = u.b;
+      meta.y = u.h;
+      meta.z = u.rt;
+    } else if (t1 == u.tiles) {
+      meta.w = 1;
+    }
+  }
+
+  __device__ void begin(const AttnParams& p, int lane, int worker, int least) {
+    int b = 0;
+    long long before = 0;
+    const Run run = share<ROWS, TP>(p, lane, worker, least, b, before);
+    at = run.begin;
+    end = run.end;
+    if (!on()) return;
+    unit_sequence(p, u, b);
+    nrt = row_tiles<ROWS>(u.n, p.G);
+    long long per_head = 0, off = at - before;
+    for (u.rt = 0; u.rt < nrt; ++u.rt) {
+      unit_range<ROWS, TP>(p, u);
+      per_head += u.tiles;
+    }
+    u.h = static_cast<int>(off / per_head);
+    off -= u.h * per_head;
+    for (u.rt = 0;; ++u.rt) {
+      unit_range<ROWS, TP>(p, u);
+      if (off < u.tiles) break;
+      off -= u.tiles;
+    }
+    t0 = static_cast<int>(off);
+    t1 = static_cast<int>(min(static_cast<long long>(u.tiles), t0 + (end - at)));
+  }
+
+  __device__ void next(const AttnParams& p) {
+    at += t1 - t0;
+    if (!on()) return;
+    if (++u.rt >= nrt) {
+      u.rt = 0;
+      if (++u.h >= p.w.c.H) {
+        u.h = 0;
+        do {
+          unit_sequence(p, u, u.b + 1);
+          nrt = row_tiles<ROWS>(u.n, p.G);
+        } while (nrt == 0);
+      }
+    }
+    unit_range<ROWS, TP>(p, u);
+    t0 = 0;
+    t1 = static_cast<int>(min(static_cast<long long>(u.tiles), end - at));
+  }
+};
+
+constexpr int kMergeThreads = 256;
+constexpr int kMergeChunk = 64;        // pieces whose weights are at hand at a time
+
+// A block per worker whose last unit goes on in later runs and SUB of the unit's rows: its piece and theirs, in order.  A few threads would
+// wait for one piece after the other, so groups of threads take every n-th piece each.
+template <int ROWS, int SUB>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float s_w[kMergeChunk][SUB];
+  __shared__ float s_top[SUB], s_inv[SUB];
+  __shared__ __align__(16) float4 s_sum[kMergeThreads];
+  __shared__ int s_last;
+  const int i = blockIdx.x, dh = p.w.c.dh, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int4 meta = p.meta[i];
+  if (meta.x < 0) return;
+  Unit u;
+  unit_sequence(p, u, meta.x);
+  u.h = meta.y;
+  u.rt = meta.z;
+  unit_range<ROWS, 16>(p, u);
+  const int first = blockIdx.y * SUB, rows = min(SUB, u.rows - first);     // of the unit, this block's
+  if (rows <= 0) return;
+  if (tid < 32) {                                      // the worker that ends the unit
+    int j = i + 1;
+    for (;; j += 32) {
+      const int k = j + tid;
+      const unsigned end = __ballot_sync(0xffffffffu, k >= p.workers || p.meta[k].w != 0);
+      if (end != 0u) {
+        j += __ffs(end) - 1;
+        break;
+      }
+    }
+    if (tid == 0) s_last = min(j, p.workers - 1);
+  }
+  __syncthreads();
+  const int last = s_last, stride = piece_floats<ROWS>(dh);
+  // maxima and sums of this block's rows, and their O
+  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride + 2 * first; };
+  const int to_o = 2 * ROWS - 2 * first + first * dh;
+  for (int r = warp; r < rows; r += kMergeThreads / 32) {
+    float top = kFloor;
+    for (int j = i + lane; j <= last; j += 32) top = fmaxf(top, piece(j)[2 * r]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float sum = 0.f;
+    for (int j = i + lane; j <= last; j += 32) sum = fmaf(exp2_fast(piece(j)[2 * r] - top), piece(j)[2 * r + 1], sum);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (lane == 0) {
+      s_top[r] = top;
+      s_inv[r] = sum == 0.f ? 0.f : 1.f / sum;
+    }
+  }
+  const int tasks = rows * (dh / 4);                 // float4s of the unit
+  const int groups = tasks >= kMergeThreads ? 1 : kMergeThreads / tasks;
+  const int grp = groups == 1 ? 0 : tid / tasks, at = groups == 1 ? tid : tid - grp * tasks;
+  const int rounds = groups == 1 ? (tasks + kMergeThreads - 1) / kMergeThreads : 1;
+  constexpr int kRounds = (SUB * 32 + kMergeThreads - 1) / kMergeThreads;
+  float4 a[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = i; j0 <= last; j0 += kMergeChunk) {
+    const int n = min(kMergeChunk, last + 1 - j0);
+    __syncthreads();
+    for (int x = tid; x < n * rows; x += kMergeThreads) {
+      const int j = x / rows, r = x - j * rows;
+      s_w[j][r] = exp2_fast(piece(j0 + j)[2 * r] - s_top[r]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
+      if (k < rounds && task < tasks && grp < groups) {
+#pragma unroll 8
+        for (int j = grp; j < n; j += groups) {
+          const float w = s_w[j][r];
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(piece(j0 + j) + to_o + r * dh + c));
+          a[k].x = fmaf(w, o.x, a[k].x);
+          a[k].y = fmaf(w, o.y, a[k].y);
+          a[k].z = fmaf(w, o.z, a[k].z);
+          a[k].w = fmaf(w, o.w, a[k].w);
+        }
+      }
+    }
+  }
+  if (groups > 1) {
+    s_sum[tid] = a[0];
+    __syncthreads();
+    if (grp != 0) return;
+    for (int x = 1; x < groups; ++x) {
+      const float4 o = s_sum[at + x * tasks];
+      a[0].x += o.x;
+      a[0].y += o.y;
+      a[0].z += o.z;
+      a[0].w += o.w;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
+    if (k < rounds && task < tasks)
+      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + first + r) + c) =
+          make_uint2(pack_bf16x2(a[k].x * s_inv[r], a[k].y * s_inv[r]), pack_bf16x2(a[k].z * s_inv[r], a[k].w * s_inv[r]));
+  }
+}
+
+template <int ROWS, int SUB>
+int launch_merge(const AttnParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.workers, ROWS / SUB);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<ROWS, SUB>, p) == cudaSuccess ? 0 : 946;
+}
+
+inline long long workspace_bytes(long long workers, int rows, int dh) {
+  return workers * static_cast<long long>(sizeof(int4)) + 2 * workers * rows * (dh + 2) * static_cast<long long>(sizeof(float));
+}
+
+inline int device_sms() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
 }
 
 }  // namespace paged

@@ -1,0 +1,652 @@
+// Attention of a chunk of new tokens over a paged cache, on the tensor cores (tcgen05).
+//
+// A unit is 256 query rows of one key/value head: two tiles of 128 rows (one TMEM lane and one thread per row) that
+// share every tile of 128 positions.  Per tile i and positions j:  S_i = Q_i K_j^T (TMEM);  P_i = exp2(S_i - m), written
+// back to TMEM as the A operand of  O_i += P_i V_j.  While the softmax threads of one tile work, the tensor core
+// works for the other.  m is a row's running maximum as of the last time that it had grown by more than 2^8: O is
+// rescaled then only, and a weight stays below 2^8 times one of the true maximum (floating point loses nothing by it).
+//
+// bf16 pages come by TMA, one box per page and 64 columns, into the 128-byte-swizzled tiles that the instructions
+// read: K-major for K, MN-major for V.  8-bit codes are read by four warps, converted to fp16 (exactly) on the way to
+// the same layout; as in the few-row kernel the keys' scales go to the scores, the values' to the exponents.  Rows of V
+// that no query row sees are zeros, whatever the page holds there.
+//
+// The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
+// SMs idle; units that several blocks share are left in pieces for the merge kernel.
+#include "common/host_utils.cuh"
+#include "common/paged_launch.h"
+
+namespace dsb {
+namespace paged {
+namespace {
+
+constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows, kTP = 128;
+constexpr int kAtom = kTP * 128;            // 128 rows x 64 16-bit columns
+constexpr int kStages = 2;
+constexpr int kMeta = 4;                    // slots of scales and absences: a softmax is at most two tiles behind the loads
+constexpr float kSlack = 8.f;               // how far (in powers of two) a maximum may grow before O is rescaled
+constexpr int kLeast = 2;                   // tiles of a run
+
+// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warpgroup 2: MMA issue (warp 8), TMA (warp 9).  Warpgroup 3, 8-bit
+// kinds: loaders.  Registers: what a warpgroup takes comes out of the launch's own.
+template <int KIND>
+struct Roles {
+  static constexpr int kThreads = KIND == kBf16 ? 384 : 512;
+  static constexpr int kLaunchRegs = KIND == kBf16 ? 168 : 128;
+  static constexpr int kSoftmaxRegs = KIND == kBf16 ? 192 : 144;
+  static constexpr int kIssueRegs = KIND == kBf16 ? 120 : 112;
+  static constexpr int kLoadRegs = KIND == kBf16 ? 0 : 112;
+  static_assert(2 * kSoftmaxRegs + kIssueRegs + kLoadRegs <= kLaunchRegs * (kThreads / 128), "setmaxnreg would wait forever");
+};
+
+template <int NA>                            // 64-column atoms of a head
+struct Smem {
+  static constexpr int kQ = 0;                                   // [2 tiles][NA atoms]
+  static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages][NA]
+  static constexpr int kV = kK + kStages * NA * kAtom;           // [kStages][NA]
+  static constexpr int kKs = kV + kStages * NA * kAtom;          // [kMeta][128] scales of the keys
+  static constexpr int kLv = kKs + kMeta * 512;                  // log2 of the values' scales
+  static constexpr int kRv = kLv + kMeta * 512;                  // their reciprocals
+  static constexpr int kBar = kRv + kMeta * 512;
+  static constexpr int kTotal = kBar + 256 + 1024;
+  static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
+};
+
+struct ChunkParams {
+  CUtensorMap k, v;                          // bf16 pages: [n_pages * H][page][dh]
+  AttnParams a;
+};
+
+// D += A B with A in tensor memory (128 lanes, two 16-bit values per column).
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+template <int REGS>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
+// Instruction descriptor, kind::f16, fp32 accumulators: A and B both bf16 or both fp16.
+__host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn_major) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(b_mn_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int kk) { return umma_desc(tile + (kk >> 2) * kAtom + (kk & 3) * 32, 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int kk) { return umma_desc(tile + kk * 2048, kAtom, 1024); }
+// 16-byte word c8 (eight columns) of a row of a tile made of swizzled atoms.
+__device__ __forceinline__ uint32_t swz(uint32_t tile, int row, int c8) {
+  return tile + (c8 >> 3) * kAtom + row * 128 + (((c8 & 7) ^ (row & 7)) << 4);
+}
+
+// How many of a unit's tiles of positions query tile i works on (its rows see none of the later ones).
+__device__ __forceinline__ int tiles_of(const AttnParams& p, const Unit& u, int i) {
+  const int r0 = i * kTileRows, r1 = min(u.rows, r0 + kTileRows);
+  if (r0 >= u.rows) return 0;
+  const int last = u.len - u.n + (u.rt * kUnitRows + r1 - 1) / p.G;
+  const int end = (max(last + 1, 0) + kTP - 1) / kTP;       // tiles of positions that begin at or before `last`
+  return min(u.tiles, end <= u.st ? end : max(end - u.skip, u.st));
+}
+
+// Tiles of a segment that query tile i works on.
+__device__ __forceinline__ int work_of(const AttnParams& p, const Segments<kUnitRows, kTP>& s, int i) {
+  return max(0, min(s.t1, tiles_of(p, s.u, i)) - s.t0);
+}
+__device__ __forceinline__ int place(const Unit& u, int tile) { return (tile < u.st ? tile : tile + u.skip) * kTP; }
+
+// Bit k: a row at position pos sees position x + k; gone: bits of the two sixteens from x.
+__device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks, uint32_t gone) {
+  auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+  const uint32_t by = below(pos - x + 1), old = below(pos - window + 1 - x) & ~below(sinks - x);
+  return by & ~old & ((gone & 1u) ? 0xffff0000u : 0xffffffffu) & ((gone & 2u) ? 0x0000ffffu : 0xffffffffu);
+}
+
+struct Bars {
+  uint64_t* q_full;     // [2] queries of tile i are in shared memory (4 warps)
+  uint64_t* k_full;     // [kStages] K, and the tile's scales and absences
+  uint64_t* k_empty;    // [kStages] both S of the stage are done
+  uint64_t* v_full;     // [kStages]
+  uint64_t* v_empty;    // [kStages] both O of the stage are done
+  uint64_t* v_fix;      // V has landed, rows behind the end still have to be cleared
+  uint64_t* s_full;     // [2]
+  uint64_t* p_full;     // [2] P is in TMEM, S has been read (4 warps)
+  uint64_t* o_done;     // [2]
+};
+
+template <int KIND, int NA>
+__global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
+  using L = Smem<NA>;
+  using Rl = Roles<KIND>;
+  constexpr bool kF16 = KIND != kBf16;
+  constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  const Bars b = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 11, bars + 13, bars + 15};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* absent = tmem_slot + 2;    // [kMeta] bit i: no row sees sixteen positions i, or they have no page
+  const AttnParams& p = cp.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.w.c.dh, ksteps = dh >> 4;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&b.q_full[i], 4);
+      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_full[i], 4);
+      mbar_init(&b.o_done[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&b.k_full[i], kF16 ? 4 : 1);
+      mbar_init(&b.k_empty[i], 1);
+      mbar_init(&b.v_full[i], kF16 ? 4 : 1);
+      mbar_init(&b.v_empty[i], 1);
+    }
+    mbar_init(b.v_fix, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    if (!kF16) {
+      tma_prefetch_desc(&cp.k);
+      tma_prefetch_desc(&cp.v);
+    }
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+  // S: columns 0 and 128;  O: 256 and 256 + 64 NA;  P: where S is, or behind O
+  auto s_col = [&](int i) { return tmem + 128 * i; };
+  auto o_col = [&](int i) { return tmem + 256 + 64 * NA * i; };
+  auto p_col = [&](int i) { return kAlias ? s_col(i) : tmem + 384 + 64 * i; };
+
+  zero_other_rows(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+  Segments<kUnitRows, kTP> seg;
+  seg.begin(p, lane, blockIdx.x, kLeast);
+
+  if (warp >= 8 && warp < 12) {
+    regs_down<Rl::kIssueRegs>();
+    if (warp == 8) {
+      // ------------------------------------------------------------ MMA issue
+      if (lane == 0) {
+        const uint32_t idesc_s = idesc16(!kF16, kTileRows, kTP, 0), idesc_o = idesc16(!kF16, kTileRows, dh, 1);
+        // stages so far, and of each tile segments with work and P: a phase of a barrier is waited for by whoever
+        // takes part in it, and by nobody else, so that no one is ever two phases off
+        uint32_t nk = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+        bool ok = true;
+        for (; seg.on() && ok; seg.next(p)) {
+          const int n0 = work_of(p, seg, 0), n1 = work_of(p, seg, 1), n = max(n0, n1);
+          auto work = [&](int i) { return i == 0 ? n0 : n1; };
+          for (int i = 0; i < 2 && ok; ++i)
+            if (work(i) > 0) ok = mbar_wait(&b.q_full[i], nq[i]++ & 1, abort_flag);
+          // S_i of the segment's j-th tile (K stage nk + j); the last of the two frees the stage
+          auto issue_s = [&](int i, int j) {
+            const uint32_t st = (nk + j) % kStages, par = ((nk + j) / kStages) & 1;
+            if (!mbar_wait(&b.k_full[st], par, abort_flag)) return false;
+            tc_fence_after();
+            const uint32_t qa = q_addr + i * NA * kAtom, ka = k_addr + st * NA * kAtom;
+#pragma unroll 1
+            for (int kk = 0; kk < ksteps; ++kk) mma_bf16_ss(s_col(i), desc_k(qa, kk), desc_k(ka, kk), idesc_s, kk > 0);
+            mma_commit(&b.s_full[i]);
+            if (j >= work(1 - i) || i == 1) mma_commit(&b.k_empty[st]);
+            return true;
+          };
+#pragma unroll 1
+          for (int i = 0; i < 2 && ok; ++i)
+            if (work(i) > 0) ok = issue_s(i, 0);
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t st = (nk + j) % kStages, par = ((nk + j) / kStages) & 1;
+#pragma unroll 1
+            for (int i = 0; i < 2 && ok; ++i) {
+              if (j >= work(i)) continue;
+              ok = mbar_wait(&b.p_full[i], np[i] & 1, abort_flag) && mbar_wait(&b.v_full[st], par, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t va = v_addr + st * NA * kAtom;
+#pragma unroll 1
+              for (int kk = 0; kk < kTP / 16; ++kk)
+                mma_ts(o_col(i), p_col(i) + 8 * kk, desc_mn(va, kk), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+              mma_commit(&b.o_done[i]);
+              if (j >= work(1 - i) || i == 1) mma_commit(&b.v_empty[st]);
+              if (j + 1 < work(i)) {
+                // the next S takes the columns that this P is being read from
+                if (kAlias) ok = mbar_wait(&b.o_done[i], np[i] & 1, abort_flag);
+                if (ok) ok = issue_s(i, j + 1);
+              }
+              ++np[i];
+            }
+          }
+          nk += n;
+        }
+      }
+    } else if (warp == 9 && !kF16) {
+      // ------------------------------------------------------------ TMA loads of bf16 pages
+      uint32_t nk = 0, fixes = 0;
+      bool ok = true;
+      const int shift = p.w.shift, box = min(p.w.c.page, kTP);
+      for (; seg.on() && ok; seg.next(p)) {
+        const Unit& u = seg.u;
+        const int n = max(work_of(p, seg, 0), work_of(p, seg, 1));
+        const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
+        for (int j = 0; j < n && ok; ++j, ++nk) {
+          const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1;
+          const int x0 = place(u, seg.t0 + j);
+          // lane i < 8: the page of sixteen positions i, -1 where no row sees any of them
+          int id = -1;
+          const int x = x0 + 16 * lane;
+          if (lane < 8 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
+            id = __ldg(table + (x >> shift));
+            if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
+              atomicExch(p.w.c.status, kStatusBadPage);
+              id = -1;
+            }
+          }
+          const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 0xffu;
+          auto unseen = [&](int y) { return y >= u.hi || (y < u.lo && y >= u.s_end); };
+          // rows of V to clear
+          const bool cut = gone != 0u || x0 + kTP > u.hi || (x0 < u.lo && min(x0 + kTP, u.lo) > u.s_end);
+          // lanes that start a box: the first sixteen of each that the tile has
+          const int per = box >> 4;
+          const bool mine = lane < 8 && lane % per == 0;
+          // a box is fetched if its page is there at all: its sixteens are of one page
+          const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+          const uint32_t group = lane < 8 ? (have >> (lane / per * per)) & ((1u << per) - 1u) : 0u;
+          const int src_lane = group ? lane / per * per + __ffs(group) - 1 : 0;
+          const int page = __shfl_sync(0xffffffffu, id, src_lane);
+          const bool fetch = mine && group != 0u;
+          const int boxes = __popc(__ballot_sync(0xffffffffu, fetch));
+          const int c1 = (x0 + 16 * lane) & (p.w.c.page - 1), c2 = page * p.w.c.H + u.h;
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
+          if (!ok) break;
+          if (lane == 0) {
+            absent[nk % kMeta] = gone;
+            mbar_expect_tx(&b.k_full[st], boxes * NA * box * 128);
+          }
+          __syncwarp();
+          if (fetch)
+            for (int a = 0; a < NA; ++a)
+              tma_load_3d(k_addr + (st * NA + a) * kAtom + lane * 2048, &cp.k, &b.k_full[st], 64 * a, c1, c2);
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
+          if (!ok) break;
+          uint64_t* bar = cut ? b.v_fix : &b.v_full[st];
+          if (lane == 0) mbar_expect_tx(bar, boxes * NA * box * 128);
+          __syncwarp();
+          if (fetch)
+            for (int a = 0; a < NA; ++a)
+              tma_load_3d(v_addr + (st * NA + a) * kAtom + lane * 2048, &cp.v, bar, 64 * a, c1, c2);
+          if (cut) {
+            ok = __all_sync(0xffffffffu, mbar_wait(b.v_fix, fixes & 1, abort_flag));
+            if (!ok) break;
+            ++fixes;
+            for (int w = lane; w < kTP * 8; w += 32) {
+              const int row = w >> 3;
+              if (unseen(x0 + row) || ((gone >> (row >> 4)) & 1u))
+                for (int a = 0; a < NA; ++a)
+                  st_shared_v4(v_addr + (st * NA + a) * kAtom + row * 128 + (w & 7) * 16, 0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.v_full[st]);
+          }
+        }
+      }
+    }
+    else if (warp == 10) {
+      // ------------------------------------------------------------ notes for the merge
+      int4 meta = make_int4(-1, 0, 0, 0);
+      for (; seg.on(); seg.next(p)) seg.note(meta);
+      if (lane == 0) p.meta[blockIdx.x] = meta;
+    }
+  } else if (warp >= 12) {
+    // -------------------------------------------------------------- loaders of 8-bit pages
+    if (kF16) {
+      regs_down<Rl::kLoadRegs == 0 ? 112 : Rl::kLoadRegs>();
+      const int tid = threadIdx.x - 384, shift = p.w.shift;
+      uint32_t nk = 0;
+      bool ok = true;
+      for (; seg.on() && ok; seg.next(p)) {
+        const Unit& u = seg.u;
+        const int n = max(work_of(p, seg, 0), work_of(p, seg, 1));
+        const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
+        for (int j = 0; j < n && ok; ++j, ++nk) {
+          const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1, slot = nk % kMeta;
+          const int x = place(u, seg.t0 + j) + tid;                      // this thread's position: a row of K and of V
+          int id = -1;
+          const int x16 = x & ~15;
+          if (x16 < u.hi && (x16 + 16 > u.lo || x16 < u.s_end)) {
+            id = __ldg(table + (x >> shift));
+            if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
+              atomicExch(p.w.c.status, kStatusBadPage);
+              id = -1;
+            }
+          }
+          const uint32_t none = __ballot_sync(0xffffffffu, id < 0);      // two sixteens of this warp
+          const bool on = id >= 0 && x < u.hi && (x >= u.lo || x < u.s_end);
+          const size_t row = on ? slot_row(p.w, id, u.h, x) : 0;
+          const float ks = on ? __ldg(p.w.c.k_scale + row) : 0.f;
+          float vs = on ? __ldg(p.w.c.v_scale + row) : 1.f;
+          vs = vs < kLeastScale ? kLeastScale : vs;                      // keeps NaN
+          auto fill = [&](const void* pool, uint32_t tile) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + row * dh);
+#pragma unroll
+            for (int c = 0; c < 4 * NA; ++c) {                            // sixteen codes: two words of eight columns
+              if (c < ksteps) {
+                const uint4 r = on ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+                const uint2 a = codes_to_f16<KIND, false>(r.x), d = codes_to_f16<KIND, false>(r.y),
+                            e = codes_to_f16<KIND, false>(r.z), f = codes_to_f16<KIND, false>(r.w);
+                st_shared_v4(swz(tile, tid, 2 * c), a.x, a.y, d.x, d.y);
+                st_shared_v4(swz(tile, tid, 2 * c + 1), e.x, e.y, f.x, f.y);
+              }
+            }
+          };
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
+          if (!ok) break;
+          reinterpret_cast<float*>(smem + L::kKs)[slot * kTP + tid] = ks;
+          reinterpret_cast<float*>(smem + L::kLv)[slot * kTP + tid] = log2_fast(vs);
+          reinterpret_cast<float*>(smem + L::kRv)[slot * kTP + tid] = __fdividef(1.f, vs);
+          if (lane == 0)
+            reinterpret_cast<volatile uint8_t*>(absent + slot)[warp - 12] = (none & 0xffffu ? 1 : 0) | (none >> 16 ? 2 : 0);
+          fill(p.w.c.k, k_addr + st * NA * kAtom);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.k_full[st]);
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
+          if (!ok) break;
+          fill(p.w.c.v, v_addr + st * NA * kAtom);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&b.v_full[st]);
+        }
+      }
+    }
+  } else {
+    // -------------------------------------------------------------- softmax, a thread per query row
+    regs_up<Rl::kSoftmaxRegs>();
+    const int i = warp >> 2, row = threadIdx.x - 128 * i;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
+    uint32_t nk = 0, ns = 0;                       // tiles loaded, S of this tile so far
+    bool ok = true;
+    for (; seg.on() && ok; seg.next(p)) {
+      const Unit& u = seg.u;
+      const int n0 = work_of(p, seg, 0), n1 = work_of(p, seg, 1), n = max(n0, n1), mine = i == 0 ? n0 : n1;
+      const int ru = i * kTileRows + row;          // row of the unit
+      const bool real = ru < u.rows;
+      const int r = u.rt * kUnitRows + ru;         // row of the sequence's head
+      const int pos = real ? u.len - u.n + r / p.G : -1;
+      const int w0 = u.rt * kUnitRows + i * kTileRows + (warp & 3) * 32;       // positions of this warp's rows
+      const int pos_lo = u.len - u.n + min(w0, u.n * p.G - 1) / p.G, pos_hi = u.len - u.n + min(w0 + 31, u.n * p.G - 1) / p.G;
+      // the scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which
+      // would turn the -inf of hidden scores into NaN, into queries of zero
+      const bool flat = p.scale_log2 == 0.f;
+      float f = flat ? 1.f : fabsf(p.scale_log2);
+      if (mine > 0) {
+        // queries into the swizzled tile; fp16 ones scaled by a power of two (see the few-row kernel)
+        const __nv_bfloat16* src = p.q;
+        if (real) src += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
+        float up = p.scale_log2 < 0.f ? -1.f : 1.f;
+        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+        if (kF16) {
+          uint32_t top = 0;
+          for (int c = 0; c < 2 * ksteps; ++c) {
+            const uint4 v = real && !flat ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+          }
+          const uint32_t e = top >> 7;
+          if (e >= 16u && e != 255u) {
+            up *= __uint_as_float((261u - e) << 23);
+            f *= __uint_as_float((e - 7u) << 23);
+          }
+        }
+        for (int c = 0; c < 2 * ksteps; ++c) {
+          uint4 v = real && !flat ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+          if (kF16) {
+            float t[8];
+            bf16x8_to_f32(v, t);
+            v = make_uint4(pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up), pack_f16x2(t[4] * up, t[5] * up),
+                           pack_f16x2(t[6] * up, t[7] * up));
+          } else {
+            v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+          }
+          st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), v.x, v.y, v.z, v.w);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.q_full[i]);
+      }
+      float m = kFloor, l = 0.f;
+      for (int j = 0; j < mine; ++j, ++ns) {
+        const uint32_t st = (nk + j) % kMeta;
+        // also says that all MMAs issued before are done: P and O of the last tile
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.s_full[i], ns & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t gone = absent[st];
+        const int x0 = place(u, seg.t0 + j);
+        const bool hidden = gone != 0u || x0 + kTP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
+        const float* meta = reinterpret_cast<const float*>(smem + L::kKs) + st * kTP;
+        // scores (in powers of two) of columns 32 c ..: what a row does not see is -inf and weighs nothing
+        auto finish = [&](float* s, int c) {
+          if (kF16) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 ks = reinterpret_cast<const float4*>(meta)[8 * c + k];
+              const float4 lv = reinterpret_cast<const float4*>(meta + kMeta * kTP)[8 * c + k];
+              s[4 * k] = fmaf(s[4 * k] * f, ks.x, lv.x);
+              s[4 * k + 1] = fmaf(s[4 * k + 1] * f, ks.y, lv.y);
+              s[4 * k + 2] = fmaf(s[4 * k + 2] * f, ks.z, lv.z);
+              s[4 * k + 3] = fmaf(s[4 * k + 3] * f, ks.w, lv.w);
+            }
+          }
+          if (hidden) {
+            const uint32_t seen = seen32(x0 + 32 * c, pos, p.window, p.sinks, gone >> (2 * c));
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (((seen >> k) & 1u) == 0u) s[k] = -INFINITY;
+          }
+        };
+        float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float s[64];
+          tmem_ld32(s_at + 64 * h, s);
+          tmem_ld32(s_at + 64 * h + 32, s + 32);
+          tmem_ld_wait_dep32(s);
+          tmem_ld_wait_dep32(s + 32);
+          finish(s, 2 * h);
+          finish(s + 32, 2 * h + 1);
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            t0 = fmaxf(t0, s[c]);
+            t1 = fmaxf(t1, s[c + 1]);
+            t2 = fmaxf(t2, s[c + 2]);
+            t3 = fmaxf(t3, s[c + 3]);
+          }
+        }
+        const float most = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+        const float top = fmaxf(kF16 ? most : most * f, kFloor);          // f >= 0
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
+          const float m_new = fmaxf(m, top), d = exp2_fast(m - m_new);
+          for (int c = 0; c < ksteps; ++c) {
+            float o[16];
+            tmem_ld16(o_at + 16 * c, o);
+            tmem_ld_wait_dep16(o);
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * d);
+            tmem_st16(o_at + 16 * c, w);
+          }
+          tmem_st_wait();
+          l *= d;
+          m = m_new;
+        }
+        // fp16 weights: 2^14 at most, so that 2^-24 of one is 2^-30 of the reference
+        const float ref = kF16 ? m - 6.f : m;
+        float l0 = 0.f, l1 = 0.f;
+        float s[2][32];
+        tmem_ld32(s_at, s[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float* x = s[c & 1];
+          tmem_ld_wait_dep32(x);
+          if (c < 3) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+          finish(x, c);
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k + e] = exp2_fast(kF16 ? x[k + e] - ref : fmaf(x[k + e], f, -ref));
+            if (kF16) {
+              const float4 rv = reinterpret_cast<const float4*>(meta + 2 * kMeta * kTP)[8 * c + k / 4];
+              l0 = fmaf(x[k], rv.x, l0);
+              l1 = fmaf(x[k + 1], rv.y, l1);
+              l0 = fmaf(x[k + 2], rv.z, l0);
+              l1 = fmaf(x[k + 3], rv.w, l1);
+              w[k / 2] = pack_f16x2(x[k], x[k + 1]);
+              w[k / 2 + 1] = pack_f16x2(x[k + 2], x[k + 3]);
+            } else {
+              l0 += x[k] + x[k + 2];
+              l1 += x[k + 1] + x[k + 3];
+              w[k / 2] = pack_bf16x2(x[k], x[k + 1]);
+              w[k / 2 + 1] = pack_bf16x2(x[k + 2], x[k + 3]);
+            }
+          }
+          tmem_st16(p_at + 16 * c, w);             // where P takes the place of S: columns already read
+        }
+        l += l0 + l1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.p_full[i]);
+      }
+      nk += n;
+      if (!ok) break;
+      if (mine > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.o_done[i], (ns - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool whole = seg.whole();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + seg.slot()) * piece_floats<kUnitRows>(dh);
+      if (real && !whole) *reinterpret_cast<float2*>(piece + 2 * ru) = make_float2(m, l);
+      __nv_bfloat16* dst = real ? out_row(p, u, r) : nullptr;
+      for (int c = 0; c < ksteps; ++c) {
+        float o[16];
+        if (mine > 0) {
+          tmem_ld16(o_at + 16 * c, o);
+          tmem_ld_wait_dep16(o);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = 0.f;
+        }
+        if (!real) continue;
+        if (whole) {
+          st_global_v4(dst + 16 * c, pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                       pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
+          st_global_v4(dst + 16 * c + 8, pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
+                       pack_bf16x2(o[12] * inv, o[13] * inv), pack_bf16x2(o[14] * inv, o[15] * inv));
+        } else {
+          float4* q = reinterpret_cast<float4*>(piece + 2 * kUnitRows + static_cast<size_t>(ru) * dh + 16 * c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) q[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+      tc_fence_before();                           // O has been read: the next unit's P may follow
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) atomicExch(p.w.c.status, kStatusWaitTimeout);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) { }         // copies and MMAs in flight end before the memory goes
+    __syncthreads();
+  }
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (128 rows at most).
+int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
+  auto enc = tensor_map_encoder();
+  if (enc == nullptr) return 1;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.dh), static_cast<cuuint64_t>(c.page),
+                        static_cast<cuuint64_t>(c.n_pages) * static_cast<cuuint64_t>(c.H)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.dh) * 2, static_cast<cuuint64_t>(c.dh) * 2 * c.page};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(c.page < kTP ? c.page : kTP), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  if (dims[2] == 0) dims[2] = 1;              // no page: nothing is fetched
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(pool), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
+}
+
+template <int KIND, int NA>
+int launch(const ChunkParams& p, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(paged_chunk_kernel<KIND, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA>::kTotal) !=
+      cudaSuccess)
+    return 950;
+  paged_chunk_kernel<KIND, NA><<<p.a.workers, Roles<KIND>::kThreads, Smem<NA>::kTotal, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : 951;
+}
+
+template <int KIND>
+int launch_dim(const ChunkParams& p, cudaStream_t stream) {
+  return p.a.w.c.dh <= 64 ? launch<KIND, 1>(p, stream) : launch<KIND, 2>(p, stream);
+}
+
+}  // namespace
+
+long long chunk_workspace(const DsbPaged* c) { return workspace_bytes(device_sms(), kUnitRows, c->dh); }
+
+int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
+  ChunkParams p;
+  a.workers = device_sms();
+  a.meta = static_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(a.meta + a.workers);
+  p.a = a;
+  int rc;
+  if (a.w.c.kind == kBf16) {
+    if (page_map(&p.k, a.w.c.k, a.w.c) || page_map(&p.v, a.w.c.v, a.w.c)) return 952;
+    rc = launch_dim<kBf16>(p, stream);
+  } else if (a.w.c.kind == kE4m3) {
+    rc = launch_dim<kE4m3>(p, stream);
+  } else {
+    rc = launch_dim<kInt8>(p, stream);
+  }
+  return rc ? rc : launch_merge<kUnitRows, 16>(a, stream);
+}
+
+}  // namespace paged
+}  // namespace dsb

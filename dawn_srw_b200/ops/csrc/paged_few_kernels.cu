@@ -15,9 +15,7 @@
 // in shared memory: one launch.  Long ones take as many warps as the GPU holds, each with an equal run of consecutive
 // tiles of all units; a unit that several warps share is left in pieces, which a second kernel adds up in order.  The
 // lengths are read on the device, so a captured call follows them.
-#include <cuda_fp16.h>
-
-#include "common/paged_units.cuh"
+#include "common/paged_launch.h"
 #include "common/ptx.cuh"
 
 namespace dsb {
@@ -25,8 +23,6 @@ namespace paged {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kFloor = -3.0e38f;     // below every score
-constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
 
 template <bool F16>
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -45,11 +41,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void ldmatrix(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -66,37 +57,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Four codes as two registers of fp16 pairs: bytes 0, 1 and 2, 3 (K: neighbours of a row), or, crossed, 0, 2 and 1, 3
-// (V: ldmatrix transposed pairs of columns, a register holds two columns of two positions).  int8: 0x6400 + u is the
-// fp16 number 1024 + u, u = code + 128.
-template <int KIND, bool CROSSED>
-__device__ __forceinline__ uint2 codes_to_f16(uint32_t x) {
-  uint2 r;
-  if (KIND == kInt8) {
-    x ^= 0x80808080u;
-    const uint32_t a = __byte_perm(x, 0x64646464u, CROSSED ? 0x4240 : 0x4140), b = __byte_perm(x, 0x64646464u, CROSSED ? 0x4341 : 0x4342);
-    const uint32_t off = 0x64806480u;                    // 1152 twice
-    const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
-    r.x = *reinterpret_cast<const uint32_t*>(&u);
-    r.y = *reinterpret_cast<const uint32_t*>(&v);
-    return r;
-  }
-  if (CROSSED) x = __byte_perm(x, 0u, 0x3120);
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\ncvt.rn.f16x2.e4m3x2 %0, lo;\ncvt.rn.f16x2.e4m3x2 %1, hi;\n}\n"
-      : "=r"(r.x), "=r"(r.y) : "r"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ float log2_fast(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Shared memory of a warp: kStages tiles of keys, values and scales.  Rows are an odd number of 16-byte words
 // apart, so that the eight rows of an ldmatrix fall on different banks.
@@ -429,10 +389,6 @@ struct Warp {
   }
 };
 
-__device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) {
-  return p.out + (static_cast<size_t>(u.first + row / p.G) * p.Hq + u.h * p.G + row % p.G) * p.w.c.dh;
-}
-
 // One block per unit: grid (row tiles, heads, sequences); more row tiles than the grid has are taken in turn.
 template <int KIND, int KD, int NT>
 __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const AttnParams p) {
@@ -493,57 +449,9 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const A
   }
 }
 
-// Where a worker's run of tiles begins, among all tiles of all units in order (sequence, head, row tile).
-struct Run { long long begin, end, total; };
-
-// Equal runs of the warps: worker i of n takes tiles [i T / n, (i + 1) T / n).
-template <int ROWS, int TP>
-__device__ __forceinline__ Run share(const AttnParams& p, int lane, long long worker, int least, int& b, long long& before) {
-  const int B = p.w.c.B;
-  long long total = 0;
-  for (int i = 0; i < B; i += 32) {
-    long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    total += x;
-  }
-  const long long most = total / least;
-  const long long n = most < 1 ? 1 : most < p.workers ? most : p.workers;
-  Run r = {0, 0, total};
-  if (worker >= n) return r;
-  r.begin = worker * total / n;
-  r.end = (worker + 1) * total / n;
-  b = 0;
-  before = 0;
-  for (int i = 0; i < B; i += 32) {                    // the sequence that holds tile r.begin
-    const long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
-    long long c = x;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, c, d);
-      if (lane >= d) c += y;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, before + c > r.begin);
-    if (past != 0u) {
-      const int k = __ffs(past) - 1;
-      b = i + k;
-      before += __shfl_sync(0xffffffffu, c - x, k);
-      return r;
-    }
-    before += __shfl_sync(0xffffffffu, c, 31);
-  }
-  return r;
-}
-
-// A piece of a unit in the workspace: per row maximum and sum, then O.
-template <int ROWS>
-__host__ __device__ constexpr int piece_floats(int dh) { return ROWS * (dh + 2); }
-
 constexpr int kLeastTiles = 8;
 
-// Equal runs of tiles for every warp.  Piece 2 i + 1 of worker i: a unit that begins in its run and ends in a later
-// one; piece 2 i: a unit that began in an earlier run.  meta[i] = {unit of piece 2 i + 1 or -1 .., rows | 1 << 16 if
-// piece 2 i ends its unit}.
+// Equal runs of tiles for every warp.
 template <int KIND, int KD, int NT>
 __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const AttnParams p) {
   using W = Warp<KIND, KD, NT>;
@@ -552,194 +460,38 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
   const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
   zero_other_rows(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
-  int b = 0;
-  long long before = 0;
-  const Run run = share<W::kRows, W::kTP>(p, lane, worker, kLeastTiles, b, before);
   int4 meta = make_int4(-1, 0, 0, 0);
-  long long at = run.begin;
-  if (at < run.end) {
-    Unit u;
-    unit_sequence(p, u, b);
-    int nrt = row_tiles<W::kRows>(u.n, p.G);
-    // head and row tile of the first unit
-    long long per_head = 0, off = at - before;
-    for (u.rt = 0; u.rt < nrt; ++u.rt) {
-      unit_range<W::kRows, W::kTP>(p, u);
-      per_head += u.tiles;
-    }
-    u.h = static_cast<int>(off / per_head);
-    off -= u.h * per_head;
-    for (u.rt = 0;; ++u.rt) {
-      unit_range<W::kRows, W::kTP>(p, u);
-      if (off < u.tiles) break;
-      off -= u.tiles;
-    }
-    int t0 = static_cast<int>(off);
-    while (true) {
-      const long long left = run.end - at;
-      const int t1 = static_cast<int>(min(static_cast<long long>(u.tiles), t0 + left));
-      W s;
-      s.begin(p, u, g, t);
-      s.run(p, u, t0, t1, 1, lane, ring);
-      const bool whole = t0 == 0 && t1 == u.tiles;
-      float* piece = p.part + (2 * static_cast<size_t>(worker) + (t0 == 0 ? 1 : 0)) * piece_floats<W::kRows>(dh);
-      if (!whole) {
-        if (t0 == 0) {
-          meta.x = u.b;
-          meta.y = u.h;
-          meta.z = u.rt;
-        } else if (t1 == u.tiles) {
-          meta.w = 1;
-        }
-      }
+  Segments<W::kRows, W::kTP> seg;
+  for (seg.begin(p, lane, worker, kLeastTiles); seg.on(); seg.next(p)) {
+    const Unit& u = seg.u;
+    W s;
+    s.begin(p, u, g, t);
+    s.run(p, u, seg.t0, seg.t1, 1, lane, ring);
+    float* piece = p.part + (2 * static_cast<size_t>(worker) + seg.slot()) * piece_floats<W::kRows>(dh);
+    seg.note(meta);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 8 * nt + 2 * t + e;
-          if (r >= u.rows) continue;
-          const float inv = s.l[nt][e] == 0.f ? 0.f : 1.f / s.l[nt][e];
-          if (!whole && g == 0) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(s.m[nt][e], s.l[nt][e]);
-          float* row = piece + 2 * W::kRows + r * dh;
-          __nv_bfloat16* dst = out_row(p, u, u.rt * W::kRows + r);
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * nt + 2 * t + e;
+        if (r >= u.rows) continue;
+        const float inv = s.l[nt][e] == 0.f ? 0.f : 1.f / s.l[nt][e];
+        if (!seg.whole() && g == 0) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(s.m[nt][e], s.l[nt][e]);
+        float* row = piece + 2 * W::kRows + r * dh;
+        __nv_bfloat16* dst = out_row(p, u, u.rt * W::kRows + r);
 #pragma unroll
-          for (int c = 0; c < KD; ++c)
-            if (16 * c < dh) {
+        for (int c = 0; c < KD; ++c)
+          if (16 * c < dh) {
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float f = s.o[nt][c][2 * x + e];
-                if (whole) dst[W::column(c, x, g)] = __float2bfloat16(f * inv);
-                else row[W::column(c, x, g)] = f;
-              }
+            for (int x = 0; x < 2; ++x) {
+              const float f = s.o[nt][c][2 * x + e];
+              if (seg.whole()) dst[W::column(c, x, g)] = __float2bfloat16(f * inv);
+              else row[W::column(c, x, g)] = f;
             }
-        }
-      at += t1 - t0;
-      if (at >= run.end) break;
-      // the next unit
-      t0 = 0;
-      if (++u.rt >= nrt) {
-        u.rt = 0;
-        if (++u.h >= p.w.c.H) {
-          u.h = 0;
-          do {
-            unit_sequence(p, u, u.b + 1);
-            nrt = row_tiles<W::kRows>(u.n, p.G);
-          } while (nrt == 0);
-        }
+          }
       }
-      unit_range<W::kRows, W::kTP>(p, u);
-    }
   }
   if (lane == 0) p.meta[worker] = meta;
-}
-
-constexpr int kMergeThreads = 256;
-constexpr int kMergeChunk = 64;        // pieces whose weights are at hand at a time
-
-// One block per worker whose last unit goes on in later runs: its piece and theirs, in order.  A few threads would
-// wait for one piece after the other, so groups of threads take every n-th piece each.
-template <int ROWS>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float s_w[kMergeChunk][ROWS];
-  __shared__ float s_top[ROWS], s_inv[ROWS];
-  __shared__ __align__(16) float4 s_sum[kMergeThreads];
-  __shared__ int s_last;
-  const int i = blockIdx.x, dh = p.w.c.dh, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int4 meta = p.meta[i];
-  if (meta.x < 0) return;
-  Unit u;
-  unit_sequence(p, u, meta.x);
-  u.h = meta.y;
-  u.rt = meta.z;
-  unit_range<ROWS, 16>(p, u);
-  if (tid < 32) {                                      // the worker that ends the unit
-    int j = i + 1;
-    for (;; j += 32) {
-      const int k = j + tid;
-      const unsigned end = __ballot_sync(0xffffffffu, k >= p.workers || p.meta[k].w != 0);
-      if (end != 0u) {
-        j += __ffs(end) - 1;
-        break;
-      }
-    }
-    if (tid == 0) s_last = min(j, p.workers - 1);
-  }
-  __syncthreads();
-  const int last = s_last, stride = piece_floats<ROWS>(dh);
-  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride; };
-  for (int r = warp; r < u.rows; r += kMergeThreads / 32) {
-    float top = kFloor;
-    for (int j = i + lane; j <= last; j += 32) top = fmaxf(top, piece(j)[2 * r]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float sum = 0.f;
-    for (int j = i + lane; j <= last; j += 32) sum = fmaf(exp2_fast(piece(j)[2 * r] - top), piece(j)[2 * r + 1], sum);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) {
-      s_top[r] = top;
-      s_inv[r] = sum == 0.f ? 0.f : 1.f / sum;
-    }
-  }
-  const int tasks = u.rows * (dh / 4);                 // float4s of the unit
-  const int groups = tasks >= kMergeThreads ? 1 : kMergeThreads / tasks;
-  const int grp = groups == 1 ? 0 : tid / tasks, at = groups == 1 ? tid : tid - grp * tasks;
-  const int rounds = groups == 1 ? (tasks + kMergeThreads - 1) / kMergeThreads : 1;
-  constexpr int kRounds = (ROWS * 32 + kMergeThreads - 1) / kMergeThreads;
-  float4 a[kRounds];
-#pragma unroll
-  for (int k = 0; k < kRounds; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j0 = i; j0 <= last; j0 += kMergeChunk) {
-    const int n = min(kMergeChunk, last + 1 - j0);
-    __syncthreads();
-    for (int x = tid; x < n * u.rows; x += kMergeThreads) {
-      const int j = x / u.rows, r = x - j * u.rows;
-      s_w[j][r] = exp2_fast(piece(j0 + j)[2 * r] - s_top[r]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-      const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
-      if (k < rounds && task < tasks && grp < groups) {
-#pragma unroll 8
-        for (int j = grp; j < n; j += groups) {
-          const float w = s_w[j][r];
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(piece(j0 + j) + 2 * ROWS + r * dh + c));
-          a[k].x = fmaf(w, o.x, a[k].x);
-          a[k].y = fmaf(w, o.y, a[k].y);
-          a[k].z = fmaf(w, o.z, a[k].z);
-          a[k].w = fmaf(w, o.w, a[k].w);
-        }
-      }
-    }
-  }
-  if (groups > 1) {
-    s_sum[tid] = a[0];
-    __syncthreads();
-    if (grp != 0) return;
-    for (int x = 1; x < groups; ++x) {
-      const float4 o = s_sum[at + x * tasks];
-      a[0].x += o.x;
-      a[0].y += o.y;
-      a[0].z += o.z;
-      a[0].w += o.w;
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kRounds; ++k) {
-    const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
-    if (k < rounds && task < tasks)
-      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r) + c) =
-          make_uint2(pack_bf16x2(a[k].x * s_inv[r], a[k].y * s_inv[r]), pack_bf16x2(a[k].z * s_inv[r], a[k].w * s_inv[r]));
-  }
-}
-
-int device_sms() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
 }
 
 constexpr int kBlocksPerSm = 3;
@@ -767,16 +519,7 @@ int launch(AttnParams& p, int max_rt, cudaStream_t stream) {
   if (with_smem(paged_few_run_kernel<KIND, KD, NT>, bytes)) return 944;
   paged_few_run_kernel<KIND, KD, NT><<<p.workers / kWarps, 32 * kWarps, bytes, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 945;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.workers);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<8 * NT>, p) == cudaSuccess ? 0 : 946;
+  return launch_merge<W::kRows, W::kRows>(p, stream);
 }
 
 // Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.
@@ -790,53 +533,28 @@ int launch_dim(AttnParams& p, int max_rt, cudaStream_t stream) {
 }
 
 template <int KIND>
-int launch_rows(AttnParams& p, int max_new, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(max_new) * p.G;
+int launch_rows(AttnParams& p, long long rows, cudaStream_t stream) {
   if (rows <= 8) return launch_dim<KIND, 1>(p, 1, stream);
   const long long rt = (rows + 15) / 16;
   return launch_dim<KIND, 2>(p, static_cast<int>(rt > 65535 ? 65535 : rt), stream);
 }
 
 }  // namespace
+
+long long few_workspace(const DsbPaged* c, int rows) {
+  return by_blocks(c) ? 0 : workspace_bytes(few_workers(), rows <= 8 ? 8 : 16, c->dh);
+}
+
+int launch_few(AttnParams& p, long long rows, void* workspace, cudaStream_t stream) {
+  if (!by_blocks(&p.w.c)) {
+    p.workers = few_workers();
+    p.meta = static_cast<int4*>(workspace);
+    p.part = reinterpret_cast<float*>(p.meta + p.workers);
+  }
+  if (p.w.c.kind == kBf16) return launch_rows<kBf16>(p, rows, stream);
+  if (p.w.c.kind == kE4m3) return launch_rows<kE4m3>(p, rows, stream);
+  return launch_rows<kInt8>(p, rows, stream);
+}
+
 }  // namespace paged
 }  // namespace dsb
-
-using namespace dsb::paged;
-
-extern "C" long long dsb_paged_attention_workspace(const DsbPaged* c, int Hq, int max_new) {
-  if (c->N == 0 || c->B == 0 || c->H <= 0 || by_blocks(c)) return 0;
-  const int rows = static_cast<long long>(max_new) * (Hq / c->H) <= 8 ? 8 : 16;
-  const long long w = few_workers();
-  return w * static_cast<long long>(sizeof(int4)) + 2 * w * rows * (c->dh + 2) * static_cast<long long>(sizeof(float));
-}
-
-extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
-                                   int max_new, int window, int sinks, float scale, void* workspace, cudaStream_t stream) {
-  if (bad_cache(c) || Hq <= 0 || Hq % c->H != 0 || window < 0 || sinks < 0 || max_new < 0) return 940;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8 || c->H > 65535 || c->B > 65535) return 941;
-  if (c->N == 0) return 0;
-  if (c->B == 0) {
-    const size_t bytes = static_cast<size_t>(c->N) * Hq * c->dh * sizeof(__nv_bfloat16);
-    return cudaMemsetAsync(out, 0, bytes, stream) == cudaSuccess ? 0 : 942;
-  }
-  if (!by_blocks(c) && workspace == nullptr) return 943;
-  AttnParams p;
-  p.w = make_view(c);
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.q_st = q_st;
-  p.q_sh = q_sh;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.Hq = Hq;
-  p.G = Hq / c->H;
-  p.window = window > 0 && window < kMostPositions ? window : kMostPositions;
-  p.sinks = sinks;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.workers = few_workers();
-  p.meta = static_cast<int4*>(workspace);
-  p.part = reinterpret_cast<float*>(p.meta + p.workers);
-  if (max_new < 1) max_new = 1;
-  if (max_new > c->N) max_new = c->N;
-  if (c->kind == kBf16) return launch_rows<kBf16>(p, max_new, stream);
-  if (c->kind == kE4m3) return launch_rows<kE4m3>(p, max_new, stream);
-  return launch_rows<kInt8>(p, max_new, stream);
-}

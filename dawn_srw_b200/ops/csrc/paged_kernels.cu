@@ -2,8 +2,7 @@
 // tensors, attention of new tokens over pages.  Types, layouts and bounds: dsb_api_paged.h.
 #include <cuda_fp8.h>
 
-#include "common/paged.cuh"
-#include "common/ptx.cuh"
+#include "common/paged_launch.h"
 
 namespace dsb {
 namespace paged {
@@ -245,4 +244,50 @@ extern "C" int dsb_paged_read(const DsbPaged* c, void* k, void* v, int dst_bf16,
   if (c->kind == kE4m3) return DSB_KIND(kE4m3);
   return DSB_KIND(kInt8);
 #undef DSB_KIND
+}
+
+namespace {
+
+// Query rows of a head above which the tensor cores take over (units of 256 rows).
+constexpr long long kFewRows = 16;
+
+long long rows_of(const DsbPaged* c, int Hq, int max_new) {
+  const long long most = max_new < 1 ? 1 : max_new > c->N ? c->N : max_new;
+  return most * (Hq / c->H);
+}
+
+}  // namespace
+
+extern "C" long long dsb_paged_attention_workspace(const DsbPaged* c, int Hq, int max_new) {
+  if (bad_cache(c) || c->N == 0 || c->B == 0) return 0;
+  const long long rows = rows_of(c, Hq, max_new);
+  return rows <= kFewRows ? few_workspace(c, static_cast<int>(rows)) : chunk_workspace(c);
+}
+
+extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
+                                   int max_new, int window, int sinks, float scale, void* workspace, cudaStream_t stream) {
+  if (bad_cache(c) || Hq <= 0 || Hq % c->H != 0 || window < 0 || sinks < 0 || max_new < 0) return 940;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8 || c->H > 65535 || c->B > 65535) return 941;
+  if (c->N == 0) return 0;
+  if (c->B == 0) {
+    const size_t bytes = static_cast<size_t>(c->N) * Hq * c->dh * sizeof(__nv_bfloat16);
+    return cudaMemsetAsync(out, 0, bytes, stream) == cudaSuccess ? 0 : 942;
+  }
+  if (workspace == nullptr && dsb_paged_attention_workspace(c, Hq, max_new) > 0) return 943;
+  AttnParams p;
+  p.w = make_view(c);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.Hq = Hq;
+  p.G = Hq / c->H;
+  p.window = window > 0 && window < kMostPositions ? window : kMostPositions;
+  p.sinks = sinks;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = nullptr;
+  p.meta = nullptr;
+  p.workers = 0;
+  const long long rows = rows_of(c, Hq, max_new);
+  return rows <= kFewRows ? launch_few(p, rows, workspace, stream) : launch_chunk(p, workspace, stream);
 }
