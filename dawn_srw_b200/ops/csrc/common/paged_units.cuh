@@ -250,43 +250,46 @@ struct Segments {
 constexpr int kMergeThreads = 256;
 constexpr int kMergeChunk = 64;        // pieces whose weights are at hand at a time
 
-// A block per worker whose last unit goes on in later runs and SUB of the unit's rows: its piece and theirs, in order.  A few threads would
-// wait for one piece after the other, so groups of threads take every n-th piece each.
-template <int ROWS, int SUB>
-__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float s_w[kMergeChunk][SUB];
-  __shared__ float s_top[SUB], s_inv[SUB];
-  __shared__ __align__(16) float4 s_sum[kMergeThreads];
-  __shared__ int s_last;
-  const int i = blockIdx.x, dh = p.w.c.dh, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// The unit that worker i left for others to end, and the worker that ends it (all lanes of a warp).
+template <int ROWS>
+__device__ __forceinline__ bool shared_unit(const AttnParams& p, int i, int lane, Unit& u, int& last) {
   const int4 meta = p.meta[i];
-  if (meta.x < 0) return;
-  Unit u;
-  unit_sequence(p, u, meta.x);
+  if (meta.x < 0) return false;
+  u.b = meta.x;
   u.h = meta.y;
   u.rt = meta.z;
-  unit_range<ROWS, 16>(p, u);
-  const int first = blockIdx.y * SUB, rows = min(SUB, u.rows - first);     // of the unit, this block's
-  if (rows <= 0) return;
-  if (tid < 32) {                                      // the worker that ends the unit
-    int j = i + 1;
-    for (;; j += 32) {
-      const int k = j + tid;
-      const unsigned end = __ballot_sync(0xffffffffu, k >= p.workers || p.meta[k].w != 0);
-      if (end != 0u) {
-        j += __ffs(end) - 1;
-        break;
-      }
+  const Rows r = seq_rows(p.w, u.b);
+  u.first = r.first;
+  u.n = r.count;
+  u.rows = min(ROWS, u.n * p.G - u.rt * ROWS);
+  int j = i + 1;
+  for (;; j += 32) {
+    const int k = j + lane;
+    const unsigned end = __ballot_sync(0xffffffffu, k >= p.workers || p.meta[k].w != 0);
+    if (end != 0u) {
+      j += __ffs(end) - 1;
+      break;
     }
-    if (tid == 0) s_last = min(j, p.workers - 1);
   }
-  __syncthreads();
-  const int last = s_last, stride = piece_floats<ROWS>(dh);
-  // maxima and sums of this block's rows, and their O
-  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride + 2 * first; };
-  const int to_o = 2 * ROWS - 2 * first + first * dh;
-  for (int r = warp; r < rows; r += kMergeThreads / 32) {
+  last = min(j, p.workers - 1);
+  return true;
+}
+
+// Units of few rows and many pieces: a block per worker whose last unit goes on in later runs.  A few threads would
+// wait for one piece after the other, so groups of threads take every n-th piece each; sums in a fixed order.
+template <int ROWS>
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_few_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float s_w[kMergeChunk][ROWS];
+  __shared__ float s_top[ROWS], s_inv[ROWS];
+  __shared__ __align__(16) float4 s_sum[kMergeThreads];
+  const int i = blockIdx.x, dh = p.w.c.dh, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  Unit u;
+  int last;
+  if (!shared_unit<ROWS>(p, i, lane, u, last)) return;
+  const int stride = piece_floats<ROWS>(dh), per = dh / 4;
+  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride; };
+  for (int r = warp; r < u.rows; r += kMergeThreads / 32) {
     float top = kFloor;
     for (int j = i + lane; j <= last; j += 32) top = fmaxf(top, piece(j)[2 * r]);
 #pragma unroll
@@ -300,30 +303,34 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnPa
       s_inv[r] = sum == 0.f ? 0.f : 1.f / sum;
     }
   }
-  const int tasks = rows * (dh / 4);                 // float4s of the unit
+  const int tasks = u.rows * per;                      // float4s of the unit
   const int groups = tasks >= kMergeThreads ? 1 : kMergeThreads / tasks;
   const int grp = groups == 1 ? 0 : tid / tasks, at = groups == 1 ? tid : tid - grp * tasks;
-  const int rounds = groups == 1 ? (tasks + kMergeThreads - 1) / kMergeThreads : 1;
-  constexpr int kRounds = (SUB * 32 + kMergeThreads - 1) / kMergeThreads;
+  constexpr int kRounds = (ROWS * 32 + kMergeThreads - 1) / kMergeThreads;
   float4 a[kRounds];
+  int row[kRounds];
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < kRounds; ++k) {
+    a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int task = at + k * kMergeThreads;
+    row[k] = task < tasks && grp < groups && (k == 0 || groups == 1) ? task / per : -1;
+  }
   for (int j0 = i; j0 <= last; j0 += kMergeChunk) {
     const int n = min(kMergeChunk, last + 1 - j0);
     __syncthreads();
-    for (int x = tid; x < n * rows; x += kMergeThreads) {
-      const int j = x / rows, r = x - j * rows;
-      s_w[j][r] = exp2_fast(piece(j0 + j)[2 * r] - s_top[r]);
+    for (int x = tid; x < n * ROWS; x += kMergeThreads) {
+      const int j = x / ROWS, r = x % ROWS;
+      if (r < u.rows) s_w[j][r] = exp2_fast(piece(j0 + j)[2 * r] - s_top[r]);
     }
     __syncthreads();
+#pragma unroll 4
+    for (int j = grp; j < n; j += groups) {
+      const float4* from = reinterpret_cast<const float4*>(piece(j0 + j) + 2 * ROWS) + at;
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-      const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
-      if (k < rounds && task < tasks && grp < groups) {
-#pragma unroll 8
-        for (int j = grp; j < n; j += groups) {
-          const float w = s_w[j][r];
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(piece(j0 + j) + to_o + r * dh + c));
+      for (int k = 0; k < kRounds; ++k) {
+        if (row[k] >= 0) {
+          const float4 o = __ldcg(from + k * kMergeThreads);
+          const float w = s_w[j][row[k]];
           a[k].x = fmaf(w, o.x, a[k].x);
           a[k].y = fmaf(w, o.y, a[k].y);
           a[k].z = fmaf(w, o.z, a[k].z);
@@ -346,25 +353,79 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const AttnPa
   }
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int task = at + k * kMergeThreads, r = task / (dh / 4), c = 4 * (task - r * (dh / 4));
-    if (k < rounds && task < tasks)
-      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + first + r) + c) =
-          make_uint2(pack_bf16x2(a[k].x * s_inv[r], a[k].y * s_inv[r]), pack_bf16x2(a[k].z * s_inv[r], a[k].w * s_inv[r]));
+    if (row[k] < 0) continue;
+    const int r = row[k], c = 4 * (at + k * kMergeThreads - r * per);
+    *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r) + c) =
+        make_uint2(pack_bf16x2(a[k].x * s_inv[r], a[k].y * s_inv[r]), pack_bf16x2(a[k].z * s_inv[r], a[k].w * s_inv[r]));
   }
 }
 
-template <int ROWS, int SUB>
-int launch_merge(const AttnParams& p, cudaStream_t stream) {
+// Units of many rows and few pieces: a warp per four rows.
+constexpr int kMergeRows = 4, kMergeWarps = 8;
+template <int ROWS>
+__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_rows_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int i = blockIdx.x, dh = p.w.c.dh, lane = threadIdx.x & 31;
+  const int r0 = (blockIdx.y * kMergeWarps + (threadIdx.x >> 5)) * kMergeRows;
+  Unit u;
+  int last;
+  if (!shared_unit<ROWS>(p, i, lane, u, last)) return;
+  if (r0 >= u.rows) return;
+  const int stride = piece_floats<ROWS>(dh);
+  const bool mine = 4 * lane < dh;
+  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride; };
+  float top[kMergeRows], sum[kMergeRows];
+  float4 a[kMergeRows];
+#pragma unroll
+  for (int k = 0; k < kMergeRows; ++k) {
+    top[k] = kFloor;
+    sum[k] = 0.f;
+    a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 2
+  for (int j = i; j <= last; ++j) {
+    const float* from = piece(j);
+    float2 ml[kMergeRows];
+    float4 o[kMergeRows];
+#pragma unroll
+    for (int k = 0; k < kMergeRows; ++k) {
+      const bool on = r0 + k < u.rows;
+      ml[k] = on ? __ldcg(reinterpret_cast<const float2*>(from) + r0 + k) : make_float2(kFloor, 0.f);
+      o[k] = on && mine ? __ldcg(reinterpret_cast<const float4*>(from + 2 * ROWS + (r0 + k) * dh) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kMergeRows; ++k) {
+      const float most = fmaxf(top[k], ml[k].x), x = exp2_fast(top[k] - most), w = exp2_fast(ml[k].x - most);
+      top[k] = most;
+      sum[k] = fmaf(sum[k], x, w * ml[k].y);
+      a[k].x = fmaf(a[k].x, x, w * o[k].x);
+      a[k].y = fmaf(a[k].y, x, w * o[k].y);
+      a[k].z = fmaf(a[k].z, x, w * o[k].z);
+      a[k].w = fmaf(a[k].w, x, w * o[k].w);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kMergeRows; ++k) {
+    if (r0 + k >= u.rows || !mine) continue;
+    const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+    *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r0 + k) + 4 * lane) =
+        make_uint2(pack_bf16x2(a[k].x * inv, a[k].y * inv), pack_bf16x2(a[k].z * inv, a[k].w * inv));
+  }
+}
+
+// After the kernel that leaves the pieces, in its stream; launched early, it waits for that kernel's end by itself.
+template <typename F>
+int launch_merge(F* kernel, dim3 grid, int threads, const AttnParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.workers, ROWS / SUB);
-  cfg.blockDim = dim3(kMergeThreads);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<ROWS, SUB>, p) == cudaSuccess ? 0 : 946;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : 946;
 }
 
 inline long long workspace_bytes(long long workers, int rows, int dh) {

@@ -7,9 +7,12 @@
 // rescaled then only, and a weight stays below 2^8 times one of the true maximum (floating point loses nothing by it).
 //
 // bf16 pages come by TMA, one box per page and 64 columns, into the 128-byte-swizzled tiles that the instructions
-// read: K-major for K, MN-major for V.  8-bit codes are read by four warps, converted to fp16 (exactly) on the way to
-// the same layout; as in the few-row kernel the keys' scales go to the scores, the values' to the exponents.  Rows of V
-// that no query row sees are zeros, whatever the page holds there.
+// read: K-major for K, MN-major for V.  8-bit codes are read by four warps and go to the same layout as fp16 numbers,
+// code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: rounded once, by 2^-11 at
+// most (an eighth of a weight's rounding and far below the codes' own; a scale per column in the softmax would cost
+// each thread three shared-memory reads per column).  2^e of the keys goes to the scores, 2^e of the values, as in
+// the few-row kernel, to the exponents and out of the sum.  Rows of V that no query row sees are zeros, whatever the
+// page holds there; a scale that is no number makes the scores of its position NaN.
 //
 // The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
@@ -27,27 +30,17 @@ constexpr int kMeta = 4;                    // slots of scales and absences: a s
 constexpr float kSlack = 8.f;               // how far (in powers of two) a maximum may grow before O is rescaled
 constexpr int kLeast = 2;                   // tiles of a run
 
-// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warpgroup 2: MMA issue (warp 8), TMA (warp 9).  Warpgroup 3, 8-bit
-// kinds: loaders.  Registers: what a warpgroup takes comes out of the launch's own.
+// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8 and 9: MMA issue, TMA.  Warpgroup 3, 8-bit kinds: loaders.
 template <int KIND>
-struct Roles {
-  static constexpr int kThreads = KIND == kBf16 ? 384 : 512;
-  static constexpr int kLaunchRegs = KIND == kBf16 ? 168 : 128;
-  static constexpr int kSoftmaxRegs = KIND == kBf16 ? 192 : 144;
-  static constexpr int kIssueRegs = KIND == kBf16 ? 120 : 112;
-  static constexpr int kLoadRegs = KIND == kBf16 ? 0 : 112;
-  static_assert(2 * kSoftmaxRegs + kIssueRegs + kLoadRegs <= kLaunchRegs * (kThreads / 128), "setmaxnreg would wait forever");
-};
+constexpr int kThreadsOf = KIND == kBf16 ? 384 : 512;
 
 template <int NA>                            // 64-column atoms of a head
 struct Smem {
   static constexpr int kQ = 0;                                   // [2 tiles][NA atoms]
   static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages][NA]
   static constexpr int kV = kK + kStages * NA * kAtom;           // [kStages][NA]
-  static constexpr int kKs = kV + kStages * NA * kAtom;          // [kMeta][128] scales of the keys
-  static constexpr int kLv = kKs + kMeta * 512;                  // log2 of the values' scales
-  static constexpr int kRv = kLv + kMeta * 512;                  // their reciprocals
-  static constexpr int kBar = kRv + kMeta * 512;
+  static constexpr int kExp = kV + kStages * NA * kAtom;         // [kMeta][2][4] 2^e of the keys, e of the values
+  static constexpr int kBar = kExp + kMeta * 32;
   static constexpr int kTotal = kBar + 256 + 1024;
   static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
 };
@@ -81,10 +74,20 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-template <int REGS>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
-template <int REGS>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+// Two fp32 operations in an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.ftz.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.ftz.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 
 // Instruction descriptor, kind::f16, fp32 accumulators: A and B both bf16 or both fp16.
 __host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn_major) {
@@ -133,9 +136,8 @@ struct Bars {
 };
 
 template <int KIND, int NA>
-__global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
+__global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   using L = Smem<NA>;
-  using Rl = Roles<KIND>;
   constexpr bool kF16 = KIND != kBf16;
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
   extern __shared__ uint8_t smem_raw[];
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
   const Bars b = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 11, bars + 13, bars + 15};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* absent = tmem_slot + 2;    // [kMeta] bit i: no row sees sixteen positions i, or they have no page
+  volatile uint32_t* absent = tmem_slot + 2;    // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
   const AttnParams& p = cp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.w.c.dh, ksteps = dh >> 4;
 
@@ -188,7 +190,6 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
   seg.begin(p, lane, blockIdx.x, kLeast);
 
   if (warp >= 8 && warp < 12) {
-    regs_down<Rl::kIssueRegs>();
     if (warp == 8) {
       // ------------------------------------------------------------ MMA issue
       if (lane == 0) {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
           ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
           if (!ok) break;
           if (lane == 0) {
-            absent[nk % kMeta] = gone;
+            absent[nk % kMeta] = (gone & 3u) | (gone & 12u) << 6 | (gone & 48u) << 12 | (gone & 192u) << 18;
             mbar_expect_tx(&b.k_full[st], boxes * NA * box * 128);
           }
           __syncwarp();
@@ -323,68 +324,120 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
   } else if (warp >= 12) {
     // -------------------------------------------------------------- loaders of 8-bit pages
     if (kF16) {
-      regs_down<Rl::kLoadRegs == 0 ? 112 : Rl::kLoadRegs>();
-      const int tid = threadIdx.x - 384, shift = p.w.shift;
-      uint32_t nk = 0;
-      bool ok = true;
-      for (; seg.on() && ok; seg.next(p)) {
-        const Unit& u = seg.u;
-        const int n = max(work_of(p, seg, 0), work_of(p, seg, 1));
-        const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
-        for (int j = 0; j < n && ok; ++j, ++nk) {
-          const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1, slot = nk % kMeta;
-          const int x = place(u, seg.t0 + j) + tid;                      // this thread's position: a row of K and of V
-          int id = -1;
-          const int x16 = x & ~15;
-          if (x16 < u.hi && (x16 + 16 > u.lo || x16 < u.s_end)) {
-            id = __ldg(table + (x >> shift));
-            if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
-              atomicExch(p.w.c.status, kStatusBadPage);
-              id = -1;
-            }
-          }
-          const uint32_t none = __ballot_sync(0xffffffffu, id < 0);      // two sixteens of this warp
-          const bool on = id >= 0 && x < u.hi && (x >= u.lo || x < u.s_end);
-          const size_t row = on ? slot_row(p.w, id, u.h, x) : 0;
-          const float ks = on ? __ldg(p.w.c.k_scale + row) : 0.f;
-          float vs = on ? __ldg(p.w.c.v_scale + row) : 1.f;
-          vs = vs < kLeastScale ? kLeastScale : vs;                      // keeps NaN
-          auto fill = [&](const void* pool, uint32_t tile) {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + row * dh);
-#pragma unroll
-            for (int c = 0; c < 4 * NA; ++c) {                            // sixteen codes: two words of eight columns
-              if (c < ksteps) {
-                const uint4 r = on ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
-                const uint2 a = codes_to_f16<KIND, false>(r.x), d = codes_to_f16<KIND, false>(r.y),
-                            e = codes_to_f16<KIND, false>(r.z), f = codes_to_f16<KIND, false>(r.w);
-                st_shared_v4(swz(tile, tid, 2 * c), a.x, a.y, d.x, d.y);
-                st_shared_v4(swz(tile, tid, 2 * c + 1), e.x, e.y, f.x, f.y);
-              }
-            }
-          };
-          ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
-          if (!ok) break;
-          reinterpret_cast<float*>(smem + L::kKs)[slot * kTP + tid] = ks;
-          reinterpret_cast<float*>(smem + L::kLv)[slot * kTP + tid] = log2_fast(vs);
-          reinterpret_cast<float*>(smem + L::kRv)[slot * kTP + tid] = __fdividef(1.f, vs);
-          if (lane == 0)
-            reinterpret_cast<volatile uint8_t*>(absent + slot)[warp - 12] = (none & 0xffffu ? 1 : 0) | (none >> 16 ? 2 : 0);
-          fill(p.w.c.k, k_addr + st * NA * kAtom);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b.k_full[st]);
-          ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
-          if (!ok) break;
-          fill(p.w.c.v, v_addr + st * NA * kAtom);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&b.v_full[st]);
+      const int tid = threadIdx.x - 384, shift = p.w.shift;              // a thread per position: a row of K and of V
+      // the tile that is fetched, one ahead of the one that is stored
+      int j = 0, n = 0;
+      auto more = [&]() {                                                // skips segments without work
+        while (seg.on()) {
+          n = max(work_of(p, seg, 0), work_of(p, seg, 1));
+          if (j < n) return true;
+          j = 0;
+          seg.next(p);
         }
+        return false;
+      };
+      struct Row { bool on, gone; size_t at; float ks, vs; };
+      auto find = [&]() {
+        const Unit& u = seg.u;
+        const int x = place(u, seg.t0 + j) + tid, x16 = x & ~15;
+        int id = -1;
+        if (x16 < u.hi && (x16 + 16 > u.lo || x16 < u.s_end)) {
+          id = __ldg(p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width + (x >> shift));
+          if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
+            atomicExch(p.w.c.status, kStatusBadPage);
+            id = -1;
+          }
+        }
+        Row r;
+        r.gone = id < 0;
+        r.on = id >= 0 && x < u.hi && (x >= u.lo || x < u.s_end);
+        r.at = r.on ? slot_row(p.w, id, u.h, x) : 0;
+        r.ks = r.on ? __ldg(p.w.c.k_scale + r.at) : 0.f;
+        r.vs = r.on ? __ldg(p.w.c.v_scale + r.at) : 0.f;
+        return r;
+      };
+      auto fetch = [&](const void* pool, const Row& r, uint4 (&raw)[4 * NA]) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + r.at * dh);
+#pragma unroll
+        for (int c = 0; c < 4 * NA; ++c) raw[c] = r.on && c < ksteps ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+      };
+      // biased exponent of the warp's largest finite scale: that of 1 where there is none, and of 2^-107 at least, so
+      // that its products with a score's factor do not vanish
+      auto largest = [&](float x) {
+        uint32_t e = (__float_as_uint(x) >> 23) & 0xffu;
+        e = e == 255u ? 0u : e;
+        e = __reduce_max_sync(0xffffffffu, e);
+        return e == 0u ? 127u : max(e, 20u);
+      };
+      // codes * r as fp16, r in two parts: the product is rounded once
+      auto store = [&](const uint4 (&raw)[4 * NA], uint32_t tile, float r) {
+        const __half hi = __float2half_rn(r), lo = __float2half_rn(r - __half2float(hi));
+        const __half2 h2 = __half2half2(hi), l2 = __half2half2(lo);
+        auto scaled = [&](uint32_t x) {
+          const __half2 v = *reinterpret_cast<const __half2*>(&x);
+          const __half2 y = __hfma2(v, h2, __hmul2(v, l2));
+          return *reinterpret_cast<const uint32_t*>(&y);
+        };
+#pragma unroll
+        for (int c = 0; c < 4 * NA; ++c) {                                // sixteen codes: two words of eight columns
+          if (c < ksteps) {
+            const uint2 a = codes_to_f16<KIND, false>(raw[c].x), d = codes_to_f16<KIND, false>(raw[c].y),
+                        e = codes_to_f16<KIND, false>(raw[c].z), f = codes_to_f16<KIND, false>(raw[c].w);
+            st_shared_v4(swz(tile, tid, 2 * c), scaled(a.x), scaled(a.y), scaled(d.x), scaled(d.y));
+            st_shared_v4(swz(tile, tid, 2 * c + 1), scaled(e.x), scaled(e.y), scaled(f.x), scaled(f.y));
+          }
+        }
+      };
+      uint4 kraw[4 * NA], vraw[4 * NA];
+      Row r = {false, true, 0, 0.f, 0.f};
+      bool have = more(), ok = true;
+      if (have) {
+        r = find();
+        fetch(p.w.c.k, r, kraw);
+        fetch(p.w.c.v, r, vraw);
+      }
+      for (uint32_t nk = 0; have && ok; ++nk) {
+        const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1, slot = nk % kMeta;
+        const uint32_t none = __ballot_sync(0xffffffffu, r.gone);         // two sixteens of this warp
+        const uint32_t ek = largest(r.ks), ev = largest(r.vs);
+        // 2^(127 - e) as a float: e of 254 at most
+        float rk = r.ks * __uint_as_float((254u - ek) << 23), rv = r.vs * __uint_as_float((254u - ev) << 23);
+        const bool odd = !(fabsf(r.ks) < INFINITY) || !(fabsf(r.vs) < INFINITY);
+        if (odd) {                                                        // NaN scores for whoever sees the position
+          rk = __uint_as_float(0x7fc00000u);
+          rv = 0.f;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
+        if (!ok) break;
+        if (lane == 0) {
+          float* e = reinterpret_cast<float*>(smem + L::kExp) + slot * 8 + (warp - 12);
+          e[0] = __uint_as_float(ek << 23);
+          e[4] = static_cast<float>(static_cast<int>(ev) - 127);
+          reinterpret_cast<volatile uint8_t*>(absent + slot)[warp - 12] = (none & 0xffffu ? 1 : 0) | (none >> 16 ? 2 : 0);
+        }
+        store(kraw, k_addr + st * NA * kAtom, rk);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.k_full[st]);
+        ++j;
+        have = more();
+        Row next = {false, true, 0, 0.f, 0.f};
+        if (have) {
+          next = find();
+          fetch(p.w.c.k, next, kraw);
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
+        if (!ok) break;
+        store(vraw, v_addr + st * NA * kAtom, rv);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.v_full[st]);
+        if (have) fetch(p.w.c.v, next, vraw);
+        r = next;
       }
     }
   } else {
     // -------------------------------------------------------------- softmax, a thread per query row
-    regs_up<Rl::kSoftmaxRegs>();
     const int i = warp >> 2, row = threadIdx.x - 128 * i;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
@@ -409,11 +462,15 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
         if (real) src += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
         float up = p.scale_log2 < 0.f ? -1.f : 1.f;
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+        uint4 v[8 * NA];
+#pragma unroll
+        for (int c = 0; c < 8 * NA; ++c)
+          v[c] = real && !flat && c < 2 * ksteps ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
         if (kF16) {
           uint32_t top = 0;
-          for (int c = 0; c < 2 * ksteps; ++c) {
-            const uint4 v = real && !flat ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int c = 0; c < 8 * NA; ++c) {
+            const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
           }
@@ -423,17 +480,17 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
             f *= __uint_as_float((e - 7u) << 23);
           }
         }
-        for (int c = 0; c < 2 * ksteps; ++c) {
-          uint4 v = real && !flat ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < 8 * NA; ++c) {
+          if (c >= 2 * ksteps) continue;
           if (kF16) {
             float t[8];
-            bf16x8_to_f32(v, t);
-            v = make_uint4(pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up), pack_f16x2(t[4] * up, t[5] * up),
-                           pack_f16x2(t[6] * up, t[7] * up));
+            bf16x8_to_f32(v[c], t);
+            st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
+                         pack_f16x2(t[4] * up, t[5] * up), pack_f16x2(t[6] * up, t[7] * up));
           } else {
-            v = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+            st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
           }
-          st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), v.x, v.y, v.z, v.w);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -449,47 +506,47 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
         const uint32_t gone = absent[st];
         const int x0 = place(u, seg.t0 + j);
         const bool hidden = gone != 0u || x0 + kTP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
-        const float* meta = reinterpret_cast<const float*>(smem + L::kKs) + st * kTP;
-        // scores (in powers of two) of columns 32 c ..: what a row does not see is -inf and weighs nothing
-        auto finish = [&](float* s, int c) {
-          if (kF16) {
+        // of columns 32 c ..: score (in powers of two) = product * fc + ev
+        float fc[4] = {f, f, f, f}, ev[4] = {0.f, 0.f, 0.f, 0.f};
+        if (kF16) {
+          const float* e = reinterpret_cast<const float*>(smem + L::kExp) + st * 8;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 ks = reinterpret_cast<const float4*>(meta)[8 * c + k];
-              const float4 lv = reinterpret_cast<const float4*>(meta + kMeta * kTP)[8 * c + k];
-              s[4 * k] = fmaf(s[4 * k] * f, ks.x, lv.x);
-              s[4 * k + 1] = fmaf(s[4 * k + 1] * f, ks.y, lv.y);
-              s[4 * k + 2] = fmaf(s[4 * k + 2] * f, ks.z, lv.z);
-              s[4 * k + 3] = fmaf(s[4 * k + 3] * f, ks.w, lv.w);
-            }
-          }
-          if (hidden) {
-            const uint32_t seen = seen32(x0 + 32 * c, pos, p.window, p.sinks, gone >> (2 * c));
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (((seen >> k) & 1u) == 0u) s[k] = -INFINITY;
-          }
-        };
-        float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float s[64];
-          tmem_ld32(s_at + 64 * h, s);
-          tmem_ld32(s_at + 64 * h + 32, s + 32);
-          tmem_ld_wait_dep32(s);
-          tmem_ld_wait_dep32(s + 32);
-          finish(s, 2 * h);
-          finish(s + 32, 2 * h + 1);
-#pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            t0 = fmaxf(t0, s[c]);
-            t1 = fmaxf(t1, s[c + 1]);
-            t2 = fmaxf(t2, s[c + 2]);
-            t3 = fmaxf(t3, s[c + 3]);
+          for (int c = 0; c < 4; ++c) {
+            fc[c] *= e[c];
+            ev[c] = e[4 + c];
           }
         }
-        const float most = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-        const float top = fmaxf(kF16 ? most : most * f, kFloor);          // f >= 0
+        // two passes over S in TMEM, 64 and 32 columns at a time: a row of 128 would not fit the registers
+        auto hide = [&](float* x, int c) {             // what a row does not see is -inf and weighs nothing
+          const uint32_t seen = seen32(x0 + 32 * c, pos, p.window, p.sinks, gone >> (8 * c));
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (((seen >> k) & 1u) == 0u) x[k] = -INFINITY;
+        };
+        float top = kFloor;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[64];
+          tmem_ld32(s_at + 64 * h, x);
+          tmem_ld32(s_at + 64 * h + 32, x + 32);
+          tmem_ld_wait_dep32(x);
+          tmem_ld_wait_dep32(x + 32);
+          if (hidden) {
+            hide(x, 2 * h);
+            hide(x + 32, 2 * h + 1);
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float* y = x + 32 * c;
+            float t0 = fmaxf(y[0], y[1]), t1 = fmaxf(y[2], y[3]);
+#pragma unroll
+            for (int k = 4; k < 32; k += 4) {
+              t0 = fmaxf(fmaxf(t0, y[k]), y[k + 1]);
+              t1 = fmaxf(fmaxf(t1, y[k + 2]), y[k + 3]);
+            }
+            top = fmaxf(top, fmaf(fmaxf(t0, t1), fc[2 * h + c], ev[2 * h + c]));       // fc >= 0
+          }
+        }
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
@@ -509,7 +566,6 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
         }
         // fp16 weights: 2^14 at most, so that 2^-24 of one is 2^-30 of the reference
         const float ref = kF16 ? m - 6.f : m;
-        float l0 = 0.f, l1 = 0.f;
         float s[2][32];
         tmem_ld32(s_at, s[0]);
 #pragma unroll
@@ -517,30 +573,22 @@ __global__ void __launch_bounds__(Roles<KIND>::kThreads, 1) paged_chunk_kernel(c
           float* x = s[c & 1];
           tmem_ld_wait_dep32(x);
           if (c < 3) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-          finish(x, c);
+          if (hidden) hide(x, c);
+          const float off = ev[c] - ref;
+          float2 sum = make_float2(0.f, 0.f);
           uint32_t w[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k + e] = exp2_fast(kF16 ? x[k + e] - ref : fmaf(x[k + e], f, -ref));
-            if (kF16) {
-              const float4 rv = reinterpret_cast<const float4*>(meta + 2 * kMeta * kTP)[8 * c + k / 4];
-              l0 = fmaf(x[k], rv.x, l0);
-              l1 = fmaf(x[k + 1], rv.y, l1);
-              l0 = fmaf(x[k + 2], rv.z, l0);
-              l1 = fmaf(x[k + 3], rv.w, l1);
-              w[k / 2] = pack_f16x2(x[k], x[k + 1]);
-              w[k / 2 + 1] = pack_f16x2(x[k + 2], x[k + 3]);
-            } else {
-              l0 += x[k] + x[k + 2];
-              l1 += x[k + 1] + x[k + 3];
-              w[k / 2] = pack_bf16x2(x[k], x[k + 1]);
-              w[k / 2 + 1] = pack_bf16x2(x[k + 2], x[k + 3]);
-            }
+          for (int k = 0; k < 32; k += 2) {
+            float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(fc[c], fc[c]), make_float2(off, off));
+            y.x = exp2_fast(y.x);
+            y.y = exp2_fast(y.y);
+            sum = add2(sum, y);
+            w[k / 2] = kF16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
           }
           tmem_st16(p_at + 16 * c, w);             // where P takes the place of S: columns already read
+          const float part = sum.x + sum.y;
+          l += kF16 ? part * exp2_fast(-ev[c]) : part;
         }
-        l += l0 + l1;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -617,7 +665,7 @@ int launch(const ChunkParams& p, cudaStream_t stream) {
   if (cudaFuncSetAttribute(paged_chunk_kernel<KIND, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA>::kTotal) !=
       cudaSuccess)
     return 950;
-  paged_chunk_kernel<KIND, NA><<<p.a.workers, Roles<KIND>::kThreads, Smem<NA>::kTotal, stream>>>(p);
+  paged_chunk_kernel<KIND, NA><<<p.a.workers, kThreadsOf<KIND>, Smem<NA>::kTotal, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : 951;
 }
 
@@ -645,7 +693,8 @@ int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
   } else {
     rc = launch_dim<kInt8>(p, stream);
   }
-  return rc ? rc : launch_merge<kUnitRows, 16>(a, stream);
+  return rc ? rc : launch_merge(paged_merge_rows_kernel<kUnitRows>, dim3(a.workers, kUnitRows / (kMergeRows * kMergeWarps)),
+                                32 * kMergeWarps, a, stream);
 }
 
 }  // namespace paged
