@@ -16,6 +16,8 @@
 //
 // The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
+#include <type_traits>
+
 #include "common/host_utils.cuh"
 #include "common/paged_launch.h"
 
@@ -65,6 +67,57 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// 64 columns of this thread's row, complete on return (loads whose values pass through a later wait cost a register
+// move each).
+__device__ __forceinline__ void tmem_ld64_now(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+        "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+        "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+      : "r"(taddr)
+      : "memory");
+}
+// 32 columns of this thread's row, complete on return (loads whose values pass through a later wait cost a register
+// move each).
+__device__ __forceinline__ void tmem_ld32_now(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 columns of this thread's row, complete on return (loads whose values pass through a later wait cost a register
+// move each).
+__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15"
+      "}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -121,6 +174,41 @@ __device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks
   auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
   const uint32_t by = below(pos - x + 1), old = below(pos - window + 1 - x) & ~below(sinks - x);
   return by & ~old & ((gone & 1u) ? 0xffff0000u : 0xffffffffu) & ((gone & 2u) ? 0x0000ffffu : 0xffffffffu);
+}
+
+// D = A B^T over KS steps of sixteen columns, both K-major.
+template <int KS>
+__device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < KS; ++kk) {
+    const uint32_t off = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
+    mma_bf16_ss(d, a + off, b + off, idesc, kk > 0 ? 1u : 0u);
+  }
+}
+
+// mbar_wait for the waits between softmax and MMA, one after the other in every tile: no sleeping in between.
+__device__ __forceinline__ bool wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  long long t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 0xff) == 0xff) {
+      if (*abort_flag) return false;
+      const long long now = clock64();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > kWaitLimitCycles) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// One lane of the warp, in a form that tells the compiler that it is one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on != 0u;
 }
 
 struct Bars {
@@ -192,53 +280,67 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   if (warp >= 8 && warp < 12) {
     if (warp == 8) {
       // ------------------------------------------------------------ MMA issue
-      if (lane == 0) {
+      if (elect_one()) {
+        // one lane does all of it; what does not change from tile to tile is a constant or made beforehand, so that an
+        // instruction costs few moves to uniform registers
         const uint32_t idesc_s = idesc16(!kF16, kTileRows, kTP, 0), idesc_o = idesc16(!kF16, kTileRows, dh, 1);
+        const uint64_t q_desc = desc_k(q_addr, 0), k_desc = desc_k(k_addr, 0), v_desc = desc_mn(v_addr, 0);
+        constexpr uint32_t kStage16 = NA * kAtom >> 4;        // a stage, or a query tile, in a descriptor's units
         // stages so far, and of each tile segments with work and P: a phase of a barrier is waited for by whoever
         // takes part in it, and by nobody else, so that no one is ever two phases off
-        uint32_t nk = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+        uint32_t nk = 0, nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;
         bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && wait_hot(bar, phase & 1, abort_flag); };
         for (; seg.on() && ok; seg.next(p)) {
           const int n0 = work_of(p, seg, 0), n1 = work_of(p, seg, 1), n = max(n0, n1);
-          auto work = [&](int i) { return i == 0 ? n0 : n1; };
-          for (int i = 0; i < 2 && ok; ++i)
-            if (work(i) > 0) ok = mbar_wait(&b.q_full[i], nq[i]++ & 1, abort_flag);
-          // S_i of the segment's j-th tile (K stage nk + j); the last of the two frees the stage
-          auto issue_s = [&](int i, int j) {
-            const uint32_t st = (nk + j) % kStages, par = ((nk + j) / kStages) & 1;
-            if (!mbar_wait(&b.k_full[st], par, abort_flag)) return false;
+          if (n0 > 0) wait(&b.q_full[0], nq0++);
+          if (n1 > 0) wait(&b.q_full[1], nq1++);
+          // S of tile I and the segment's j-th tile of positions; the last of the two frees the stage
+          auto issue_s = [&](auto tile, int j) {
+            constexpr int I = decltype(tile)::value;
+            const uint32_t st = (nk + j) % kStages;
+            wait(&b.k_full[st], (nk + j) / kStages);
+            if (!ok) return;
             tc_fence_after();
-            const uint32_t qa = q_addr + i * NA * kAtom, ka = k_addr + st * NA * kAtom;
-#pragma unroll 1
-            for (int kk = 0; kk < ksteps; ++kk) mma_bf16_ss(s_col(i), desc_k(qa, kk), desc_k(ka, kk), idesc_s, kk > 0);
-            mma_commit(&b.s_full[i]);
-            if (j >= work(1 - i) || i == 1) mma_commit(&b.k_empty[st]);
-            return true;
-          };
-#pragma unroll 1
-          for (int i = 0; i < 2 && ok; ++i)
-            if (work(i) > 0) ok = issue_s(i, 0);
-          for (int j = 0; j < n && ok; ++j) {
-            const uint32_t st = (nk + j) % kStages, par = ((nk + j) / kStages) & 1;
-#pragma unroll 1
-            for (int i = 0; i < 2 && ok; ++i) {
-              if (j >= work(i)) continue;
-              ok = mbar_wait(&b.p_full[i], np[i] & 1, abort_flag) && mbar_wait(&b.v_full[st], par, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t va = v_addr + st * NA * kAtom;
-#pragma unroll 1
-              for (int kk = 0; kk < kTP / 16; ++kk)
-                mma_ts(o_col(i), p_col(i) + 8 * kk, desc_mn(va, kk), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-              mma_commit(&b.o_done[i]);
-              if (j >= work(1 - i) || i == 1) mma_commit(&b.v_empty[st]);
-              if (j + 1 < work(i)) {
-                // the next S takes the columns that this P is being read from
-                if (kAlias) ok = mbar_wait(&b.o_done[i], np[i] & 1, abort_flag);
-                if (ok) ok = issue_s(i, j + 1);
-              }
-              ++np[i];
+            const uint64_t ka = k_desc + st * kStage16;
+            const uint64_t qa = q_desc + I * kStage16;
+            switch (ksteps - 4 * (NA - 1)) {                // no instruction under a condition of its own
+              case 1: issue_qk<4 * NA - 3>(s_col(I), qa, ka, idesc_s); break;
+              case 2: issue_qk<4 * NA - 2>(s_col(I), qa, ka, idesc_s); break;
+              case 3: issue_qk<4 * NA - 1>(s_col(I), qa, ka, idesc_s); break;
+              default: issue_qk<4 * NA>(s_col(I), qa, ka, idesc_s);
             }
+            mma_commit(&b.s_full[I]);
+            if (I == 1 || j >= n1) mma_commit(&b.k_empty[st]);
+          };
+          auto issue_o = [&](auto tile, int j, uint32_t& np) {
+            constexpr int I = decltype(tile)::value;
+            const int mine = I == 0 ? n0 : n1;
+            if (j >= mine || !ok) return;
+            const uint32_t st = (nk + j) % kStages;
+            wait(&b.v_full[st], (nk + j) / kStages);
+            wait(&b.p_full[I], np);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t va = v_desc + st * kStage16;
+            mma_ts(o_col(I), p_col(I), va, idesc_o, j > 0);
+#pragma unroll
+            for (int kk = 1; kk < kTP / 16; ++kk) mma_ts(o_col(I), p_col(I) + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
+            mma_commit(&b.o_done[I]);
+            if (I == 1 || j >= n1) mma_commit(&b.v_empty[st]);
+            if (j + 1 < mine) {
+              if (kAlias) wait(&b.o_done[I], np);         // the next S takes the columns that this P is being read from
+              if (ok) issue_s(tile, j + 1);
+            }
+            ++np;
+          };
+          using Tile0 = std::integral_constant<int, 0>;
+          using Tile1 = std::integral_constant<int, 1>;
+          if (n0 > 0 && ok) issue_s(Tile0{}, 0);
+          if (n1 > 0 && ok) issue_s(Tile1{}, 0);
+          for (int j = 0; j < n && ok; ++j) {
+            issue_o(Tile0{}, j, np0);
+            issue_o(Tile1{}, j, np1);
           }
           nk += n;
         }
@@ -500,7 +602,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       for (int j = 0; j < mine; ++j, ++ns) {
         const uint32_t st = (nk + j) % kMeta;
         // also says that all MMAs issued before are done: P and O of the last tile
-        ok = __all_sync(0xffffffffu, mbar_wait(&b.s_full[i], ns & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, wait_hot(&b.s_full[i], ns & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         const uint32_t gone = absent[st];
@@ -516,25 +618,27 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             ev[c] = e[4 + c];
           }
         }
-        // two passes over S in TMEM, 64 and 32 columns at a time: a row of 128 would not fit the registers
-        auto hide = [&](float* x, int c) {             // what a row does not see is -inf and weighs nothing
-          const uint32_t seen = seen32(x0 + 32 * c, pos, p.window, p.sinks, gone >> (8 * c));
+        // what a row does not see is -inf and weighs nothing: in TMEM, so that the tiles in between, most of them, have
+        // nothing to do with it
+        if (hidden) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            float x[16];
+            tmem_ld16_now(s_at + 16 * c, x);
+            const uint32_t seen = seen32(x0 + 16 * c, pos, p.window, p.sinks, gone >> (8 * (c >> 1) + (c & 1)));
+            uint32_t w[16];
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (((seen >> k) & 1u) == 0u) x[k] = -INFINITY;
-        };
+            for (int k = 0; k < 16; ++k) w[k] = (seen >> k) & 1u ? __float_as_uint(x[k]) : 0xff800000u;
+            tmem_st16(s_at + 16 * c, w);
+          }
+          tmem_st_wait();
+        }
+        // two passes over S, 64 and 32 columns at a time: a row of 128 would not fit the registers
         float top = kFloor;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x[64];
-          tmem_ld32(s_at + 64 * h, x);
-          tmem_ld32(s_at + 64 * h + 32, x + 32);
-          tmem_ld_wait_dep32(x);
-          tmem_ld_wait_dep32(x + 32);
-          if (hidden) {
-            hide(x, 2 * h);
-            hide(x + 32, 2 * h + 1);
-          }
+          tmem_ld64_now(s_at + 64 * h, x);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float* y = x + 32 * c;
@@ -553,8 +657,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           const float m_new = fmaxf(m, top), d = exp2_fast(m - m_new);
           for (int c = 0; c < ksteps; ++c) {
             float o[16];
-            tmem_ld16(o_at + 16 * c, o);
-            tmem_ld_wait_dep16(o);
+            tmem_ld16_now(o_at + 16 * c, o);
             uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(o[k] * d);
@@ -566,14 +669,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         // fp16 weights: 2^14 at most, so that 2^-24 of one is 2^-30 of the reference
         const float ref = kF16 ? m - 6.f : m;
-        float s[2][32];
-        tmem_ld32(s_at, s[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float* x = s[c & 1];
-          tmem_ld_wait_dep32(x);
-          if (c < 3) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-          if (hidden) hide(x, c);
+          float x[32];
+          tmem_ld32_now(s_at + 32 * c, x);
           const float off = ev[c] - ref;
           float2 sum = make_float2(0.f, 0.f);
           uint32_t w[16];
@@ -609,8 +708,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       for (int c = 0; c < ksteps; ++c) {
         float o[16];
         if (mine > 0) {
-          tmem_ld16(o_at + 16 * c, o);
-          tmem_ld_wait_dep16(o);
+          tmem_ld16_now(o_at + 16 * c, o);
         } else {
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = 0.f;
