@@ -130,9 +130,11 @@ __device__ __forceinline__ void zero_other_rows(const AttnParams& p, int worker,
   }
 }
 
-__device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) {
-  return p.out + (static_cast<size_t>(u.first + row / p.G) * p.Hq + u.h * p.G + row % p.G) * p.w.c.dh;
+// Row `row` (token, query head of the group) of key/value head h of a sequence.
+__device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, int first, int h, int row) {
+  return p.out + (static_cast<size_t>(first + row / p.G) * p.Hq + h * p.G + row % p.G) * p.w.c.dh;
 }
+__device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) { return out_row(p, u.first, u.h, row); }
 
 // Where a worker's run of tiles begins, among all tiles of all units in order (sequence, head, row tile).
 struct Run { long long begin, end, total; };

@@ -29,10 +29,12 @@ constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows, kTP = 128;
 constexpr int kAtom = kTP * 128;            // 128 rows x 64 16-bit columns
 constexpr int kStages = 2;
 constexpr int kMeta = 4;                    // slots of scales and absences: a softmax is at most two tiles behind the loads
+constexpr int kPlans = 4;                   // segments that the planning warp is ahead of the others at most
 constexpr float kSlack = 8.f;               // how far (in powers of two) a maximum may grow before O is rescaled
 constexpr int kLeast = 2;                   // tiles of a run
 
-// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8 and 9: MMA issue, TMA.  Warpgroup 3, 8-bit kinds: loaders.
+// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8, 9 and 10: MMA issue, TMA, the plan.  Warpgroup 3, 8-bit
+// kinds: loaders.
 template <int KIND>
 constexpr int kThreadsOf = KIND == kBf16 ? 384 : 512;
 
@@ -42,7 +44,8 @@ struct Smem {
   static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages][NA]
   static constexpr int kV = kK + kStages * NA * kAtom;           // [kStages][NA]
   static constexpr int kExp = kV + kStages * NA * kAtom;         // [kMeta][2][4] 2^e of the keys, e of the values
-  static constexpr int kBar = kExp + kMeta * 32;
+  static constexpr int kPlan = kExp + kMeta * 32;                // [kPlans] segments ahead
+  static constexpr int kBar = kPlan + kPlans * 128;
   static constexpr int kTotal = kBar + 256 + 1024;
   static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
 };
@@ -163,11 +166,18 @@ __device__ __forceinline__ int tiles_of(const AttnParams& p, const Unit& u, int 
   return min(u.tiles, end <= u.st ? end : max(end - u.skip, u.st));
 }
 
-// Tiles of a segment that query tile i works on.
-__device__ __forceinline__ int work_of(const AttnParams& p, const Segments<kUnitRows, kTP>& s, int i) {
-  return max(0, min(s.t1, tiles_of(p, s.u, i)) - s.t0);
-}
-__device__ __forceinline__ int place(const Unit& u, int tile) { return (tile < u.st ? tile : tile + u.skip) * kTP; }
+// A segment as the roles need it.  One warp works it out, ahead of them: the index arithmetic, with its divisions and
+// dependent loads, took every warp some 3000 cycles a segment.
+struct Plan {
+  int b, h, rt;                     // b < 0: there are no more
+  int len, n, first, rows;
+  int lo, hi, s_end, st, skip;
+  int t0, n0, n1;                   // first tile of positions; how many from there each query tile works on
+  int whole, slot;
+};
+static_assert(sizeof(Plan) <= 128, "slot of a plan");
+
+__device__ __forceinline__ int place(const Plan& q, int j) { return (q.t0 + j < q.st ? q.t0 + j : q.t0 + j + q.skip) * kTP; }
 
 // Bit k: a row at position pos sees position x + k; gone: bits of the two sixteens from x.
 __device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks, uint32_t gone) {
@@ -184,6 +194,12 @@ __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uin
     const uint32_t off = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
     mma_bf16_ss(d, a + off, b + off, idesc, kk > 0 ? 1u : 0u);
   }
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
 // mbar_wait for the waits between softmax and MMA, one after the other in every tile: no sleeping in between.
@@ -221,6 +237,28 @@ struct Bars {
   uint64_t* s_full;     // [2]
   uint64_t* p_full;     // [2] P is in TMEM, S has been read (4 warps)
   uint64_t* o_done;     // [2]
+  uint64_t* plan_full;  // [kPlans]
+  uint64_t* plan_empty; // [kPlans] every warp that works by the plan has read it
+};
+
+// The plans in order, for one warp.
+struct Plans {
+  const Plan* ring;
+  uint64_t* full;
+  uint64_t* empty;
+  volatile int* abort_flag;
+  uint32_t k;
+  // false: no more, or the block gives up
+  __device__ __forceinline__ bool next(Plan& q, int lane) {
+    const uint32_t slot = k % kPlans;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (k / kPlans) & 1, abort_flag));
+    if (!ok) return false;
+    q = ring[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[slot]);
+    ++k;
+    return q.b >= 0;
+  }
 };
 
 template <int KIND, int NA>
@@ -231,8 +269,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  const Bars b = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 11, bars + 13, bars + 15};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  const Bars b = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 11, bars + 13, bars + 15, bars + 17, bars + 21};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* absent = tmem_slot + 2;    // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
   const AttnParams& p = cp.a;
@@ -252,6 +290,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.v_empty[i], 1);
     }
     mbar_init(b.v_fix, 1);
+    for (int i = 0; i < kPlans; ++i) {
+      mbar_init(&b.plan_full[i], 1);
+      mbar_init(&b.plan_empty[i], kF16 ? 13 : 10);      // softmax, MMA, and TMA or loaders
+    }
     *abort_flag = 0;
     fence_barrier_init();
     if (!kF16) {
@@ -273,9 +315,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   auto o_col = [&](int i) { return tmem + 256 + 64 * NA * i; };
   auto p_col = [&](int i) { return kAlias ? s_col(i) : tmem + 384 + 64 * i; };
 
-  zero_other_rows(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
-  Segments<kUnitRows, kTP> seg;
-  seg.begin(p, lane, blockIdx.x, kLeast);
+  Plan* plan_ring = reinterpret_cast<Plan*>(smem + L::kPlan);
+  static_assert(kPlans * sizeof(Plan) <= kPlans * 128, "ring of plans");
+  Plans plans = {plan_ring, b.plan_full, b.plan_empty, abort_flag, 0};
+  Plan u;
 
   if (warp >= 8 && warp < 12) {
     if (warp == 8) {
@@ -291,8 +334,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         uint32_t nk = 0, nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && wait_hot(bar, phase & 1, abort_flag); };
-        for (; seg.on() && ok; seg.next(p)) {
-          const int n0 = work_of(p, seg, 0), n1 = work_of(p, seg, 1), n = max(n0, n1);
+        // the plan's part of this warp's, by its one lane
+        for (uint32_t k = 0; ok; ++k) {
+          const uint32_t slot = k % kPlans;
+          wait(&b.plan_full[slot], k / kPlans);
+          if (!ok) break;
+          const int n0 = plan_ring[slot].n0, n1 = plan_ring[slot].n1, n = max(n0, n1), more = plan_ring[slot].b;
+          mbar_arrive(&b.plan_empty[slot]);
+          if (more < 0) break;
           if (n0 > 0) wait(&b.q_full[0], nq0++);
           if (n1 > 0) wait(&b.q_full[1], nq1++);
           // S of tile I and the segment's j-th tile of positions; the last of the two frees the stage
@@ -350,13 +399,12 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       uint32_t nk = 0, fixes = 0;
       bool ok = true;
       const int shift = p.w.shift, box = min(p.w.c.page, kTP);
-      for (; seg.on() && ok; seg.next(p)) {
-        const Unit& u = seg.u;
-        const int n = max(work_of(p, seg, 0), work_of(p, seg, 1));
+      while (ok && plans.next(u, lane)) {
+        const int n = max(u.n0, u.n1);
         const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
         for (int j = 0; j < n && ok; ++j, ++nk) {
           const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1;
-          const int x0 = place(u, seg.t0 + j);
+          const int x0 = place(u, j);
           // lane i < 8: the page of sixteen positions i, -1 where no row sees any of them
           int id = -1;
           const int x = x0 + 16 * lane;
@@ -418,10 +466,35 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       }
     }
     else if (warp == 10) {
-      // ------------------------------------------------------------ notes for the merge
+      // ------------------------------------------------------------ the plan, and notes for the merge
+      Segments<kUnitRows, kTP> seg;
       int4 meta = make_int4(-1, 0, 0, 0);
-      for (; seg.on(); seg.next(p)) seg.note(meta);
+      uint32_t k = 0;
+      bool ok = true;
+      for (seg.begin(p, lane, blockIdx.x, kLeast); ok; ++k) {
+        const bool more = seg.on();
+        const uint32_t slot = k % kPlans;
+        ok = __all_sync(0xffffffffu, mbar_wait(&b.plan_empty[slot], ((k / kPlans) & 1) ^ 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) {
+          Plan q = {-1};
+          if (more) {
+            const Unit& x = seg.u;
+            q = {x.b, x.h, x.rt, x.len, x.n, x.first, x.rows, x.lo, x.hi, x.s_end, x.st, x.skip, seg.t0,
+                 max(0, min(seg.t1, tiles_of(p, x, 0)) - seg.t0), max(0, min(seg.t1, tiles_of(p, x, 1)) - seg.t0),
+                 seg.whole() ? 1 : 0, seg.slot()};
+          }
+          plan_ring[slot] = q;
+          mbar_arrive(&b.plan_full[slot]);
+        }
+        __syncwarp();
+        if (!more) break;
+        seg.note(meta);
+        seg.next(p);
+      }
       if (lane == 0) p.meta[blockIdx.x] = meta;
+    } else if (warp == 11) {
+      zero_other_rows(p, blockIdx.x * 32 + lane, gridDim.x * 32);
     }
   } else if (warp >= 12) {
     // -------------------------------------------------------------- loaders of 8-bit pages
@@ -430,18 +503,16 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       // the tile that is fetched, one ahead of the one that is stored
       int j = 0, n = 0;
       auto more = [&]() {                                                // skips segments without work
-        while (seg.on()) {
-          n = max(work_of(p, seg, 0), work_of(p, seg, 1));
-          if (j < n) return true;
+        while (j >= n) {
+          if (!plans.next(u, lane)) return false;
+          n = max(u.n0, u.n1);
           j = 0;
-          seg.next(p);
         }
-        return false;
+        return true;
       };
       struct Row { bool on, gone; size_t at; float ks, vs; };
       auto find = [&]() {
-        const Unit& u = seg.u;
-        const int x = place(u, seg.t0 + j) + tid, x16 = x & ~15;
+        const int x = place(u, j) + tid, x16 = x & ~15;
         int id = -1;
         if (x16 < u.hi && (x16 + 16 > u.lo || x16 < u.s_end)) {
           id = __ldg(p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width + (x >> shift));
@@ -543,11 +614,22 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     const int i = warp >> 2, row = threadIdx.x - 128 * i;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
+    const uint32_t stage = q_addr + i * NA * kAtom;              // the query tile, and on the way out its results
+    constexpr int kRowLanes = 8 * NA, kRowStep = 32 / kRowLanes;
+    const int first_row = 32 * (warp & 3), words = 2 * ksteps;  // of this warp; 16-byte words of a row
+    const int word = lane % kRowLanes, sub_row = lane / kRowLanes;
+    auto read_o = [](float* o, uint32_t at, int c, bool any) {
+      if (any) {
+        tmem_ld16_now(at + 16 * c, o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = 0.f;
+      }
+    };
     uint32_t nk = 0, ns = 0;                       // tiles loaded, S of this tile so far
     bool ok = true;
-    for (; seg.on() && ok; seg.next(p)) {
-      const Unit& u = seg.u;
-      const int n0 = work_of(p, seg, 0), n1 = work_of(p, seg, 1), n = max(n0, n1), mine = i == 0 ? n0 : n1;
+    while (ok && plans.next(u, lane)) {
+      const int n = max(u.n0, u.n1), mine = i == 0 ? u.n0 : u.n1;
       const int ru = i * kTileRows + row;          // row of the unit
       const bool real = ru < u.rows;
       const int r = u.rt * kUnitRows + ru;         // row of the sequence's head
@@ -559,39 +641,45 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       const bool flat = p.scale_log2 == 0.f;
       float f = flat ? 1.f : fabsf(p.scale_log2);
       if (mine > 0) {
-        // queries into the swizzled tile; fp16 ones scaled by a power of two (see the few-row kernel)
-        const __nv_bfloat16* src = p.q;
-        if (real) src += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
-        float up = p.scale_log2 < 0.f ? -1.f : 1.f;
+        // queries into the swizzled tile: a warp its 32 rows, kRowLanes neighbouring lanes the words of a row
+        const __nv_bfloat16* src = nullptr;
+        if (real && !flat)
+          src = p.q + static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
         uint4 v[8 * NA];
 #pragma unroll
+        for (int c = 0; c < 8 * NA; ++c) {
+          const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), kRowStep * c + sub_row));
+          v[c] = from != nullptr && word < words ? __ldg(reinterpret_cast<const uint4*>(from) + word) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
         for (int c = 0; c < 8 * NA; ++c)
-          v[c] = real && !flat && c < 2 * ksteps ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
-        if (kF16) {
+          if (word < words)
+            st_shared_v4(swz(stage, first_row + kRowStep * c + sub_row, word), v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
+        if (kF16) {                                // fp16 queries, scaled by a power of two (see the few-row kernel)
+          __syncwarp();
           uint32_t top = 0;
 #pragma unroll
           for (int c = 0; c < 8 * NA; ++c) {
+            v[c] = c < words ? ld_shared_v4(swz(stage, row, c)) : make_uint4(0u, 0u, 0u, 0u);
             const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
           }
           const uint32_t e = top >> 7;
+          float up = 1.f;
           if (e >= 16u && e != 255u) {
-            up *= __uint_as_float((261u - e) << 23);
+            up = __uint_as_float((261u - e) << 23);
             f *= __uint_as_float((e - 7u) << 23);
           }
-        }
 #pragma unroll
-        for (int c = 0; c < 8 * NA; ++c) {
-          if (c >= 2 * ksteps) continue;
-          if (kF16) {
+          for (int c = 0; c < 8 * NA; ++c) {
+            if (c >= words) continue;
             float t[8];
             bf16x8_to_f32(v[c], t);
-            st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
+            st_shared_v4(swz(stage, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
                          pack_f16x2(t[4] * up, t[5] * up), pack_f16x2(t[6] * up, t[7] * up));
-          } else {
-            st_shared_v4(swz(q_addr + i * NA * kAtom, row, c), v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
           }
         }
         fence_proxy_async_smem();
@@ -606,7 +694,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         if (!ok) break;
         tc_fence_after();
         const uint32_t gone = absent[st];
-        const int x0 = place(u, seg.t0 + j);
+        const int x0 = place(u, j);
         const bool hidden = gone != 0u || x0 + kTP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
         // of columns 32 c ..: score (in powers of two) = product * fc + ev
         float fc[4] = {f, f, f, f}, ev[4] = {0.f, 0.f, 0.f, 0.f};
@@ -700,29 +788,58 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         if (!ok) break;
         tc_fence_after();
       }
-      const bool whole = seg.whole();
+      const bool whole = u.whole != 0;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + seg.slot()) * piece_floats<kUnitRows>(dh);
+      float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + u.slot) * piece_floats<kUnitRows>(dh);
       if (real && !whole) *reinterpret_cast<float2*>(piece + 2 * ru) = make_float2(m, l);
-      __nv_bfloat16* dst = real ? out_row(p, u, r) : nullptr;
-      for (int c = 0; c < ksteps; ++c) {
-        float o[16];
-        if (mine > 0) {
-          tmem_ld16_now(o_at + 16 * c, o);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0.f;
-        }
-        if (!real) continue;
-        if (whole) {
-          st_global_v4(dst + 16 * c, pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+      // out through the query tile, which every S of the unit has been made from: words of a row by neighbouring lanes
+      __nv_bfloat16* dst = real ? out_row(p, u.first, u.h, r) : nullptr;
+      __syncwarp();
+      if (whole) {
+#pragma unroll 2
+        for (int c = 0; c < ksteps; ++c) {
+          float o[16];
+          read_o(o, o_at, c, mine > 0);
+          st_shared_v4(swz(stage, row, 2 * c), pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
                        pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-          st_global_v4(dst + 16 * c + 8, pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
+          st_shared_v4(swz(stage, row, 2 * c + 1), pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
                        pack_bf16x2(o[12] * inv, o[13] * inv), pack_bf16x2(o[14] * inv, o[15] * inv));
-        } else {
-          float4* q = reinterpret_cast<float4*>(piece + 2 * kUnitRows + static_cast<size_t>(ru) * dh + 16 * c);
+        }
+        __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) q[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        for (int c = 0; c < 8 * NA; ++c) {
+          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), kRowStep * c + sub_row));
+          if (word < words) {
+            const uint4 v = ld_shared_v4(swz(stage, first_row + kRowStep * c + sub_row, word));
+            if (to != nullptr) st_global_v4(to + 8 * word, v.x, v.y, v.z, v.w);
+          }
+        }
+      } else {
+        // 32 columns of fp32, 128 bytes of a row, at a time
+        float* to = piece + 2 * kUnitRows + static_cast<size_t>(i * kTileRows + first_row) * dh;
+        const int rows = min(max(u.rows - i * kTileRows - first_row, 0), 32), w = lane & 7;
+        for (int c = 0; c < ksteps; c += 2) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (c + h < ksteps) {
+              float o[16];
+              read_o(o, o_at, c + h, mine > 0);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                st_shared_v4(swz(stage, row, 4 * h + k), __float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]),
+                             __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int from = 4 * k + (lane >> 3);
+            const uint4 v = ld_shared_v4(swz(stage, first_row + from, w));
+            if (from < rows && 16 * c + 4 * w < dh)
+              st_global_v4(to + static_cast<size_t>(from) * dh + 16 * c + 4 * w, v.x, v.y, v.z, v.w);
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();                           // O has been read: the next unit's P may follow
