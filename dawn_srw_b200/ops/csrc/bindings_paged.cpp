@@ -133,6 +133,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, cons
   const int64_t Hq = q.size(1);
   REFUSE_UNLESS(Hq >= 1 && kp.size(1) >= 1 && Hq % kp.size(1) == 0, Hq, " query heads are no multiple of the pages' ",
                 kp.size(1), " heads");
+  REFUSE_UNLESS(q.size(0) * (Hq / kp.size(1)) <= (1 << 30), "too many rows");
   REFUSE_UNLESS(!window.has_value() || *window >= 1, "window must be at least 1 (None: no window)");
   REFUSE_UNLESS(sinks >= 0, "sinks must not be negative");
   REFUSE_UNLESS(!max_new.has_value() || *max_new >= 0, "max_new must not be negative");

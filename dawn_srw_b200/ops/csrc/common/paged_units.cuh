@@ -49,12 +49,29 @@ __device__ __forceinline__ uint2 codes_to_f16(uint32_t x) {
   return r;
 }
 
+// Division of numbers below 2^31 by a number that the host knows: with 2^s the power of two from d on,
+// m = ceil(2^(31 + s) / d) exceeds the quotient by less than 1, so that x m / 2^(31 + s) exceeds x / d by less than
+// x / 2^(31 + s) < 1 / d, too little to reach the next whole number.
+struct Divisor {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * m) >> shift);
+  }
+};
+inline Divisor make_divisor(int d) {
+  int s = 0;
+  while ((1LL << s) < d) ++s;
+  return {static_cast<uint32_t>(((1ULL << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 struct AttnParams {
   View w;
   const __nv_bfloat16* q;           // [N, Hq, dh], strides in elements
   long long q_st, q_sh;
   __nv_bfloat16* out;               // [N, Hq, dh]
   int Hq, G;
+  Divisor by_g;                     // row -> token
   int window, sinks;                // window: kMostPositions without one
   float scale_log2;                 // scale * log2(e)
   float* part;                      // pieces of units that several workers share
@@ -80,7 +97,7 @@ template <int ROWS, int TP>
 __device__ __forceinline__ void unit_range(const AttnParams& p, Unit& u) {
   const int r0 = u.rt * ROWS;
   u.rows = min(ROWS, u.n * p.G - r0);
-  const int i0 = r0 / p.G, i1 = (r0 + u.rows - 1) / p.G;
+  const int i0 = p.by_g(r0), i1 = p.by_g(r0 + u.rows - 1);
   const int p_lo = u.len - u.n + i0, p_hi = u.len - u.n + i1;
   u.hi = max(p_hi + 1, 0);
   u.lo = max(0, p_lo - p.window + 1);             // p_lo >= -N, N and window at most 2^30: no overflow
@@ -102,18 +119,38 @@ __device__ __forceinline__ void unit_sequence(const AttnParams& p, Unit& u, int 
   u.len = u.n > 0 ? seq_length(p.w, b) : 0;
 }
 
-// Tiles of all units of sequence b.
+// Tiles of the units of one head of sequence i + lane: a lane's own arithmetic for a sequence of one row tile, the
+// warp's for one of many.
 template <int ROWS, int TP>
-__device__ __forceinline__ long long sequence_tiles(const AttnParams& p, int b) {
+__device__ __forceinline__ long long head_tiles(const AttnParams& p, int i, int lane) {
   Unit u;
-  unit_sequence(p, u, b);
-  long long sum = 0;
-  const int nrt = row_tiles<ROWS>(u.n, p.G);
-  for (u.rt = 0; u.rt < nrt; ++u.rt) {
-    unit_range<ROWS, TP>(p, u);
-    sum += u.tiles;
+  int nrt = 0;
+  long long x = 0;
+  u.len = u.n = 0;
+  if (i + lane < p.w.c.B) {
+    unit_sequence(p, u, i + lane);
+    nrt = row_tiles<ROWS>(u.n, p.G);
+    if (nrt == 1) {
+      u.rt = 0;
+      unit_range<ROWS, TP>(p, u);
+      x = u.tiles;
+    }
   }
-  return sum * p.w.c.H;
+  for (unsigned many = __ballot_sync(0xffffffffu, nrt > 1); many != 0u; many &= many - 1) {
+    const int k = __ffs(many) - 1, n = __shfl_sync(0xffffffffu, nrt, k);
+    Unit v;
+    v.len = __shfl_sync(0xffffffffu, u.len, k);
+    v.n = __shfl_sync(0xffffffffu, u.n, k);
+    long long sum = 0;
+    for (v.rt = lane; v.rt < n; v.rt += 32) {
+      unit_range<ROWS, TP>(p, v);
+      sum += v.tiles;
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == k) x = sum;
+  }
+  return x;
 }
 
 // Rows of no sequence (before the first and behind the last one) are zero.
@@ -132,53 +169,57 @@ __device__ __forceinline__ void zero_other_rows(const AttnParams& p, int worker,
 
 // Row `row` (token, query head of the group) of key/value head h of a sequence.
 __device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, int first, int h, int row) {
-  return p.out + (static_cast<size_t>(first + row / p.G) * p.Hq + h * p.G + row % p.G) * p.w.c.dh;
+  const int t = p.by_g(row);
+  return p.out + (static_cast<size_t>(first + t) * p.Hq + h * p.G + (row - t * p.G)) * p.w.c.dh;
 }
 __device__ __forceinline__ __nv_bfloat16* out_row(const AttnParams& p, const Unit& u, int row) { return out_row(p, u.first, u.h, row); }
 
-// Where a worker's run of tiles begins, among all tiles of all units in order (sequence, head, row tile).
-struct Run { long long begin, end, total; };
+// A worker's run of tiles, among all tiles of all units in order (sequence, head, row tile), and the sequence of its
+// first one: its tiles of a head, and how many tiles come before it.
+struct Run { long long begin, end, per_head, before; int b; };
 
-// Equal runs of the warps: worker i of n takes tiles [i T / n, (i + 1) T / n).
+// Equal runs: worker i of n takes tiles [i T / n, (i + 1) T / n).
 template <int ROWS, int TP>
-__device__ __forceinline__ Run share(const AttnParams& p, int lane, long long worker, int least, int& b, long long& before) {
+__device__ __forceinline__ Run share(const AttnParams& p, int lane, long long worker, int least) {
   const int B = p.w.c.B;
-  long long total = 0;
+  const long long H = p.w.c.H;
+  long long total = 0, x = 0;
   for (int i = 0; i < B; i += 32) {
-    long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
+    x = head_tiles<ROWS, TP>(p, i, lane);
+    long long sum = x;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    total += x;
+    for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    total += sum * H;
   }
   const long long most = total / least;
   const long long n = most < 1 ? 1 : most < p.workers ? most : p.workers;
-  Run r = {0, 0, total};
+  Run r = {0, 0, 0, 0, 0};
   if (worker >= n) return r;
   r.begin = worker * total / n;
   r.end = (worker + 1) * total / n;
-  b = 0;
-  before = 0;
   for (int i = 0; i < B; i += 32) {                    // the sequence that holds tile r.begin
-    const long long x = i + lane < B ? sequence_tiles<ROWS, TP>(p, i + lane) : 0;
-    long long c = x;
+    if (B > 32) x = head_tiles<ROWS, TP>(p, i, lane);
+    long long c = x * H;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, c, d);
       if (lane >= d) c += y;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, before + c > r.begin);
+    const unsigned past = __ballot_sync(0xffffffffu, r.before + c > r.begin);
     if (past != 0u) {
       const int k = __ffs(past) - 1;
-      b = i + k;
-      before += __shfl_sync(0xffffffffu, c - x, k);
+      r.b = i + k;
+      r.per_head = __shfl_sync(0xffffffffu, x, k);
+      r.before += __shfl_sync(0xffffffffu, c, k) - r.per_head * H;
       return r;
     }
-    before += __shfl_sync(0xffffffffu, c, 31);
+    r.before += __shfl_sync(0xffffffffu, c, 31);
   }
   return r;
 }
 
-// A piece of a unit in the workspace: per row maximum and sum, then O.
+// A piece of a unit in the workspace: per row maximum and sum, then O.  Worker i has two: 2 i + 1 for a unit that begins
+// in its run and ends in a later one, 2 i for one that began in an earlier run.
 template <int ROWS>
 __host__ __device__ constexpr int piece_floats(int dh) { return ROWS * (dh + 2); }
 
@@ -206,27 +247,40 @@ struct Segments {
   }
 
   __device__ void begin(const AttnParams& p, int lane, int worker, int least) {
-    int b = 0;
-    long long before = 0;
-    const Run run = share<ROWS, TP>(p, lane, worker, least, b, before);
+    const Run run = share<ROWS, TP>(p, lane, worker, least);
     at = run.begin;
     end = run.end;
     if (!on()) return;
-    unit_sequence(p, u, b);
+    unit_sequence(p, u, run.b);
     nrt = row_tiles<ROWS>(u.n, p.G);
-    long long per_head = 0, off = at - before;
-    for (u.rt = 0; u.rt < nrt; ++u.rt) {
-      unit_range<ROWS, TP>(p, u);
-      per_head += u.tiles;
+    const long long off = at - run.before;
+    u.h = off >> 31 == 0 && run.per_head >> 31 == 0
+              ? static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(run.per_head))
+              : static_cast<int>(off / run.per_head);
+    long long left = off - u.h * run.per_head;         // tiles of the head before the first one
+    u.rt = 0;
+    for (int base = 0; nrt > 1 && base < nrt; base += 32) {
+      Unit v = u;
+      v.rt = base + lane;
+      int x = 0;
+      if (v.rt < nrt) {
+        unit_range<ROWS, TP>(p, v);
+        x = v.tiles;
+      }
+      int c = x;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, c, d);
+        if (lane >= d) c += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, c > left);
+      const int k = past != 0u ? __ffs(past) - 1 : 31;
+      u.rt = base + k;
+      left -= __shfl_sync(0xffffffffu, past != 0u ? c - x : c, k);
+      if (past != 0u) break;
     }
-    u.h = static_cast<int>(off / per_head);
-    off -= u.h * per_head;
-    for (u.rt = 0;; ++u.rt) {
-      unit_range<ROWS, TP>(p, u);
-      if (off < u.tiles) break;
-      off -= u.tiles;
-    }
-    t0 = static_cast<int>(off);
+    unit_range<ROWS, TP>(p, u);
+    t0 = static_cast<int>(left);
     t1 = static_cast<int>(min(static_cast<long long>(u.tiles), t0 + (end - at)));
   }
 

@@ -161,7 +161,7 @@ __device__ __forceinline__ uint32_t swz(uint32_t tile, int row, int c8) {
 __device__ __forceinline__ int tiles_of(const AttnParams& p, const Unit& u, int i) {
   const int r0 = i * kTileRows, r1 = min(u.rows, r0 + kTileRows);
   if (r0 >= u.rows) return 0;
-  const int last = u.len - u.n + (u.rt * kUnitRows + r1 - 1) / p.G;
+  const int last = u.len - u.n + p.by_g(u.rt * kUnitRows + r1 - 1);
   const int end = (max(last + 1, 0) + kTP - 1) / kTP;       // tiles of positions that begin at or before `last`
   return min(u.tiles, end <= u.st ? end : max(end - u.skip, u.st));
 }
@@ -633,9 +633,9 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       const int ru = i * kTileRows + row;          // row of the unit
       const bool real = ru < u.rows;
       const int r = u.rt * kUnitRows + ru;         // row of the sequence's head
-      const int pos = real ? u.len - u.n + r / p.G : -1;
+      const int pos = real ? u.len - u.n + p.by_g(r) : -1;
       const int w0 = u.rt * kUnitRows + i * kTileRows + (warp & 3) * 32;       // positions of this warp's rows
-      const int pos_lo = u.len - u.n + min(w0, u.n * p.G - 1) / p.G, pos_hi = u.len - u.n + min(w0 + 31, u.n * p.G - 1) / p.G;
+      const int pos_lo = u.len - u.n + p.by_g(min(w0, u.n * p.G - 1)), pos_hi = u.len - u.n + p.by_g(min(w0 + 31, u.n * p.G - 1));
       // the scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which
       // would turn the -inf of hidden scores into NaN, into queries of zero
       const bool flat = p.scale_log2 == 0.f;
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         // queries into the swizzled tile: a warp its 32 rows, kRowLanes neighbouring lanes the words of a row
         const __nv_bfloat16* src = nullptr;
         if (real && !flat)
-          src = p.q + static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
+          src = p.q + static_cast<long long>(u.first + p.by_g(r)) * p.q_st + static_cast<long long>(u.h * p.G + r - p.by_g(r) * p.G) * p.q_sh;
         const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
         uint4 v[8 * NA];
 #pragma unroll

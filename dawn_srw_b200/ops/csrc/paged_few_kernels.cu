@@ -96,7 +96,7 @@ struct Warp {
       const int r = u.rt * kRows + 8 * nt + g;
       const bool live = 8 * nt + g < u.rows;
       const __nv_bfloat16* row = p.q;
-      if (live) row += static_cast<long long>(u.first + r / p.G) * p.q_st + static_cast<long long>(u.h * p.G + r % p.G) * p.q_sh;
+      if (live) row += static_cast<long long>(u.first + p.by_g(r)) * p.q_st + static_cast<long long>(u.h * p.G + r - p.by_g(r) * p.G) * p.q_sh;
       uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
@@ -146,7 +146,7 @@ struct Warp {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t + e;
-        pos_of[nt][e] = r < u.rows ? u.len - u.n + (u.rt * kRows + r) / p.G : -1;
+        pos_of[nt][e] = r < u.rows ? u.len - u.n + p.by_g(u.rt * kRows + r) : -1;
       }
     const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
     auto place = [&](int tile) { return (tile < u.st ? tile : tile + u.skip) * kTP; };

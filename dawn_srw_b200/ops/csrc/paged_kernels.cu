@@ -267,7 +267,9 @@ extern "C" long long dsb_paged_attention_workspace(const DsbPaged* c, int Hq, in
 extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
                                    int max_new, int window, int sinks, float scale, void* workspace, cudaStream_t stream) {
   if (bad_cache(c) || Hq <= 0 || Hq % c->H != 0 || window < 0 || sinks < 0 || max_new < 0) return 940;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8 || c->H > 65535 || c->B > 65535) return 941;
+  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8 || c->H > 65535 || c->B > 65535 ||
+      static_cast<long long>(c->N) * (Hq / c->H) > kMostPositions)
+    return 941;
   if (c->N == 0) return 0;
   if (c->B == 0) {
     const size_t bytes = static_cast<size_t>(c->N) * Hq * c->dh * sizeof(__nv_bfloat16);
@@ -282,6 +284,7 @@ extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q
   p.out = static_cast<__nv_bfloat16*>(out);
   p.Hq = Hq;
   p.G = Hq / c->H;
+  p.by_g = make_divisor(p.G);
   p.window = window > 0 && window < kMostPositions ? window : kMostPositions;
   p.sinks = sinks;
   p.scale_log2 = scale * 1.4426950408889634f;
