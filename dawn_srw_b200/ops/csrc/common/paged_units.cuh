@@ -416,59 +416,6 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_few_kernel(const At
   }
 }
 
-// Units of many rows and few pieces: a warp per four rows.
-constexpr int kMergeRows = 4, kMergeWarps = 8;
-template <int ROWS>
-__global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_rows_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int i = blockIdx.x, dh = p.w.c.dh, lane = threadIdx.x & 31;
-  const int r0 = (blockIdx.y * kMergeWarps + (threadIdx.x >> 5)) * kMergeRows;
-  Unit u;
-  int last;
-  if (!shared_unit<ROWS>(p, i, lane, u, last)) return;
-  if (r0 >= u.rows) return;
-  const int stride = piece_floats<ROWS>(dh);
-  const bool mine = 4 * lane < dh;
-  auto piece = [&](int j) { return p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * stride; };
-  float top[kMergeRows], sum[kMergeRows];
-  float4 a[kMergeRows];
-#pragma unroll
-  for (int k = 0; k < kMergeRows; ++k) {
-    top[k] = kFloor;
-    sum[k] = 0.f;
-    a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-#pragma unroll 2
-  for (int j = i; j <= last; ++j) {
-    const float* from = piece(j);
-    float2 ml[kMergeRows];
-    float4 o[kMergeRows];
-#pragma unroll
-    for (int k = 0; k < kMergeRows; ++k) {
-      const bool on = r0 + k < u.rows;
-      ml[k] = on ? __ldcg(reinterpret_cast<const float2*>(from) + r0 + k) : make_float2(kFloor, 0.f);
-      o[k] = on && mine ? __ldcg(reinterpret_cast<const float4*>(from + 2 * ROWS + (r0 + k) * dh) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int k = 0; k < kMergeRows; ++k) {
-      const float most = fmaxf(top[k], ml[k].x), x = exp2_fast(top[k] - most), w = exp2_fast(ml[k].x - most);
-      top[k] = most;
-      sum[k] = fmaf(sum[k], x, w * ml[k].y);
-      a[k].x = fmaf(a[k].x, x, w * o[k].x);
-      a[k].y = fmaf(a[k].y, x, w * o[k].y);
-      a[k].z = fmaf(a[k].z, x, w * o[k].z);
-      a[k].w = fmaf(a[k].w, x, w * o[k].w);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kMergeRows; ++k) {
-    if (r0 + k >= u.rows || !mine) continue;
-    const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
-    *reinterpret_cast<uint2*>(out_row(p, u, u.rt * ROWS + r0 + k) + 4 * lane) =
-        make_uint2(pack_bf16x2(a[k].x * inv, a[k].y * inv), pack_bf16x2(a[k].z * inv, a[k].w * inv));
-  }
-}
-
 // After the kernel that leaves the pieces, in its stream; launched early, it waits for that kernel's end by itself.
 template <typename F>
 int launch_merge(F* kernel, dim3 grid, int threads, const AttnParams& p, cudaStream_t stream) {

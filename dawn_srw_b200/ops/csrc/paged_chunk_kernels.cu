@@ -27,14 +27,15 @@ namespace {
 
 constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows, kTP = 128;
 constexpr int kAtom = kTP * 128;            // 128 rows x 64 16-bit columns
-constexpr int kStages = 2;
-constexpr int kMeta = 4;                    // slots of scales and absences: a softmax is at most two tiles behind the loads
+template <int NA> constexpr int kStages = NA == 1 ? 4 : 2;      // tiles of K, and of V, in shared memory
+// Slots of scales and absences: written with K, read by a softmax that may be a tile behind the last use of the stage.
+template <int NA> constexpr int kMeta = 2 * kStages<NA>;
 constexpr int kPlans = 4;                   // segments that the planning warp is ahead of the others at most
 constexpr float kSlack = 8.f;               // how far (in powers of two) a maximum may grow before O is rescaled
 constexpr int kLeast = 2;                   // tiles of a run
 
-// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8, 9 and 10: MMA issue, TMA, the plan.  Warpgroup 3, 8-bit
-// kinds: loaders.
+// Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8 and 9: their MMA.  Warps 10 and 11: TMA, the plan.
+// Warpgroup 3, 8-bit kinds: loaders.
 template <int KIND>
 constexpr int kThreadsOf = KIND == kBf16 ? 384 : 512;
 
@@ -42,11 +43,11 @@ template <int NA>                            // 64-column atoms of a head
 struct Smem {
   static constexpr int kQ = 0;                                   // [2 tiles][NA atoms]
   static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages][NA]
-  static constexpr int kV = kK + kStages * NA * kAtom;           // [kStages][NA]
-  static constexpr int kExp = kV + kStages * NA * kAtom;         // [kMeta][2][4] 2^e of the keys, e of the values
-  static constexpr int kPlan = kExp + kMeta * 32;                // [kPlans] segments ahead
+  static constexpr int kV = kK + kStages<NA> * NA * kAtom;       // [kStages][NA]
+  static constexpr int kExp = kV + kStages<NA> * NA * kAtom;     // [kMeta][2][4] 2^e of the keys, e of the values
+  static constexpr int kPlan = kExp + kMeta<NA> * 32;            // [kPlans] segments ahead
   static constexpr int kBar = kPlan + kPlans * 128;
-  static constexpr int kTotal = kBar + 256 + 1024;
+  static constexpr int kTotal = kBar + 512 + 1024;
   static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -196,6 +197,11 @@ __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uin
   }
 }
 
+// 16 bytes to shared memory, zeros where `on` is false (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -227,18 +233,24 @@ __device__ __forceinline__ bool elect_one() {
   return on != 0u;
 }
 
+template <int S>
 struct Bars {
-  uint64_t* q_full;     // [2] queries of tile i are in shared memory (4 warps)
-  uint64_t* k_full;     // [kStages] K, and the tile's scales and absences
-  uint64_t* k_empty;    // [kStages] both S of the stage are done
-  uint64_t* v_full;     // [kStages]
-  uint64_t* v_empty;    // [kStages] both O of the stage are done
-  uint64_t* v_fix;      // V has landed, rows behind the end still have to be cleared
-  uint64_t* s_full;     // [2]
-  uint64_t* p_full;     // [2] P is in TMEM, S has been read (4 warps)
-  uint64_t* o_done;     // [2]
-  uint64_t* plan_full;  // [kPlans]
-  uint64_t* plan_empty; // [kPlans] every warp that works by the plan has read it
+  uint64_t q_full[2];       // queries of tile i are in shared memory (4 warps)
+  uint64_t k_full[S];       // K, and the tile's scales and absences
+  uint64_t k_empty[S];      // both tiles' S of the stage are done
+  uint64_t v_full[S];
+  uint64_t v_empty[S];      // both tiles' O of the stage are done
+  uint64_t v_fix;           // V has landed, rows behind the end still have to be cleared
+  uint64_t s_full[2];
+  uint64_t s_free[2];       // S has been read (4 warps); only where P has columns of its own
+  uint64_t p_half[2];       // the first 64 positions of P are in TMEM (4 warps)
+  uint64_t p_full[2];       // all of them
+  uint64_t o_done[2];
+  uint64_t plan_full[kPlans];
+  uint64_t plan_empty[kPlans];  // every warp that works by the plan has read it
+  uint32_t tmem;
+  int abort;
+  uint32_t absent[2 * S];   // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
 };
 
 // The plans in order, for one warp.
@@ -268,11 +280,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  const Bars b = {bars, bars + 2, bars + 4, bars + 6, bars + 8, bars + 10, bars + 11, bars + 13, bars + 15, bars + 17, bars + 21};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* absent = tmem_slot + 2;    // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
+  constexpr int S = kStages<NA>;
+  static_assert(sizeof(Bars<S>) <= 512 && kMeta<NA> == 2 * S, "barriers");
+  Bars<S>& b = *reinterpret_cast<Bars<S>*>(smem + L::kBar);
+  volatile int* abort_flag = &b.abort;
+  volatile uint32_t* absent = b.absent;
   const AttnParams& p = cp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.w.c.dh, ksteps = dh >> 4;
 
@@ -280,21 +292,23 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.q_full[i], 4);
       mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.s_free[i], 4);
+      mbar_init(&b.p_half[i], 4);
       mbar_init(&b.p_full[i], 4);
       mbar_init(&b.o_done[i], 1);
     }
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < S; ++i) {
       mbar_init(&b.k_full[i], kF16 ? 4 : 1);
-      mbar_init(&b.k_empty[i], 1);
+      mbar_init(&b.k_empty[i], 2);
       mbar_init(&b.v_full[i], kF16 ? 4 : 1);
-      mbar_init(&b.v_empty[i], 1);
+      mbar_init(&b.v_empty[i], 2);
     }
-    mbar_init(b.v_fix, 1);
+    mbar_init(&b.v_fix, 1);
     for (int i = 0; i < kPlans; ++i) {
       mbar_init(&b.plan_full[i], 1);
-      mbar_init(&b.plan_empty[i], kF16 ? 13 : 10);      // softmax, MMA, and TMA or loaders
+      mbar_init(&b.plan_empty[i], kF16 ? 14 : 11);      // softmax, MMA, and TMA or loaders
     }
-    *abort_flag = 0;
+    b.abort = 0;
     fence_barrier_init();
     if (!kF16) {
       tma_prefetch_desc(&cp.k);
@@ -302,13 +316,13 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     }
   }
   if (warp == 8) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(&b.tmem, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = b.tmem;
   const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
   // S: columns 0 and 128;  O: 256 and 256 + 64 NA;  P: where S is, or behind O
   auto s_col = [&](int i) { return tmem + 128 * i; };
@@ -321,80 +335,85 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   Plan u;
 
   if (warp >= 8 && warp < 12) {
-    if (warp == 8) {
-      // ------------------------------------------------------------ MMA issue
+    if (warp < 10) {
+      // ------------------------------------------------------------ MMA issue of tile I
       if (elect_one()) {
-        // one lane does all of it; what does not change from tile to tile is a constant or made beforehand, so that an
-        // instruction costs few moves to uniform registers
+        // One lane does all of it, and no instruction stands under a condition of its own: a tcgen05.mma that became a
+        // predicated one gave wrong results.  What does not change from tile to tile is made beforehand.
+        const int I = warp - 8;
         const uint32_t idesc_s = idesc16(!kF16, kTileRows, kTP, 0), idesc_o = idesc16(!kF16, kTileRows, dh, 1);
-        const uint64_t q_desc = desc_k(q_addr, 0), k_desc = desc_k(k_addr, 0), v_desc = desc_mn(v_addr, 0);
         constexpr uint32_t kStage16 = NA * kAtom >> 4;        // a stage, or a query tile, in a descriptor's units
-        // stages so far, and of each tile segments with work and P: a phase of a barrier is waited for by whoever
-        // takes part in it, and by nobody else, so that no one is ever two phases off
-        uint32_t nk = 0, nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;
+        const uint64_t q_desc = desc_k(q_addr, 0) + I * kStage16, k_desc = desc_k(k_addr, 0), v_desc = desc_mn(v_addr, 0);
+        const uint32_t s_at = s_col(I), o_at = o_col(I), p_at = p_col(I);
+        // uses of the stages, segments with work and tiles so far.  Whoever waits for a phase of a barrier has seen the
+        // phase before it, or something later, so that no wait is two phases off.
+        uint32_t nk = 0, nq = 0, nt = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && wait_hot(bar, phase & 1, abort_flag); };
-        // the plan's part of this warp's, by its one lane
+        auto issue_s = [&](int j) {
+          const uint32_t st = (nk + j) % S;
+          wait(&b.k_full[st], (nk + j) / S);
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t ka = k_desc + st * kStage16;
+          switch (ksteps - 4 * (NA - 1)) {
+            case 1: issue_qk<4 * NA - 3>(s_at, q_desc, ka, idesc_s); break;
+            case 2: issue_qk<4 * NA - 2>(s_at, q_desc, ka, idesc_s); break;
+            case 3: issue_qk<4 * NA - 1>(s_at, q_desc, ka, idesc_s); break;
+            default: issue_qk<4 * NA>(s_at, q_desc, ka, idesc_s);
+          }
+          mma_commit(&b.s_full[I]);
+          mma_commit(&b.k_empty[st]);
+        };
         for (uint32_t k = 0; ok; ++k) {
           const uint32_t slot = k % kPlans;
           wait(&b.plan_full[slot], k / kPlans);
           if (!ok) break;
-          const int n0 = plan_ring[slot].n0, n1 = plan_ring[slot].n1, n = max(n0, n1), more = plan_ring[slot].b;
+          const int n0 = plan_ring[slot].n0, n1 = plan_ring[slot].n1, more = plan_ring[slot].b;
           mbar_arrive(&b.plan_empty[slot]);
           if (more < 0) break;
-          if (n0 > 0) wait(&b.q_full[0], nq0++);
-          if (n1 > 0) wait(&b.q_full[1], nq1++);
-          // S of tile I and the segment's j-th tile of positions; the last of the two frees the stage
-          auto issue_s = [&](auto tile, int j) {
-            constexpr int I = decltype(tile)::value;
-            const uint32_t st = (nk + j) % kStages;
-            wait(&b.k_full[st], (nk + j) / kStages);
-            if (!ok) return;
-            tc_fence_after();
-            const uint64_t ka = k_desc + st * kStage16;
-            const uint64_t qa = q_desc + I * kStage16;
-            switch (ksteps - 4 * (NA - 1)) {                // no instruction under a condition of its own
-              case 1: issue_qk<4 * NA - 3>(s_col(I), qa, ka, idesc_s); break;
-              case 2: issue_qk<4 * NA - 2>(s_col(I), qa, ka, idesc_s); break;
-              case 3: issue_qk<4 * NA - 1>(s_col(I), qa, ka, idesc_s); break;
-              default: issue_qk<4 * NA>(s_col(I), qa, ka, idesc_s);
+          const int n = max(n0, n1), mine = I == 0 ? n0 : n1;
+          if (mine > 0) {
+            wait(&b.q_full[I], nq++);
+            if (ok) issue_s(0);
+          }
+          for (int j = 0; j < mine && ok; ++j, ++nt) {
+            const uint32_t st = (nk + j) % S;
+            if (!kAlias && j + 1 < mine) {         // the next S while the weights of this one are still being made
+              wait(&b.s_free[I], nt);
+              if (ok) issue_s(j + 1);
             }
-            mma_commit(&b.s_full[I]);
-            if (I == 1 || j >= n1) mma_commit(&b.k_empty[st]);
-          };
-          auto issue_o = [&](auto tile, int j, uint32_t& np) {
-            constexpr int I = decltype(tile)::value;
-            const int mine = I == 0 ? n0 : n1;
-            if (j >= mine || !ok) return;
-            const uint32_t st = (nk + j) % kStages;
-            wait(&b.v_full[st], (nk + j) / kStages);
-            wait(&b.p_full[I], np);
-            if (!ok) return;
+            wait(&b.v_full[st], (nk + j) / S);
+            wait(&b.p_half[I], nt);
+            if (!ok) break;
             tc_fence_after();
             const uint64_t va = v_desc + st * kStage16;
-            mma_ts(o_col(I), p_col(I), va, idesc_o, j > 0);
+            mma_ts(o_at, p_at, va, idesc_o, j > 0);
 #pragma unroll
-            for (int kk = 1; kk < kTP / 16; ++kk) mma_ts(o_col(I), p_col(I) + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
+            for (int kk = 1; kk < kTP / 32; ++kk) mma_ts(o_at, p_at + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
+            wait(&b.p_full[I], nt);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = kTP / 32; kk < kTP / 16; ++kk) mma_ts(o_at, p_at + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
             mma_commit(&b.o_done[I]);
-            if (I == 1 || j >= n1) mma_commit(&b.v_empty[st]);
-            if (j + 1 < mine) {
-              if (kAlias) wait(&b.o_done[I], np);         // the next S takes the columns that this P is being read from
-              if (ok) issue_s(tile, j + 1);
+            mma_commit(&b.v_empty[st]);
+            if (kAlias && j + 1 < mine) {          // the next S takes the columns that this P is being read from
+              wait(&b.o_done[I], nt);
+              if (ok) issue_s(j + 1);
             }
-            ++np;
-          };
-          using Tile0 = std::integral_constant<int, 0>;
-          using Tile1 = std::integral_constant<int, 1>;
-          if (n0 > 0 && ok) issue_s(Tile0{}, 0);
-          if (n1 > 0 && ok) issue_s(Tile1{}, 0);
-          for (int j = 0; j < n && ok; ++j) {
-            issue_o(Tile0{}, j, np0);
-            issue_o(Tile1{}, j, np1);
+          }
+          for (int j = mine; j < n && ok; ++j) {   // the other tile's alone
+            const uint32_t st = (nk + j) % S;
+            wait(&b.k_full[st], (nk + j) / S);
+            if (ok) mbar_arrive(&b.k_empty[st]);
+            wait(&b.v_full[st], (nk + j) / S);
+            if (ok) mbar_arrive(&b.v_empty[st]);
           }
           nk += n;
         }
       }
-    } else if (warp == 9 && !kF16) {
+    } else if (warp == 10 && !kF16) {
       // ------------------------------------------------------------ TMA loads of bf16 pages
       uint32_t nk = 0, fixes = 0;
       bool ok = true;
@@ -403,7 +422,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         const int n = max(u.n0, u.n1);
         const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
         for (int j = 0; j < n && ok; ++j, ++nk) {
-          const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1;
+          const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1;
           const int x0 = place(u, j);
           // lane i < 8: the page of sixteen positions i, -1 where no row sees any of them
           int id = -1;
@@ -433,7 +452,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
           if (!ok) break;
           if (lane == 0) {
-            absent[nk % kMeta] = (gone & 3u) | (gone & 12u) << 6 | (gone & 48u) << 12 | (gone & 192u) << 18;
+            absent[nk % kMeta<NA>] = (gone & 3u) | (gone & 12u) << 6 | (gone & 48u) << 12 | (gone & 192u) << 18;
             mbar_expect_tx(&b.k_full[st], boxes * NA * box * 128);
           }
           __syncwarp();
@@ -442,14 +461,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
               tma_load_3d(k_addr + (st * NA + a) * kAtom + lane * 2048, &cp.k, &b.k_full[st], 64 * a, c1, c2);
           ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
           if (!ok) break;
-          uint64_t* bar = cut ? b.v_fix : &b.v_full[st];
+          uint64_t* bar = cut ? &b.v_fix : &b.v_full[st];
           if (lane == 0) mbar_expect_tx(bar, boxes * NA * box * 128);
           __syncwarp();
           if (fetch)
             for (int a = 0; a < NA; ++a)
               tma_load_3d(v_addr + (st * NA + a) * kAtom + lane * 2048, &cp.v, bar, 64 * a, c1, c2);
           if (cut) {
-            ok = __all_sync(0xffffffffu, mbar_wait(b.v_fix, fixes & 1, abort_flag));
+            ok = __all_sync(0xffffffffu, mbar_wait(&b.v_fix, fixes & 1, abort_flag));
             if (!ok) break;
             ++fixes;
             for (int w = lane; w < kTP * 8; w += 32) {
@@ -465,7 +484,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
       }
     }
-    else if (warp == 10) {
+    else if (warp == 11) {
       // ------------------------------------------------------------ the plan, and notes for the merge
       Segments<kUnitRows, kTP> seg;
       int4 meta = make_int4(-1, 0, 0, 0);
@@ -493,7 +512,6 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         seg.next(p);
       }
       if (lane == 0) p.meta[blockIdx.x] = meta;
-    } else if (warp == 11) {
       zero_other_rows(p, blockIdx.x * 32 + lane, gridDim.x * 32);
     }
   } else if (warp >= 12) {
@@ -570,7 +588,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         fetch(p.w.c.v, r, vraw);
       }
       for (uint32_t nk = 0; have && ok; ++nk) {
-        const uint32_t st = nk % kStages, par = ((nk / kStages) & 1) ^ 1, slot = nk % kMeta;
+        const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1, slot = nk % kMeta<NA>;
         const uint32_t none = __ballot_sync(0xffffffffu, r.gone);         // two sixteens of this warp
         const uint32_t ek = largest(r.ks), ev = largest(r.vs);
         // 2^(127 - e) as a float: e of 254 at most
@@ -614,72 +632,71 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     const int i = warp >> 2, row = threadIdx.x - 128 * i;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
-    const uint32_t stage = q_addr + i * NA * kAtom;              // the query tile, and on the way out its results
-    constexpr int kRowLanes = 8 * NA, kRowStep = 32 / kRowLanes;
+    const uint32_t q_tile = q_addr + i * NA * kAtom;
     const int first_row = 32 * (warp & 3), words = 2 * ksteps;  // of this warp; 16-byte words of a row
-    const int word = lane % kRowLanes, sub_row = lane / kRowLanes;
-    auto read_o = [](float* o, uint32_t at, int c, bool any) {
-      if (any) {
-        tmem_ld16_now(at + 16 * c, o);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = 0.f;
+    // a scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which
+    // would turn the -inf of hidden scores into NaN, into queries of zero
+    const bool flat = p.scale_log2 == 0.f;
+    // queries of the next segment on their way into the swizzled tile: a warp its 32 rows, neighbouring lanes the words
+    // of a row
+    auto fetch_q = [&]() {
+      constexpr int kRowLanes = 8 * NA, kRowStep = 32 / kRowLanes;
+      const int word = lane % kRowLanes, sub_row = lane / kRowLanes;
+      if (word < words) {
+#pragma unroll 4
+        for (int c = 0; c < 32 / kRowStep; ++c) {
+          const int x = first_row + kRowStep * c + sub_row, ru = i * kTileRows + x;
+          const int r = u.rt * kUnitRows + ru, t = p.by_g(r);
+          const bool on = ru < u.rows && !flat;
+          const __nv_bfloat16* src =
+              on ? p.q + static_cast<long long>(u.first + t) * p.q_st + static_cast<long long>(u.h * p.G + r - t * p.G) * p.q_sh : p.q;
+          copy16(swz(q_tile, x, word), src + (on ? 8 * word : 0), on);
+        }
       }
     };
     uint32_t nk = 0, ns = 0;                       // tiles loaded, S of this tile so far
-    bool ok = true;
-    while (ok && plans.next(u, lane)) {
+    bool ok = true, have = plans.next(u, lane);
+    if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
+    while (ok && have) {
       const int n = max(u.n0, u.n1), mine = i == 0 ? u.n0 : u.n1;
       const int ru = i * kTileRows + row;          // row of the unit
       const bool real = ru < u.rows;
       const int r = u.rt * kUnitRows + ru;         // row of the sequence's head
       const int pos = real ? u.len - u.n + p.by_g(r) : -1;
-      const int w0 = u.rt * kUnitRows + i * kTileRows + (warp & 3) * 32;       // positions of this warp's rows
+      const int w0 = u.rt * kUnitRows + i * kTileRows + first_row;             // positions of this warp's rows
       const int pos_lo = u.len - u.n + p.by_g(min(w0, u.n * p.G - 1)), pos_hi = u.len - u.n + p.by_g(min(w0 + 31, u.n * p.G - 1));
-      // the scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which
-      // would turn the -inf of hidden scores into NaN, into queries of zero
-      const bool flat = p.scale_log2 == 0.f;
       float f = flat ? 1.f : fabsf(p.scale_log2);
       if (mine > 0) {
-        // queries into the swizzled tile: a warp its 32 rows, kRowLanes neighbouring lanes the words of a row
-        const __nv_bfloat16* src = nullptr;
-        if (real && !flat)
-          src = p.q + static_cast<long long>(u.first + p.by_g(r)) * p.q_st + static_cast<long long>(u.h * p.G + r - p.by_g(r) * p.G) * p.q_sh;
-        const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-        uint4 v[8 * NA];
-#pragma unroll
-        for (int c = 0; c < 8 * NA; ++c) {
-          const __nv_bfloat16* from = reinterpret_cast<const __nv_bfloat16*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), kRowStep * c + sub_row));
-          v[c] = from != nullptr && word < words ? __ldg(reinterpret_cast<const uint4*>(from) + word) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int c = 0; c < 8 * NA; ++c)
-          if (word < words)
-            st_shared_v4(swz(stage, first_row + kRowStep * c + sub_row, word), v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
-        if (kF16) {                                // fp16 queries, scaled by a power of two (see the few-row kernel)
-          __syncwarp();
+        copies_wait_all();
+        __syncwarp();
+        const bool flip = p.scale_log2 < 0.f;
+        if (kF16 || flip) {
+          uint4 v[8 * NA];
           uint32_t top = 0;
 #pragma unroll
           for (int c = 0; c < 8 * NA; ++c) {
-            v[c] = c < words ? ld_shared_v4(swz(stage, row, c)) : make_uint4(0u, 0u, 0u, 0u);
+            v[c] = c < words ? ld_shared_v4(swz(q_tile, row, c)) : make_uint4(0u, 0u, 0u, 0u);
             const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
           }
-          const uint32_t e = top >> 7;
-          float up = 1.f;
-          if (e >= 16u && e != 255u) {
-            up = __uint_as_float((261u - e) << 23);
+          float up = flip ? -1.f : 1.f;
+          const uint32_t e = top >> 7;             // fp16 queries, scaled by a power of two (see the few-row kernel)
+          if (kF16 && e >= 16u && e != 255u) {
+            up *= __uint_as_float((261u - e) << 23);
             f *= __uint_as_float((e - 7u) << 23);
           }
 #pragma unroll
           for (int c = 0; c < 8 * NA; ++c) {
             if (c >= words) continue;
-            float t[8];
-            bf16x8_to_f32(v[c], t);
-            st_shared_v4(swz(stage, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
-                         pack_f16x2(t[4] * up, t[5] * up), pack_f16x2(t[6] * up, t[7] * up));
+            if (kF16) {
+              float t[8];
+              bf16x8_to_f32(v[c], t);
+              st_shared_v4(swz(q_tile, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
+                           pack_f16x2(t[4] * up, t[5] * up), pack_f16x2(t[6] * up, t[7] * up));
+            } else {
+              st_shared_v4(swz(q_tile, row, c), v[c].x ^ 0x80008000u, v[c].y ^ 0x80008000u, v[c].z ^ 0x80008000u, v[c].w ^ 0x80008000u);
+            }
           }
         }
         fence_proxy_async_smem();
@@ -688,8 +705,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       }
       float m = kFloor, l = 0.f;
       for (int j = 0; j < mine; ++j, ++ns) {
-        const uint32_t st = (nk + j) % kMeta;
-        // also says that all MMAs issued before are done: P and O of the last tile
+        const uint32_t st = (nk + j) % kMeta<NA>;
         ok = __all_sync(0xffffffffu, wait_hot(&b.s_full[i], ns & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -739,6 +755,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             top = fmaxf(top, fmaf(fmaxf(t0, t1), fc[2 * h + c], ev[2 * h + c]));       // fc >= 0
           }
         }
+        if (!kAlias && j > 0) {                    // O, and the columns of P (elsewhere S could not be here otherwise)
+          ok = __all_sync(0xffffffffu, wait_hot(&b.o_done[i], (ns - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+        }
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
@@ -761,6 +782,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         for (int c = 0; c < 4; ++c) {
           float x[32];
           tmem_ld32_now(s_at + 32 * c, x);
+          if (!kAlias && c == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.s_free[i]);
+          }
           const float off = ev[c] - ref;
           float2 sum = make_float2(0.f, 0.f);
           uint32_t w[16];
@@ -775,71 +801,49 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           tmem_st16(p_at + 16 * c, w);             // where P takes the place of S: columns already read
           const float part = sum.x + sum.y;
           l += kF16 ? part * exp2_fast(-ev[c]) : part;
+          if (c & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c == 1 ? &b.p_half[i] : &b.p_full[i]);
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b.p_full[i]);
       }
       nk += n;
       if (!ok) break;
+      // every S of the unit is done: its queries make room for the next ones
+      const bool whole = u.whole != 0;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + u.slot) * piece_floats<kUnitRows>(dh);
+      __nv_bfloat16* dst = real ? out_row(p, u.first, u.h, r) : nullptr;
+      have = plans.next(u, lane);
+      if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
       if (mine > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&b.o_done[i], (ns - 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
       }
-      const bool whole = u.whole != 0;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + u.slot) * piece_floats<kUnitRows>(dh);
-      if (real && !whole) *reinterpret_cast<float2*>(piece + 2 * ru) = make_float2(m, l);
-      // out through the query tile, which every S of the unit has been made from: words of a row by neighbouring lanes
-      __nv_bfloat16* dst = real ? out_row(p, u.first, u.h, r) : nullptr;
-      __syncwarp();
-      if (whole) {
-#pragma unroll 2
-        for (int c = 0; c < ksteps; ++c) {
-          float o[16];
-          read_o(o, o_at, c, mine > 0);
-          st_shared_v4(swz(stage, row, 2 * c), pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
-                       pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-          st_shared_v4(swz(stage, row, 2 * c + 1), pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
-                       pack_bf16x2(o[12] * inv, o[13] * inv), pack_bf16x2(o[14] * inv, o[15] * inv));
+      if (real && !whole) reinterpret_cast<float2*>(piece)[ru] = make_float2(m, l);
+      float4* to = reinterpret_cast<float4*>(piece + 2 * kUnitRows) + ru;
+      for (int c = 0; c < ksteps; ++c) {
+        float o[16];
+        if (mine > 0) {
+          tmem_ld16_now(o_at + 16 * c, o);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = 0.f;
         }
-        __syncwarp();
+        if (!real) continue;
+        if (whole) {
+          uint32_t w[8];
 #pragma unroll
-        for (int c = 0; c < 8 * NA; ++c) {
-          __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), kRowStep * c + sub_row));
-          if (word < words) {
-            const uint4 v = ld_shared_v4(swz(stage, first_row + kRowStep * c + sub_row, word));
-            if (to != nullptr) st_global_v4(to + 8 * word, v.x, v.y, v.z, v.w);
-          }
-        }
-      } else {
-        // 32 columns of fp32, 128 bytes of a row, at a time
-        float* to = piece + 2 * kUnitRows + static_cast<size_t>(i * kTileRows + first_row) * dh;
-        const int rows = min(max(u.rows - i * kTileRows - first_row, 0), 32), w = lane & 7;
-        for (int c = 0; c < ksteps; c += 2) {
+          for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(o[2 * k] * inv, o[2 * k + 1] * inv);
+          st_global_v4(dst + 16 * c, w[0], w[1], w[2], w[3]);
+          st_global_v4(dst + 16 * c + 8, w[4], w[5], w[6], w[7]);
+        } else {                                   // four columns of all rows after four columns of all rows
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (c + h < ksteps) {
-              float o[16];
-              read_o(o, o_at, c + h, mine > 0);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                st_shared_v4(swz(stage, row, 4 * h + k), __float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]),
-                             __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
-            }
-          }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int from = 4 * k + (lane >> 3);
-            const uint4 v = ld_shared_v4(swz(stage, first_row + from, w));
-            if (from < rows && 16 * c + 4 * w < dh)
-              st_global_v4(to + static_cast<size_t>(from) * dh + 16 * c + 4 * w, v.x, v.y, v.z, v.w);
-          }
-          __syncwarp();
+          for (int k = 0; k < 4; ++k)
+            to[(4 * c + k) * kUnitRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
       }
       tc_fence_before();                           // O has been read: the next unit's P may follow
@@ -858,6 +862,46 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// What several blocks left of a unit, in order: a block takes 32 rows, a lane per row, a warp per sixteen columns.
+__global__ void __launch_bounds__(256) paged_merge_chunk_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int i = blockIdx.x, dh = p.w.c.dh, lane = threadIdx.x & 31, col = 16 * (threadIdx.x >> 5);
+  const int r = blockIdx.y * 32 + lane;
+  Unit u;
+  int last;
+  if (!shared_unit<kUnitRows>(p, i, lane, u, last)) return;
+  if (r >= u.rows) return;
+  float top = kFloor, sum = 0.f, a[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) a[k] = 0.f;
+#pragma unroll 2
+  for (int j = i; j <= last; ++j) {
+    const float* from = p.part + (2 * static_cast<size_t>(j) + (j == i ? 1 : 0)) * piece_floats<kUnitRows>(dh);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(from) + r);
+    const float4* o4 = reinterpret_cast<const float4*>(from + 2 * kUnitRows) + (col / 4) * kUnitRows + r;
+    float4 o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = __ldcg(o4 + k * kUnitRows);
+    const float most = fmaxf(top, ml.x), x = exp2_fast(top - most), w = exp2_fast(ml.x - most);
+    top = most;
+    sum = fmaf(sum, x, w * ml.y);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[4 * k] = fmaf(a[4 * k], x, w * o[k].x);
+      a[4 * k + 1] = fmaf(a[4 * k + 1], x, w * o[k].y);
+      a[4 * k + 2] = fmaf(a[4 * k + 2], x, w * o[k].z);
+      a[4 * k + 3] = fmaf(a[4 * k + 3], x, w * o[k].w);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(a[2 * k] * inv, a[2 * k + 1] * inv);
+  __nv_bfloat16* dst = out_row(p, u, u.rt * kUnitRows + r) + col;
+  st_global_v4(dst, w[0], w[1], w[2], w[3]);
+  st_global_v4(dst + 8, w[4], w[5], w[6], w[7]);
 }
 
 // Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (128 rows at most).
@@ -908,8 +952,7 @@ int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
   } else {
     rc = launch_dim<kInt8>(p, stream);
   }
-  return rc ? rc : launch_merge(paged_merge_rows_kernel<kUnitRows>, dim3(a.workers, kUnitRows / (kMergeRows * kMergeWarps)),
-                                32 * kMergeWarps, a, stream);
+  return rc ? rc : launch_merge(paged_merge_chunk_kernel, dim3(a.workers, kUnitRows / 32), 2 * a.w.c.dh, a, stream);
 }
 
 }  // namespace paged
