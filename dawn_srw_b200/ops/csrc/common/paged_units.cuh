@@ -195,8 +195,16 @@ __device__ __forceinline__ Run share(const AttnParams& p, int lane, long long wo
   const long long n = most < 1 ? 1 : most < p.workers ? most : p.workers;
   Run r = {0, 0, 0, 0, 0};
   if (worker >= n) return r;
-  r.begin = worker * total / n;
-  r.end = (worker + 1) * total / n;
+  // i T / n = i (T / n) + i (T mod n) / n, in 32 bits where T fits them: a 64-bit division costs some 500 cycles
+  if (total <= 0x7fffffffLL) {
+    const uint32_t t = static_cast<uint32_t>(total), d = static_cast<uint32_t>(n), w = static_cast<uint32_t>(worker);
+    const uint32_t whole = t / d, rest = t - whole * d;              // rest, w + 1 <= n: their product fits
+    r.begin = static_cast<long long>(w) * whole + w * rest / d;
+    r.end = static_cast<long long>(w + 1) * whole + (w + 1) * rest / d;
+  } else {
+    r.begin = worker * total / n;
+    r.end = (worker + 1) * total / n;
+  }
   for (int i = 0; i < B; i += 32) {                    // the sequence that holds tile r.begin
     if (B > 32) x = head_tiles<ROWS, TP>(p, i, lane);
     long long c = x * H;
@@ -416,12 +424,14 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_few_kernel(const At
   }
 }
 
-// After the kernel that leaves the pieces, in its stream; launched early, it waits for that kernel's end by itself.
-template <typename F>
-int launch_merge(F* kernel, dim3 grid, int threads, const AttnParams& p, cudaStream_t stream) {
+// Launches a kernel that waits by itself (griddepcontrol.wait) for the stream's earlier work before it reads anything:
+// its blocks may be set up while that work ends.
+template <typename F, typename P>
+int launch_early(F* kernel, dim3 grid, int threads, int smem, const P& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

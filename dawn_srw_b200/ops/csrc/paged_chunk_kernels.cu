@@ -146,6 +146,24 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// 2^x for two x below 100 on the FMA units: the exponential unit, a sixteenth of a lane per cycle, is what the softmax
+// waits for, so it makes only some of them.  Cody and Waite's reduction to n + f, f in [-1/2, 1/2], and a polynomial in
+// f of degree 4 with value 1 at 0, fitted here to the least relative error (3e-6); n goes into the exponent's bits.
+// Below -127, and at -inf, the result is 0.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f);                    // 1.5 * 2^23: n in the low bits
+  const float2 t = add2(x, magic), f = add2(x, make_float2(12582912.f - t.x, 12582912.f - t.y));
+  float2 p = fma2(f, make_float2(0.009582813829183578f, 0.009582813829183578f), make_float2(0.055906426161527634f, 0.055906426161527634f));
+  p = fma2(p, f, make_float2(0.24024099111557007f, 0.24024099111557007f));
+  p = fma2(p, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
+  p = fma2(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+constexpr int kPoly = 1, kPolyOf = 4;       // the share of the exponentials that are made this way
+
 // Instruction descriptor, kind::f16, fp32 accumulators: A and B both bf16 or both fp16.
 __host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn_major) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(b_mn_major) << 16) |
@@ -180,11 +198,11 @@ static_assert(sizeof(Plan) <= 128, "slot of a plan");
 
 __device__ __forceinline__ int place(const Plan& q, int j) { return (q.t0 + j < q.st ? q.t0 + j : q.t0 + j + q.skip) * kTP; }
 
-// Bit k: a row at position pos sees position x + k; gone: bits of the two sixteens from x.
-__device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks, uint32_t gone) {
+// Bit k: a row at position pos sees position x + k.
+__device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks) {
   auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
   const uint32_t by = below(pos - x + 1), old = below(pos - window + 1 - x) & ~below(sinks - x);
-  return by & ~old & ((gone & 1u) ? 0xffff0000u : 0xffffffffu) & ((gone & 2u) ? 0x0000ffffu : 0xffffffffu);
+  return by & ~old;
 }
 
 // D = A B^T over KS steps of sixteen columns, both K-major.
@@ -197,6 +215,12 @@ __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uin
   }
 }
 
+// A whole sector of 32 bytes in one store.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 // 16 bytes to shared memory, zeros where `on` is false (nothing is read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -329,6 +353,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   auto o_col = [&](int i) { return tmem + 256 + 64 * NA * i; };
   auto p_col = [&](int i) { return kAlias ? s_col(i) : tmem + 384 + 64 * i; };
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the stream's earlier work: from here on its results are read
   Plan* plan_ring = reinterpret_cast<Plan*>(smem + L::kPlan);
   static_assert(kPlans * sizeof(Plan) <= kPlans * 128, "ring of plans");
   Plans plans = {plan_ring, b.plan_full, b.plan_empty, abort_flag, 0};
@@ -727,12 +752,20 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         if (hidden) {
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
-            float x[16];
-            tmem_ld16_now(s_at + 16 * c, x);
-            const uint32_t seen = seen32(x0 + 16 * c, pos, p.window, p.sinks, gone >> (8 * (c >> 1) + (c & 1)));
+            const int x = x0 + 16 * c;                 // sixteen columns: most are seen, or not, by all rows of a warp
+            const uint32_t away = gone >> (8 * (c >> 1) + (c & 1)) & 1u;
+            if (away == 0u && x + 15 <= pos_lo && (x > pos_hi - p.window || x + 15 < p.sinks)) continue;
             uint32_t w[16];
+            if (away != 0u || x > pos_hi || (x + 15 <= pos_lo - p.window && x >= p.sinks)) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) w[k] = (seen >> k) & 1u ? __float_as_uint(x[k]) : 0xff800000u;
+              for (int k = 0; k < 16; ++k) w[k] = 0xff800000u;
+            } else {
+              float y[16];
+              tmem_ld16_now(s_at + 16 * c, y);
+              const uint32_t seen = seen32(x, pos, p.window, p.sinks);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) w[k] = (seen >> k) & 1u ? __float_as_uint(y[k]) : 0xff800000u;
+            }
             tmem_st16(s_at + 16 * c, w);
           }
           tmem_st_wait();
@@ -793,8 +826,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(fc[c], fc[c]), make_float2(off, off));
-            y.x = exp2_fast(y.x);
-            y.y = exp2_fast(y.y);
+            y = (k / 2) % kPolyOf < kPoly ? exp2_poly(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
             sum = add2(sum, y);
             w[k / 2] = kF16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
           }
@@ -838,8 +870,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           uint32_t w[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(o[2 * k] * inv, o[2 * k + 1] * inv);
-          st_global_v4(dst + 16 * c, w[0], w[1], w[2], w[3]);
-          st_global_v4(dst + 16 * c + 8, w[4], w[5], w[6], w[7]);
+          st_global_v8(dst + 16 * c, w);
         } else {                                   // four columns of all rows after four columns of all rows
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -900,8 +931,7 @@ __global__ void __launch_bounds__(256) paged_merge_chunk_kernel(const AttnParams
 #pragma unroll
   for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(a[2 * k] * inv, a[2 * k + 1] * inv);
   __nv_bfloat16* dst = out_row(p, u, u.rt * kUnitRows + r) + col;
-  st_global_v4(dst, w[0], w[1], w[2], w[3]);
-  st_global_v4(dst + 8, w[4], w[5], w[6], w[7]);
+  st_global_v8(dst, w);
 }
 
 // Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (128 rows at most).
@@ -924,8 +954,7 @@ int launch(const ChunkParams& p, cudaStream_t stream) {
   if (cudaFuncSetAttribute(paged_chunk_kernel<KIND, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA>::kTotal) !=
       cudaSuccess)
     return 950;
-  paged_chunk_kernel<KIND, NA><<<p.a.workers, kThreadsOf<KIND>, Smem<NA>::kTotal, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : 951;
+  return launch_early(paged_chunk_kernel<KIND, NA>, dim3(p.a.workers), kThreadsOf<KIND>, Smem<NA>::kTotal, p, stream) ? 951 : 0;
 }
 
 template <int KIND>
@@ -952,7 +981,7 @@ int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
   } else {
     rc = launch_dim<kInt8>(p, stream);
   }
-  return rc ? rc : launch_merge(paged_merge_chunk_kernel, dim3(a.workers, kUnitRows / 32), 2 * a.w.c.dh, a, stream);
+  return rc ? rc : launch_early(paged_merge_chunk_kernel, dim3(a.workers, kUnitRows / 32), 2 * a.w.c.dh, 0, a, stream);
 }
 
 }  // namespace paged

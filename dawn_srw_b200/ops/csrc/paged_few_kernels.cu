@@ -519,7 +519,7 @@ int launch(AttnParams& p, int max_rt, cudaStream_t stream) {
   if (with_smem(paged_few_run_kernel<KIND, KD, NT>, bytes)) return 944;
   paged_few_run_kernel<KIND, KD, NT><<<p.workers / kWarps, 32 * kWarps, bytes, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 945;
-  return launch_merge(paged_merge_few_kernel<W::kRows>, dim3(p.workers), kMergeThreads, p, stream);
+  return launch_early(paged_merge_few_kernel<W::kRows>, dim3(p.workers), kMergeThreads, 0, p, stream);
 }
 
 // Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.
