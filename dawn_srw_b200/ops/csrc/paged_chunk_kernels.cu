@@ -162,7 +162,10 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
-constexpr int kPoly = 1, kPolyOf = 4;       // the share of the exponentials that are made this way
+// How many of sixteen exponentials are made this way.  With four loading warps beside the softmax the issue slots are
+// what is short, not the exponential unit: 4099 tokens over 16000 int8 positions took 183 us with none, 196 with four
+// and 220 with eight; ragged bf16 prompts of up to 2048 tokens 105, 101 (three), 102 and 107 us.
+template <int KIND> constexpr int kPoly = KIND == kBf16 ? 3 : 0;
 
 // Instruction descriptor, kind::f16, fp32 accumulators: A and B both bf16 or both fp16.
 __host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn_major) {
@@ -301,6 +304,7 @@ template <int KIND, int NA>
 __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   using L = Smem<NA>;
   constexpr bool kF16 = KIND != kBf16;
+  constexpr bool kAhead = kF16;                 // columns of S loaded one step ahead (183 us for 194; bf16 103 for 101)
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -811,10 +815,17 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         // fp16 weights: 2^14 at most, so that 2^-24 of one is 2^-30 of the reference
         const float ref = kF16 ? m - 6.f : m;
+        float xs[2][32];
+        if (kAhead) tmem_ld32(s_at, xs[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float x[32];
-          tmem_ld32_now(s_at + 32 * c, x);
+          float* x = xs[kAhead ? c & 1 : 0];
+          if (kAhead) {
+            tmem_ld_wait_dep32(x);
+            if (c < 3) tmem_ld32(s_at + 32 * (c + 1), xs[(c + 1) & 1]);
+          } else {
+            tmem_ld32_now(s_at + 32 * c, x);
+          }
           if (!kAlias && c == 3) {
             tc_fence_before();
             __syncwarp();
@@ -826,7 +837,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(fc[c], fc[c]), make_float2(off, off));
-            y = (k / 2) % kPolyOf < kPoly ? exp2_poly(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            y = (k / 2) % 16 < kPoly<KIND> ? exp2_poly(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
             sum = add2(sum, y);
             w[k / 2] = kF16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
           }
