@@ -144,12 +144,12 @@ Tensor paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, cons
   const int64_t top = 0x7fffffffLL;
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
   const int hint = static_cast<int>(std::min<int64_t>(max_new.has_value() ? *max_new : starts.has_value() ? q.size(0) : 1, top));
-  const int64_t bytes = dsb_paged_attention_workspace(&c, static_cast<int>(Hq), hint);
+  const int win = window.has_value() ? static_cast<int>(std::min(*window, top)) : 0, snk = static_cast<int>(std::min(sinks, top));
+  const int64_t bytes = dsb_paged_attention_workspace(&c, static_cast<int>(Hq), hint, win, snk);
   Tensor ws;                    // of this call alone: captured graphs and streams share nothing
   if (bytes > 0) ws = torch::empty({bytes}, kp.options().dtype(torch::kUInt8));
   const int rc = dsb_paged_attention(&c, qr.data_ptr(), qr.stride(0), qr.stride(1), out.data_ptr(), static_cast<int>(Hq),
-                                     hint, window.has_value() ? static_cast<int>(std::min(*window, top)) : 0,
-                                     static_cast<int>(std::min(sinks, top)), static_cast<float>(s),
+                                     hint, win, snk, static_cast<float>(s),
                                      bytes > 0 ? ws.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "dsb_paged_attention failed with code ", rc);
   return out;

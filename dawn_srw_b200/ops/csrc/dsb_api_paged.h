@@ -37,7 +37,7 @@ int dsb_paged_read(const struct DsbPaged* c, void* k, void* v, int dst_bf16, int
 // of H; B and H at most 65535.  A row without a key, or of no sequence, is zero.  max_new: the most new tokens a
 // sequence has, as far as the caller knows (it chooses the kernel; a wrong one costs time only).  workspace:
 // dsb_paged_attention_workspace bytes of scratch, 16-byte aligned, this call's alone while it runs.
-long long dsb_paged_attention_workspace(const struct DsbPaged* c, int Hq, int max_new);
+long long dsb_paged_attention_workspace(const struct DsbPaged* c, int Hq, int max_new, int window, int sinks);
 int dsb_paged_attention(const struct DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
                         int max_new, int window, int sinks, float scale, void* workspace, cudaStream_t stream);
 

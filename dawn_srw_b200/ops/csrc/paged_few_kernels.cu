@@ -11,10 +11,10 @@
 // each row that brings the largest to [128, 256): exact down to 2^-22 of it, off by 2^-33 of it below.  The keys'
 // scales go to the scores in fp32, the values' to the exponents (see below).  Running maximum and sum stay in registers.
 //
-// Two ways to share the work: short caches take one block per unit, its warps interleaved over the tiles and merged
-// in shared memory: one launch.  Long ones take as many warps as the GPU holds, each with an equal run of consecutive
-// tiles of all units; a unit that several warps share is left in pieces, which a second kernel adds up in order.  The
-// lengths are read on the device, so a captured call follows them.
+// Two ways to share the work.  Where a warp has few tiles, a cluster of blocks takes a unit, its warps every n-th tile,
+// and merges in (distributed) shared memory: one launch.  For long caches as many warps as the GPU holds take equal
+// runs of consecutive tiles of all units, whatever the sequences' lengths; a unit that several warps share is left in
+// pieces, which a second kernel adds up in order.  The lengths are read on the device, so a captured call follows them.
 #include "common/paged_launch.h"
 #include "common/ptx.cuh"
 
@@ -389,26 +389,40 @@ struct Warp {
   }
 };
 
-// One block per unit: grid (row tiles, heads, sequences); more row tiles than the grid has are taken in turn.
+constexpr int kMostWarps = 12;          // of a block: what fits an SM
+
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// A cluster of blocks per unit, every warp every n-th tile: grid (blocks of a cluster x row tiles, heads, sequences);
+// more row tiles than the grid has are taken in turn.
 template <int KIND, int KD, int NT>
-__global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(const AttnParams p, int blocks) {
   using W = Warp<KIND, KD, NT>;
+  static_assert(2 * W::kRows * (16 * KD + 4) * 4 <= W::R::kBytes, "two O fit a warp's ring");
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float s_ml[kWarps][W::kRows][2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
-  const int ld = dh + 4;                               // of a row of O: the merge's rows fall on different banks
-  float* s_o = reinterpret_cast<float*>(smem);         // [kWarps][kRows][ld], over the rings once they are read
+  __shared__ float s_ml[kMostWarps][W::kRows][2];
+  __shared__ float s_all[W::kRows][2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
+  const int ld = dh + 4, per = dh / 4;                 // floats between rows of O: the merge's rows fall on different banks
+  const int rank = blocks > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  auto o_of = [&](int w) { return reinterpret_cast<float*>(smem + w * W::R::kBytes); };      // over the ring once it is read
+  float* mine = o_of(warp);
+  float* both = o_of(0) + W::kRows * ld;               // the block's O, for the cluster
   if (blockIdx.x == 0 && blockIdx.y == 0) zero_other_rows(p, blockIdx.z * blockDim.x + threadIdx.x, gridDim.z * blockDim.x);
   Unit u;
   unit_sequence(p, u, blockIdx.z);
   u.h = blockIdx.y;
-  const int nrt = row_tiles<W::kRows>(u.n, p.G);
-  for (u.rt = blockIdx.x; u.rt < nrt; u.rt += gridDim.x) {
+  const int nrt = row_tiles<W::kRows>(u.n, p.G), step = gridDim.x / blocks;
+  for (u.rt = blockIdx.x / blocks; u.rt < nrt; u.rt += step) {
     unit_range<W::kRows, W::kTP>(p, u);
     W s;
     s.begin(p, u, g, t);
-    s.run(p, u, warp, u.tiles, kWarps, lane, smem_u32(smem) + warp * W::R::kBytes);
-    __syncthreads();
+    s.run(p, u, rank * warps + warp, u.tiles, blocks * warps, lane, smem_u32(mine));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -417,8 +431,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const A
 #pragma unroll
         for (int c = 0; c < KD; ++c)
           if (16 * c < dh) {
-            s_o[(warp * W::kRows + r) * ld + W::column(c, 0, g)] = s.o[nt][c][e];
-            s_o[(warp * W::kRows + r) * ld + W::column(c, 1, g)] = s.o[nt][c][2 + e];
+            mine[r * ld + W::column(c, 0, g)] = s.o[nt][c][e];
+            mine[r * ld + W::column(c, 1, g)] = s.o[nt][c][2 + e];
           }
         if (g == 0) {
           s_ml[warp][r][0] = s.m[nt][e];
@@ -426,26 +440,57 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_block_kernel(const A
         }
       }
     __syncthreads();
-    for (int i = threadIdx.x; i < u.rows * (dh / 4); i += blockDim.x) {
-      const int r = i / (dh / 4), c = 4 * (i - r * (dh / 4));
-      float top = kFloor, sum = 0.f, f[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][r][0]);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+    for (int i = threadIdx.x; i < u.rows * per; i += blockDim.x) {
+      const int r = i / per, c = 4 * (i - r * per);
+      float top = kFloor, sum = 0.f;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < warps; ++w) top = fmaxf(top, s_ml[w][r][0]);
+      for (int w = 0; w < warps; ++w) {
         const float x = exp2_fast(s_ml[w][r][0] - top);
-        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * W::kRows + r) * ld + c);
+        const float4 v = *reinterpret_cast<const float4*>(o_of(w) + r * ld + c);
         sum = fmaf(x, s_ml[w][r][1], sum);
-        f[0] = fmaf(x, v.x, f[0]);
-        f[1] = fmaf(x, v.y, f[1]);
-        f[2] = fmaf(x, v.z, f[2]);
-        f[3] = fmaf(x, v.w, f[3]);
+        f.x = fmaf(x, v.x, f.x);
+        f.y = fmaf(x, v.y, f.y);
+        f.z = fmaf(x, v.z, f.z);
+        f.w = fmaf(x, v.w, f.w);
       }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
-          make_uint2(pack_bf16x2(f[0] * inv, f[1] * inv), pack_bf16x2(f[2] * inv, f[3] * inv));
+      if (blocks > 1) {
+        *reinterpret_cast<float4*>(both + r * ld + c) = f;
+        if (c == 0) {
+          s_all[r][0] = top;
+          s_all[r][1] = sum;
+        }
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
+            make_uint2(pack_bf16x2(f.x * inv, f.y * inv), pack_bf16x2(f.z * inv, f.w * inv));
+      }
     }
-    __syncthreads();                                   // before the next unit's copies
+    if (blocks > 1) {
+      cluster_sync_all();
+      for (int i = rank * blockDim.x + threadIdx.x; i < u.rows * per; i += blocks * blockDim.x) {
+        const int r = i / per, c = 4 * (i - r * per);
+        const uint32_t ml = smem_u32(s_all[r]), at = smem_u32(both + r * ld + c);
+        float top = kFloor, sum = 0.f;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < blocks; ++k) top = fmaxf(top, ld_cluster_f32(mapa_shared(ml, k)));
+        for (int k = 0; k < blocks; ++k) {
+          const float x = exp2_fast(ld_cluster_f32(mapa_shared(ml, k)) - top);
+          const float4 v = ld_cluster_f32x4(mapa_shared(at, k));
+          sum = fmaf(x, ld_cluster_f32(mapa_shared(ml + 4, k)), sum);
+          f.x = fmaf(x, v.x, f.x);
+          f.y = fmaf(x, v.y, f.y);
+          f.z = fmaf(x, v.z, f.z);
+          f.w = fmaf(x, v.w, f.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
+            make_uint2(pack_bf16x2(f.x * inv, f.y * inv), pack_bf16x2(f.z * inv, f.w * inv));
+      }
+      cluster_sync_all();                              // nobody goes on while its memory may still be read
+    } else {
+      __syncthreads();                                 // before the next unit's copies
+    }
   }
 }
 
@@ -459,6 +504,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
   const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * W::R::kBytes;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, dh = p.w.c.dh;
   const int worker = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   zero_other_rows(p, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
   int4 meta = make_int4(-1, 0, 0, 0);
   Segments<W::kRows, W::kTP> seg;
@@ -498,8 +544,29 @@ constexpr int kBlocksPerSm = 3;
 
 int few_workers() { return device_sms() * kBlocksPerSm * kWarps; }
 
-// Short caches: a block per unit.
-bool by_blocks(const DsbPaged* c) { return static_cast<long long>(c->width) * c->page <= 1024; }
+// How the work is shared: `blocks` = 0: equal runs; else clusters of that many blocks of `warps` warps per unit.
+struct Sharing { int blocks, warps; };
+
+// The warps that the GPU holds (twelve an SM) are dealt to the units; a unit gets as many as its tiles at most.  What a
+// sequence really has is not known here, only what its table holds and a window leaves of it.  Above kLong positions
+// for a warp the differences between sequences cost more than the plan, the pieces and the merge of equal runs.
+Sharing sharing(const DsbPaged* c, int window, int sinks, int max_new, long long units) {
+  constexpr int kLong = 1024;
+  long long most = static_cast<long long>(c->width) * c->page;
+  if (window > 0 && static_cast<long long>(window) + sinks + max_new < most) most = static_cast<long long>(window) + sinks + max_new;
+  long long w = static_cast<long long>(kMostWarps) * device_sms() / (units > 0 ? units : 1);
+  const long long tiles = (most + 31) / 32;
+  if (w > tiles) w = tiles;
+  if (w < 1) w = 1;
+  if (w > 8 * kMostWarps) w = 8 * kMostWarps;
+  Sharing s = {1, static_cast<int>(w)};
+  if (w > kMostWarps) {
+    s.warps = w / 6 <= 8 ? 6 : kMostWarps;
+    s.blocks = static_cast<int>(w / s.warps);
+  }
+  if (most > static_cast<long long>(kLong) * s.blocks * s.warps) s.blocks = 0;
+  return s;
+}
 
 template <typename F>
 int with_smem(F* kernel, int bytes) {
@@ -507,53 +574,65 @@ int with_smem(F* kernel, int bytes) {
 }
 
 template <int KIND, int KD, int NT>
-int launch(AttnParams& p, int max_rt, cudaStream_t stream) {
+int launch(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
   using W = Warp<KIND, KD, NT>;
-  constexpr int bytes = kWarps * (W::R::kBytes > W::kRows * (16 * KD + 4) * 4 ? W::R::kBytes : W::kRows * (16 * KD + 4) * 4);
-  if (by_blocks(&p.w.c)) {
-    if (with_smem(paged_few_block_kernel<KIND, KD, NT>, bytes)) return 944;
-    const dim3 grid(max_rt, p.w.c.H, p.w.c.B);
-    paged_few_block_kernel<KIND, KD, NT><<<grid, 32 * kWarps, bytes, stream>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : 945;
+  if (how.blocks > 0) {
+    const int bytes = how.warps * W::R::kBytes;
+    if (with_smem(paged_few_unit_kernel<KIND, KD, NT>, bytes)) return 944;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(max_rt * how.blocks, p.w.c.H, p.w.c.B);
+    cfg.blockDim = dim3(32 * how.warps);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = how.blocks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = how.blocks > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, paged_few_unit_kernel<KIND, KD, NT>, p, how.blocks) == cudaSuccess ? 0 : 945;
   }
+  constexpr int bytes = kWarps * W::R::kBytes;
   if (with_smem(paged_few_run_kernel<KIND, KD, NT>, bytes)) return 944;
-  paged_few_run_kernel<KIND, KD, NT><<<p.workers / kWarps, 32 * kWarps, bytes, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return 945;
+  if (launch_early(paged_few_run_kernel<KIND, KD, NT>, dim3(p.workers / kWarps), 32 * kWarps, bytes, p, stream)) return 945;
   return launch_early(paged_merge_few_kernel<W::kRows>, dim3(p.workers), kMergeThreads, 0, p, stream);
 }
 
 // Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.
 template <int KIND, int NT>
-int launch_dim(AttnParams& p, int max_rt, cudaStream_t stream) {
+int launch_dim(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
   const int dh = p.w.c.dh;
-  if (dh <= 32) return launch<KIND, 2, NT>(p, max_rt, stream);
-  if (dh <= 64) return launch<KIND, 4, NT>(p, max_rt, stream);
-  if (dh <= 80) return launch<KIND, 5, NT>(p, max_rt, stream);
-  return launch<KIND, 8, NT>(p, max_rt, stream);
+  if (dh <= 32) return launch<KIND, 2, NT>(p, max_rt, how, stream);
+  if (dh <= 64) return launch<KIND, 4, NT>(p, max_rt, how, stream);
+  if (dh <= 80) return launch<KIND, 5, NT>(p, max_rt, how, stream);
+  return launch<KIND, 8, NT>(p, max_rt, how, stream);
 }
 
 template <int KIND>
-int launch_rows(AttnParams& p, long long rows, cudaStream_t stream) {
-  if (rows <= 8) return launch_dim<KIND, 1>(p, 1, stream);
-  const long long rt = (rows + 15) / 16;
-  return launch_dim<KIND, 2>(p, static_cast<int>(rt > 65535 ? 65535 : rt), stream);
+int launch_rows(AttnParams& p, long long rows, const Sharing& how, cudaStream_t stream) {
+  return rows <= 8 ? launch_dim<KIND, 1>(p, 1, how, stream) : launch_dim<KIND, 2>(p, 1, how, stream);
 }
 
 }  // namespace
 
-long long few_workspace(const DsbPaged* c, int rows) {
-  return by_blocks(c) ? 0 : workspace_bytes(few_workers(), rows <= 8 ? 8 : 16, c->dh);
+long long few_workspace(const DsbPaged* c, int window, int sinks, int max_new, int rows) {
+  const Sharing how = sharing(c, window, sinks, max_new, static_cast<long long>(c->B) * c->H);
+  return how.blocks > 0 ? 0 : workspace_bytes(few_workers(), rows <= 8 ? 8 : 16, c->dh);
 }
 
-int launch_few(AttnParams& p, long long rows, void* workspace, cudaStream_t stream) {
-  if (!by_blocks(&p.w.c)) {
+int launch_few(AttnParams& p, int window, int sinks, int max_new, long long rows, void* workspace, cudaStream_t stream) {
+  const Sharing how = sharing(&p.w.c, window, sinks, max_new, static_cast<long long>(p.w.c.B) * p.w.c.H);
+  if (how.blocks == 0) {
     p.workers = few_workers();
     p.meta = static_cast<int4*>(workspace);
     p.part = reinterpret_cast<float*>(p.meta + p.workers);
   }
-  if (p.w.c.kind == kBf16) return launch_rows<kBf16>(p, rows, stream);
-  if (p.w.c.kind == kE4m3) return launch_rows<kE4m3>(p, rows, stream);
-  return launch_rows<kInt8>(p, rows, stream);
+  if (p.w.c.kind == kBf16) return launch_rows<kBf16>(p, rows, how, stream);
+  if (p.w.c.kind == kE4m3) return launch_rows<kE4m3>(p, rows, how, stream);
+  return launch_rows<kInt8>(p, rows, how, stream);
 }
 
 }  // namespace paged

@@ -251,17 +251,15 @@ namespace {
 // Query rows of a head above which the tensor cores take over (units of 256 rows).
 constexpr long long kFewRows = 16;
 
-long long rows_of(const DsbPaged* c, int Hq, int max_new) {
-  const long long most = max_new < 1 ? 1 : max_new > c->N ? c->N : max_new;
-  return most * (Hq / c->H);
-}
+int new_of(const DsbPaged* c, int max_new) { return max_new < 1 ? 1 : max_new > c->N ? c->N : max_new; }
 
 }  // namespace
 
-extern "C" long long dsb_paged_attention_workspace(const DsbPaged* c, int Hq, int max_new) {
+extern "C" long long dsb_paged_attention_workspace(const DsbPaged* c, int Hq, int max_new, int window, int sinks) {
   if (bad_cache(c) || c->N == 0 || c->B == 0) return 0;
-  const long long rows = rows_of(c, Hq, max_new);
-  return rows <= kFewRows ? few_workspace(c, static_cast<int>(rows)) : chunk_workspace(c);
+  max_new = new_of(c, max_new);
+  const long long rows = static_cast<long long>(max_new) * (Hq / c->H);
+  return rows <= kFewRows ? few_workspace(c, window, sinks, max_new, static_cast<int>(rows)) : chunk_workspace(c);
 }
 
 extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q_st, long long q_sh, void* out, int Hq,
@@ -275,7 +273,7 @@ extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q
     const size_t bytes = static_cast<size_t>(c->N) * Hq * c->dh * sizeof(__nv_bfloat16);
     return cudaMemsetAsync(out, 0, bytes, stream) == cudaSuccess ? 0 : 942;
   }
-  if (workspace == nullptr && dsb_paged_attention_workspace(c, Hq, max_new) > 0) return 943;
+  if (workspace == nullptr && dsb_paged_attention_workspace(c, Hq, max_new, window, sinks) > 0) return 943;
   AttnParams p;
   p.w = make_view(c);
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -291,6 +289,7 @@ extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q
   p.part = nullptr;
   p.meta = nullptr;
   p.workers = 0;
-  const long long rows = rows_of(c, Hq, max_new);
-  return rows <= kFewRows ? launch_few(p, rows, workspace, stream) : launch_chunk(p, workspace, stream);
+  max_new = new_of(c, max_new);
+  const long long rows = static_cast<long long>(max_new) * p.G;
+  return rows <= kFewRows ? launch_few(p, window, sinks, max_new, rows, workspace, stream) : launch_chunk(p, workspace, stream);
 }
