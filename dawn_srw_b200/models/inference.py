@@ -10,6 +10,9 @@ build_suppressed_forward :2246-2338):
 * ``decode_step(model, tok, cache_K, cache_V, length)`` -> ``(logits [B,V],
   cache_K, cache_V, length + 1)``;
 * ``generate(model, ids, ...)``: KV-cache sampler with temperature / top-k;
+* ``PagedSession(model, max_seqs, ...)``: sequences of their own lengths over one paged cache (bf16, e4m3 or
+  int8), prompts in chunks, single tokens in a CUDA graph, an optional attention window with sinks (no
+  counterpart in the reference, whose caches are dense, fp32 and of one length for the batch);
 * ``vectorized_eval(model, batches)`` -> ``(avg_loss, ppl, acc %, n_valid)``;
   note its valid mask is ``label > 0`` (pad id 0), unlike training's
   ``label != -100`` — kept as in the reference and documented;
@@ -34,6 +37,7 @@ import torch
 
 from ..ops import reference as R
 from ..ops.backend import ParallelCtx
+from ..ops.paged import PAGE_DTYPES
 
 
 def _be(model, device):
@@ -312,6 +316,236 @@ class DecodeSession:
         return self.out.clone()
 
 
+class PagedSession:
+    """Decoding of up to ``max_seqs`` sequences, each of its own length, over one paged key/value cache.
+
+    Keys and values live in pages ``[n_layers, n_pages, H, page_size, dh]`` in bf16, or as e4m3 / int8 codes
+    with an fp32 scale for each position and head (``kv_dtype``); a sequence takes pages from a common pool
+    as it grows and gives them back when it is freed.  With ``window`` a token attends to the last
+    ``window`` positions and the first ``sinks`` ones only, and pages that no later token can see go back
+    to the pool early.
+
+        s = PagedSession(model, max_seqs=8, kv_dtype="e4m3")
+        a, b = s.open(), s.open()
+        logits = s.extend({a: ids_a, b: ids_b})     # prompts, or further chunks of them: [2, V], last tokens
+        logits = s.step({a: tok_a, b: tok_b})       # one token each: a CUDA graph on a GPU
+        s.close(a)
+
+    Attention reads what the pages hold, so the logits are those of the rounded cache.  Dense and SRW models;
+    pools must not be sharded."""
+
+    def __init__(self, model, max_seqs: int, *, n_pages: Optional[int] = None, page_size: int = 16,
+                 kv_dtype: str = "bf16", window: Optional[int] = None, sinks: int = 0,
+                 use_graph: Optional[bool] = None):
+        if kv_dtype not in PAGE_DTYPES:
+            raise ValueError(f"kv_dtype {kv_dtype!r} is none of {sorted(PAGE_DTYPES)}")
+        if max_seqs < 1 or page_size < 16 or page_size > 256 or page_size & (page_size - 1):
+            raise ValueError("max_seqs must be positive and page_size a power of two from 16 to 256")
+        if window is not None and window < 1 or sinks < 0:
+            raise ValueError("window must be at least 1 (None: no window), sinks not negative")
+        if not _is_dense(model) and model.shard_group is not None:
+            raise ValueError("a paged session needs unsharded pools")
+        self.model, self.page_size, self.window, self.sinks = model, page_size, window, sinks
+        dev = model.token_emb.weight.device
+        self.be = _be(model, dev)
+        L, H = model.n_layers, model.n_heads
+        dh = model.d_model // H
+        self.width = -(-model.max_seq_len // page_size)
+        n_pages = max_seqs * self.width if n_pages is None else int(n_pages)
+        dtype = PAGE_DTYPES[kv_dtype]
+        shape = (L, n_pages, H, page_size, dh)
+        self.k_pages, self.v_pages = torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev)
+        scaled = dtype != torch.bfloat16
+        self.k_scale = torch.ones(shape[:4], device=dev) if scaled else None
+        self.v_scale = torch.ones(shape[:4], device=dev) if scaled else None
+        self._layers = [(self.k_pages[l], self.v_pages[l],
+                         dict(k_scale=self.k_scale[l] if scaled else None, v_scale=self.v_scale[l] if scaled else None))
+                        for l in range(L)]
+        self.free_pages = list(range(n_pages - 1, -1, -1))
+        self.pages: List[Optional[List[int]]] = [None] * max_seqs      # of each open sequence; -1: given back
+        self.lengths = [0] * max_seqs
+        self.max_seqs = max_seqs
+        z = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)
+        self._table, self._len, self._tok = z(max_seqs, self.width), z(max_seqs), z(max_seqs).long()
+        self._graph = self._out = None
+        self._pools = self._key = None
+        self._params = list(model.parameters())
+        self.use_graph = dev.type == "cuda" if use_graph is None else bool(use_graph)
+
+    # ---- sequences and pages -------------------------------------------
+    def open(self) -> int:
+        """A new, empty sequence; its number."""
+        for s, p in enumerate(self.pages):
+            if p is None:
+                self.pages[s], self.lengths[s] = [], 0
+                return s
+        raise RuntimeError(f"all {self.max_seqs} sequences are open")
+
+    def close(self, seq: int) -> None:
+        """The sequence ends; its pages go back to the pool."""
+        self._check(seq)
+        self.free_pages.extend(p for p in self.pages[seq] if p >= 0)
+        self.pages[seq], self.lengths[seq] = None, 0
+
+    def _check(self, seq: int) -> None:
+        if not 0 <= seq < self.max_seqs or self.pages[seq] is None:
+            raise ValueError(f"sequence {seq} is not open")
+
+    def _grow(self, new: Dict[int, int]) -> None:
+        """Room for ``new`` tokens of each sequence, or an error that changes nothing."""
+        need = 0
+        for s, n in new.items():
+            self._check(s)
+            if n < 1:
+                raise ValueError(f"sequence {s}: no new token")
+            if self.lengths[s] + n > self.model.max_seq_len:
+                raise ValueError(f"sequence {s}: {self.lengths[s]} + {n} tokens exceed max_seq_len")
+            need += -(-(self.lengths[s] + n) // self.page_size) - len(self.pages[s])
+        if need > len(self.free_pages):
+            raise RuntimeError(f"paged cache is full: {need} pages wanted, {len(self.free_pages)} free")
+        for s, n in new.items():
+            self.lengths[s] += n
+            while len(self.pages[s]) * self.page_size < self.lengths[s]:
+                self.pages[s].append(self.free_pages.pop())
+
+    def _forget(self, seqs) -> None:
+        """Pages that no later token sees go back to the pool."""
+        if self.window is None:
+            return
+        first = -(-self.sinks // self.page_size)
+        for s in seqs:
+            last = max(0, self.lengths[s] + 1 - self.window) // self.page_size      # the next token's first page
+            for i in range(first, last):
+                if self.pages[s][i] >= 0:
+                    self.free_pages.append(self.pages[s][i])
+                    self.pages[s][i] = -1
+
+    def _table_of(self, seqs, width: int) -> torch.Tensor:
+        t = torch.full((len(seqs), width), -1, dtype=torch.int32)
+        for i, s in enumerate(seqs):
+            p = self.pages[s] or []
+            t[i, : len(p)] = torch.tensor(p, dtype=torch.int32)
+        return t
+
+    # ---- forward -------------------------------------------------------
+    def _forward(self, x, table, lengths, starts, max_new):
+        """Final hidden states [T, D] of packed new tokens x [T, D]."""
+        m, be, H = self.model, self.be, self.model.n_heads
+        T, D = x.shape
+        dh, dense = D // H, _is_dense(m)
+        heads = lambda t: t.reshape(T, H, dh)
+        for li, blk in enumerate(m.layers):
+            kp, vp, scales = self._layers[li]
+            n = be.layer_norm(x, blk.norm1.weight, blk.norm1.bias).reshape(T, D)
+            if dense:
+                q, k, v = (be.linear(n, w.weight, w.bias) for w in (blk.attn.q_proj, blk.attn.k_proj, blk.attn.v_proj))
+            else:
+                q, k, v, _, _ = _layer_qkv(m, be, n, self._pools)
+            be.paged_write(heads(k).float(), heads(v).float(), kp, vp, table, lengths, starts, **scales)
+            o = be.paged_attention(heads(q).float(), kp, vp, table, lengths, starts, max_new=max_new,
+                                   window=self.window, sinks=self.sinks, **scales).reshape(T, D)
+            if dense:
+                x = x + be.linear(o, blk.attn.o_proj.weight, None)
+                n = be.layer_norm(x, blk.norm2.weight, blk.norm2.bias).reshape(T, D)
+                hdn = torch.nn.functional.gelu(be.linear(n, blk.ffn.w_up.weight, blk.ffn.w_up.bias), approximate="tanh")
+                x = x + be.linear(hdn, blk.ffn.w_down.weight, blk.ffn.w_down.bias)
+            else:
+                x = x + be.linear(o, blk.attn.expand_O.weight, None)
+                n = be.layer_norm(x, blk.norm2.weight, blk.norm2.bias).reshape(T, D)
+                x = x + _know(m, be, n, self._pools)[0]
+        return be.layer_norm(x, m.norm.weight, m.norm.bias)
+
+    def _embed(self, ids, pos):
+        m = self.model
+        return (m.token_emb.weight.index_select(0, ids) + m.pos_emb.weight.index_select(0, pos)).float()
+
+    def _refresh(self) -> None:
+        """What is made from the parameters, made again after a write to one: a captured step reads the copies
+        that it was captured with."""
+        key = tuple(p._version for p in self._params) + (self._params[0].data_ptr(),)
+        if key != self._key:
+            self._key, self._graph, self._out = key, None, None
+            self._pools = None if _is_dense(self.model) else _pools(self.model, self.be)
+
+    @torch.no_grad()
+    def extend(self, new: Dict[int, torch.Tensor], all_logits: bool = False):
+        """New tokens (1-D ids) of some sequences, any number each: a prompt, a chunk of one, drafted tokens.
+        Logits [len(new), V] of each one's last token, in the order of ``new``; with ``all_logits`` a list of
+        [n, V]."""
+        if not new:
+            raise ValueError("no sequence to extend")
+        dev = self._table.device
+        ids = {s: torch.as_tensor(t, dtype=torch.long, device=dev).reshape(-1) for s, t in new.items()}
+        counts = {s: t.numel() for s, t in ids.items()}
+        self._grow(counts)
+        self._refresh()
+        seqs, ns = list(ids), list(counts.values())
+        width = max(len(self.pages[s]) for s in seqs)
+        table = self._table_of(seqs, width).to(dev)
+        lengths = torch.tensor([self.lengths[s] for s in seqs], dtype=torch.int32, device=dev)
+        starts = torch.tensor([0] + ns, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+        pos = torch.cat([torch.arange(self.lengths[s] - n, self.lengths[s]) for s, n in zip(seqs, ns)]).to(dev)
+        h = self._forward(self._embed(torch.cat([ids[s] for s in seqs]), pos), table, lengths, starts, max(ns))
+        self._forget(seqs)
+        if all_logits:
+            return list(self.be.logits(h, self.model.token_emb.weight).split(ns))
+        return self.be.logits(h[starts[1:].long() - 1].contiguous(), self.model.token_emb.weight)
+
+    def _step_static(self):
+        pos = (self._len.long() - 1).clamp(min=0)              # an idle slot has no position and attends to nothing
+        h = self._forward(self._embed(self._tok, pos), self._table, self._len, None, 1)
+        return self.be.logits(h, self.model.token_emb.weight)
+
+    @torch.no_grad()
+    def step(self, tokens: Dict[int, int]) -> torch.Tensor:
+        """One new token for each of some sequences; logits [len(tokens), V] in their order.  On a GPU the
+        whole step, over all ``max_seqs`` slots, is a CUDA graph: sequences come and go between replays."""
+        if not tokens:
+            raise ValueError("no sequence to extend")
+        tokens = {s: int(t) for s, t in tokens.items()}
+        self._grow({s: 1 for s in tokens})
+        self._refresh()
+        dev = self._table.device
+        active = list(range(self.max_seqs))
+        self._table.copy_(self._table_of(active, self.width))
+        self._len.copy_(torch.tensor([self.lengths[s] if s in tokens else 0 for s in active], dtype=torch.int32))
+        self._tok.copy_(torch.tensor([tokens.get(s, 0) for s in active]))
+        if not self.use_graph:
+            out = self._step_static()
+        else:
+            if self._graph is None:
+                # outside the capture first (lazy initialisation); it writes the slots that the replay writes again
+                side = torch.cuda.Stream(device=dev)
+                side.wait_stream(torch.cuda.current_stream(dev))
+                with torch.cuda.stream(side):
+                    for _ in range(2):
+                        self._step_static()
+                torch.cuda.current_stream(dev).wait_stream(side)
+                self._graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self._graph):
+                    self._out = self._step_static()
+            self._graph.replay()
+            out = self._out
+        self._forget(tokens)
+        return out[torch.tensor(list(tokens), device=dev)]
+
+    @torch.no_grad()
+    def dense(self, seqs: Iterable[int]) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The caches of some sequences as ``prefill`` returns them: fp32 [L, n, H, max_seq, dh], zeros behind a
+        length (sequences without a window, all their pages still there)."""
+        seqs = list(seqs)
+        for s in seqs:
+            self._check(s)
+            if any(p < 0 for p in self.pages[s]):
+                raise ValueError(f"sequence {s}: pages outside the window are gone")
+        dev = self._table.device
+        table = self._table_of(seqs, self.width).to(dev)
+        lengths = torch.tensor([self.lengths[s] for s in seqs], dtype=torch.int32, device=dev)
+        got = [self.be.paged_read(kp, vp, table, lengths, self.model.max_seq_len, dtype=torch.float32, **scales)
+               for kp, vp, scales in self._layers]
+        return torch.stack([k for k, _ in got]), torch.stack([v for _, v in got])
+
+
 def sample_token(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 0.0, generator=None) -> torch.Tensor:
     if temperature <= 0:
@@ -329,18 +563,50 @@ def sample_token(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0,
     return torch.multinomial(lg.softmax(-1), 1, generator=generator).squeeze(-1)
 
 
+class _PagedBatch:
+    """A batch of prompts of one length in a ``PagedSession``, stepped as ``DecodeSession`` is."""
+
+    def __init__(self, model, input_ids, kv_dtype, window, sinks, use_graph, max_new_tokens):
+        B, S = input_ids.shape
+        if S > model.max_seq_len:
+            raise ValueError(f"Sequence length {S} exceeds max_seq_len")
+        page = 16
+        most = min(model.max_seq_len, S + max_new_tokens)
+        self.session = PagedSession(model, B, n_pages=B * -(-most // page), page_size=page, kv_dtype=kv_dtype,
+                                    window=window, sinks=sinks, use_graph=use_graph)
+        self.seqs = [self.session.open() for _ in range(B)]
+        self.first = self.session.extend(dict(zip(self.seqs, input_ids)))
+        self.use_graph = self.session.use_graph
+
+    @property
+    def length(self) -> int:
+        return self.session.lengths[0]
+
+    def step(self, tokens):
+        return self.session.step(dict(zip(self.seqs, tokens.tolist())))
+
+
 @torch.no_grad()
 def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, temperature: float = 1.0,
              top_k: int = 0, top_p: float = 0.0, stop_ids: Iterable[int] = (), generator=None,
-             use_graph: Optional[bool] = None) -> Tuple[torch.Tensor, Dict[str, float]]:
+             use_graph: Optional[bool] = None, kv_dtype: Optional[str] = None, window: Optional[int] = None,
+             sinks: int = 0) -> Tuple[torch.Tensor, Dict[str, float]]:
     """KV-cache sampling (reference sampler: scripts/analysis/standalone/
-    spatial_analysis.py:444-546).  Returns the full sequences and tokens/s."""
+    spatial_analysis.py:444-546).  Returns the full sequences and tokens/s.  With ``kv_dtype`` (bf16, e4m3,
+    int8) or ``window`` the caches are paged (``PagedSession``), otherwise dense and fp32."""
     import time
     model.eval()
-    logits, ck, cv, length = prefill(model, input_ids)
-    session = DecodeSession(model, ck, cv, length, use_graph=use_graph)
+    if kv_dtype is not None or window is not None:
+        session = _PagedBatch(model, input_ids, kv_dtype or "bf16", window, sinks, use_graph, max_new_tokens)
+        first = session.first
+    else:
+        if sinks:
+            raise ValueError("sinks belong to a window")
+        logits, ck, cv, length = prefill(model, input_ids)
+        session = DecodeSession(model, ck, cv, length, use_graph=use_graph)
+        first = logits[:, -1]
     out = [input_ids]
-    nxt = sample_token(logits[:, -1], temperature, top_k, top_p, generator)
+    nxt = sample_token(first, temperature, top_k, top_p, generator)
     stop = set(int(s) for s in stop_ids)
     sync = torch.cuda.synchronize if input_ids.is_cuda else (lambda: None)
     t0, n, t1 = time.perf_counter(), 0, None
