@@ -54,6 +54,9 @@ __device__ __forceinline__ void ldmatrix_t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16_all(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -69,7 +72,7 @@ struct Ring {
   static constexpr int kScale = 2 * kTP * kRowMost;                     // scales behind the rows
   static constexpr int kStage = kScale + (KIND == kBf16 ? 0 : 2 * kTP * 4);
   // twelve warps fit an SM with a ring of 18.9 KB each
-  static constexpr int kStages = 4 * kStage <= 18944 ? 4 : 3 * kStage <= 18944 ? 3 : 2;
+  static constexpr int kStages = 4 * kStage <= 18944 ? 4 : 3 * kStage <= 18944 ? 3 : 2 * kStage <= 18944 ? 2 : 1;
   static constexpr int kBytes = kStages * kStage;
   static_assert(kBytes <= 18944, "three blocks of four warps have to fit an SM");
 };
@@ -172,6 +175,7 @@ struct Warp {
       copy_row[c] = i < 16 * wpr ? (i * per_word) >> 16 : 99;            // i / wpr: exact for i < 256, wpr <= 16
       copy_dst[c] = copy_row[c] * row_b + ((i - copy_row[c] * wpr) << 4);
     }
+    const bool exact = wpr == KD * R::kElem;             // the head dimension is the one of the layout: 32, 64, 80 or 128
     uint32_t absent[R::kStages];                         // bit mt: the sixteen positions have no page
     auto issue = [&](int tile, int slot, int ids) {
       uint32_t gone = 0;
@@ -183,17 +187,28 @@ struct Warp {
           const int id = __shfl_sync(0xffffffffu, ids, mt), x = x0 + 16 * mt;
           gone |= static_cast<uint32_t>(id < 0) << mt;
           const size_t base = ((static_cast<size_t>(max(id, 0)) * p.w.c.H + u.h) << shift) + (x & (p.w.c.page - 1));
-          const char* ks = static_cast<const char*>(p.w.c.k) + base * dh * R::kElem;
-          const char* vs = static_cast<const char*>(p.w.c.v) + base * dh * R::kElem;
-          const bool all = id >= 0 && x + 16 <= u.hi && x >= u.lo;
+          const size_t bytes = base * static_cast<uint32_t>(dh * R::kElem) + 16 * lane;
+          const char* ks = static_cast<const char*>(p.w.c.k) + bytes;
+          const char* vs = static_cast<const char*>(p.w.c.v) + bytes;
+          const uint32_t kd = kdst + 16 * mt * row_b, vd = vdst + 16 * mt * row_b;
+          if (exact && id >= 0 && x + 16 <= u.hi && x >= u.lo) {
+            // all sixteen are seen: nothing to ask for a word, which is most of the work of a tile otherwise
 #pragma unroll
-          for (int c = 0; c < kCopies; ++c) {
-            if (copy_row[c] >= 16u) continue;
-            const uint32_t off = 16 * mt * row_b + copy_dst[c];
-            const int y = x + static_cast<int>(copy_row[c]);
-            const bool on = all || (id >= 0 && y < u.hi && (y >= u.lo || y < u.s_end));
-            copy16(kdst + off, ks + 16 * lane + 512 * c, on);
-            copy16(vdst + off, vs + 16 * lane + 512 * c, on);
+            for (int c = 0; c < kCopies; ++c) {
+              if (32 * (c + 1) <= 16 * KD * R::kElem || lane < 16 * KD * R::kElem - 32 * c) {
+                copy16_all(kd + copy_dst[c], ks + 512 * c);
+                copy16_all(vd + copy_dst[c], vs + 512 * c);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+              if (copy_row[c] >= 16u) continue;
+              const int y = x + static_cast<int>(copy_row[c]);
+              const bool on = id >= 0 && y < u.hi && (y >= u.lo || y < u.s_end);
+              copy16(kd + copy_dst[c], ks + 512 * c, on);
+              copy16(vd + copy_dst[c], vs + 512 * c, on);
+            }
           }
           if (KIND != kBf16 && lane < 8) {
             const float* src = (lane < 4 ? p.w.c.k_scale : p.w.c.v_scale) + base + 4 * (lane & 3);
@@ -204,33 +219,26 @@ struct Warp {
       copies_commit();
       return gone;
     };
-    // S - 1 tiles ahead of the one in work; page ids one tile ahead of the copies that need them
+    // as many tiles ahead as the ring holds; page ids one tile ahead of the copies that need them
     int next = t0, ids = page_ids(t0);
-#pragma unroll
-    for (int i = 0; i < R::kStages - 1; ++i) {
+    auto ahead = [&](int slot) {
       const int now = ids;
       ids = page_ids(next + step);
-      absent[i] = issue(next, i, now);
+      const uint32_t gone = issue(next, slot, now);
       next += step;
-    }
+      return gone;
+    };
+#pragma unroll
+    for (int i = 0; i < R::kStages; ++i) absent[i] = ahead(i);
     // rows of an ldmatrix: K: positions (lane & 7) + 8 (bit 3), words by bit 4; V: positions by bit 4 (bf16) or 3
     const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_word = lane >> 4;
     const int v_row = (lane & 7) + (KIND == kBf16 ? (lane >> 4) * 8 : ((lane >> 3) & 1) * 8);
     const int v_word = KIND == kBf16 ? (lane >> 3) & 1 : lane >> 4;
     int slot = 0;
     for (int tile = t0; tile < t1; tile += step) {
-      copies_wait<R::kStages - 2>();
+      copies_wait<R::kStages - 1>();
       __syncwarp();
       const uint32_t gone = absent[0];
-      {
-        const int now = ids;
-        ids = page_ids(next + step);
-        const uint32_t more = issue(next, slot == 0 ? R::kStages - 1 : slot - 1, now);
-        next += step;
-#pragma unroll
-        for (int i = 0; i + 2 < R::kStages; ++i) absent[i] = absent[i + 1];
-        absent[R::kStages - 2] = more;
-      }
       const int x0 = place(tile);
       const uint32_t kst = ring + slot * R::kStage, vst = kst + kTP * row_b;
       const uint32_t sst = kst + R::kScale;
@@ -376,6 +384,10 @@ struct Warp {
           }
         }
       }
+      __syncwarp();                                      // the whole warp has read the slot
+#pragma unroll
+      for (int i = 0; i + 1 < R::kStages; ++i) absent[i] = absent[i + 1];
+      absent[R::kStages - 1] = ahead(slot);
       slot = slot + 1 == R::kStages ? 0 : slot + 1;
     }
     copies_wait<0>();
