@@ -141,8 +141,9 @@ struct Warp {
   // Tiles t0, t0 + step, .. below t1 of the unit; ring: this warp's shared memory.
   __device__ void run(const AttnParams& p, const Unit& u, int t0, int t1, int step, int lane, uint32_t ring) {
     const int g = lane >> 2, t = lane & 3, dh = p.w.c.dh, shift = p.w.shift;
-    const int wpr = dh * R::kElem >> 4, row_b = (wpr | 1) << 4;          // 16-byte words of a row, bytes between rows
-    const int steps = dh >> 4, per_word = 65536 / wpr + 1;
+    // 16-byte words of a row in memory; rows in shared memory are those of the layout's dimension
+    const int wpr = dh * R::kElem >> 4, per_word = 65536 / wpr + 1;
+    constexpr int row_b = R::kRowMost;
     int pos_of[NT][2];                                   // positions of this lane's rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -153,11 +154,12 @@ struct Warp {
       }
     const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
     auto place = [&](int tile) { return (tile < u.st ? tile : tile + u.skip) * kTP; };
-    // lane i < kMT: the page of the tile's i-th sixteen positions, -1 where no row sees any of them
-    auto page_ids = [&](int tile) {
+    // lane l: the page of sixteen positions l % kMT of this warp's tile n + l / kMT, -1 where no row sees any of them
+    constexpr int kAhead = 32 / kMT;
+    auto page_ids = [&](int n) {
       int id = -1;
-      const int x = place(tile) + 16 * lane;
-      if (lane < kMT && tile < t1 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
+      const int tile = t0 + (n + lane / kMT) * step, x = place(tile) + 16 * (lane % kMT);
+      if (tile < t1 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
         id = __ldg(table + (x >> shift));
         if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
           atomicExch(p.w.c.status, kStatusBadPage);
@@ -177,14 +179,14 @@ struct Warp {
     }
     const bool exact = wpr == KD * R::kElem;             // the head dimension is the one of the layout: 32, 64, 80 or 128
     uint32_t absent[R::kStages];                         // bit mt: the sixteen positions have no page
-    auto issue = [&](int tile, int slot, int ids) {
+    auto issue = [&](int tile, int slot, int ids, int from) {
       uint32_t gone = 0;
       if (tile < t1) {
         const int x0 = place(tile);
         const uint32_t kdst = ring + slot * R::kStage, vdst = kdst + kTP * row_b;
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt) {
-          const int id = __shfl_sync(0xffffffffu, ids, mt), x = x0 + 16 * mt;
+          const int id = __shfl_sync(0xffffffffu, ids, from + mt), x = x0 + 16 * mt;
           gone |= static_cast<uint32_t>(id < 0) << mt;
           const size_t base = ((static_cast<size_t>(max(id, 0)) * p.w.c.H + u.h) << shift) + (x & (p.w.c.page - 1));
           const size_t bytes = base * static_cast<uint32_t>(dh * R::kElem) + 16 * lane;
@@ -219,13 +221,18 @@ struct Warp {
       copies_commit();
       return gone;
     };
-    // as many tiles ahead as the ring holds; page ids one tile ahead of the copies that need them
-    int next = t0, ids = page_ids(t0);
+    if (!exact) {                                        // the words that no copy writes are zeros
+      for (int i = lane; i < R::kBytes / 16; i += 32) st_shared_v4(ring + 16 * i, 0u, 0u, 0u, 0u);
+      __syncwarp();
+    }
+    // as many tiles ahead as the ring holds, page ids kAhead tiles and more ahead of the copies that need them
+    int n = 0, ids = page_ids(0), ids_after = page_ids(kAhead);
     auto ahead = [&](int slot) {
-      const int now = ids;
-      ids = page_ids(next + step);
-      const uint32_t gone = issue(next, slot, now);
-      next += step;
+      const uint32_t gone = issue(t0 + n * step, slot, ids, (n % kAhead) * kMT);
+      if (++n % kAhead == 0) {
+        ids = ids_after;
+        ids_after = page_ids(n + kAhead);
+      }
       return gone;
     };
 #pragma unroll
@@ -254,27 +261,23 @@ struct Warp {
         if (KIND == kBf16) {
 #pragma unroll
           for (int k = 0; k < KD; ++k) {
-            if (k < steps) {
-              uint32_t a[4];
-              ldmatrix(at + 32 * k, a);
+            uint32_t a[4];
+            ldmatrix(at + 32 * k, a);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<false>(s[nt][mt], a[0], a[1], a[2], a[3], q[nt][k][0], q[nt][k][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma16816<false>(s[nt][mt], a[0], a[1], a[2], a[3], q[nt][k][0], q[nt][k][1]);
           }
         } else {
 #pragma unroll
           for (int k = 0; k < KD; k += 2) {
-            if (k < steps) {
-              uint32_t a[4];
-              ldmatrix(at + 16 * k, a);
+            uint32_t a[4];                               // the last word of an odd number of them: a next row's beside it
+            ldmatrix(at + 16 * k, a);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (k + e < KD && k + e < steps) {
-                  const uint2 lo = codes_to_f16<KIND, false>(a[2 * e]), hi = codes_to_f16<KIND, false>(a[2 * e + 1]);
+            for (int e = 0; e < 2; ++e) {
+              if (k + e < KD) {
+                const uint2 lo = codes_to_f16<KIND, false>(a[2 * e]), hi = codes_to_f16<KIND, false>(a[2 * e + 1]);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
-                    mma16816<true>(s[nt][mt], lo.x, hi.x, lo.y, hi.y, q[nt][k + e][0], q[nt][k + e][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816<true>(s[nt][mt], lo.x, hi.x, lo.y, hi.y, q[nt][k + e][0], q[nt][k + e][1]);
               }
             }
           }
@@ -358,27 +361,23 @@ struct Warp {
         if (KIND == kBf16) {
 #pragma unroll
           for (int c = 0; c < KD; ++c) {
-            if (c < steps) {
-              uint32_t a[4];
-              ldmatrix_t(at + 32 * c, a);
+            uint32_t a[4];
+            ldmatrix_t(at + 32 * c, a);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][c], a[0], a[1], a[2], a[3], pt[nt][mt][0], pt[nt][mt][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][c], a[0], a[1], a[2], a[3], pt[nt][mt][0], pt[nt][mt][1]);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < KD; c += 2) {
-            if (c < steps) {
-              uint32_t a[4];
-              ldmatrix_t(at + 16 * c, a);
+            uint32_t a[4];
+            ldmatrix_t(at + 16 * c, a);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (c + e < KD && c + e < steps) {
-                  const uint2 lo = codes_to_f16<KIND, true>(a[2 * e]), hi = codes_to_f16<KIND, true>(a[2 * e + 1]);
+            for (int e = 0; e < 2; ++e) {
+              if (c + e < KD) {
+                const uint2 lo = codes_to_f16<KIND, true>(a[2 * e]), hi = codes_to_f16<KIND, true>(a[2 * e + 1]);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
-                    mma16816<true>(o[nt][c + e], lo.x, lo.y, hi.x, hi.y, pt[nt][mt][0], pt[nt][mt][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816<true>(o[nt][c + e], lo.x, lo.y, hi.x, hi.y, pt[nt][mt][0], pt[nt][mt][1]);
               }
             }
           }
