@@ -102,6 +102,7 @@ void paged_write(const Tensor& k, const Tensor& v, const Tensor& kp, const Tenso
   REFUSE_UNLESS(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.size(1) == kp.size(1),
                 "k and v must have one type and one shape with the pages' heads");
   DsbPaged c = view(kp, vp, ks, vs, table, lengths, starts, k.size(0), status);
+  const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(kp.device());
   const Tensor kr = rows_of(k), vr = rows_of(v);
   const int rc = dsb_paged_write(&c, kr.data_ptr(), vr.data_ptr(), kr.scalar_type() == torch::kBFloat16, kr.stride(0),
@@ -116,6 +117,7 @@ std::vector<Tensor> paged_read(const Tensor& kp, const Tensor& vp, const Tensor&
   const int64_t B = table.dim() == 2 ? table.size(0) : 0;
   DsbPaged c = view(kp, vp, ks, vs, table, lengths, none, B, status);
   REFUSE_UNLESS(B * kp.size(1) <= 0x7fffffffLL, "too many sequences");
+  const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(kp.device());
   const auto opt = kp.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat32);
   Tensor k = torch::empty({B, kp.size(1), max_len, kp.size(3)}, opt), v = torch::empty_like(k);
@@ -138,6 +140,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& kp, const Tensor& vp, cons
   REFUSE_UNLESS(sinks >= 0, "sinks must not be negative");
   REFUSE_UNLESS(!max_new.has_value() || *max_new >= 0, "max_new must not be negative");
   DsbPaged c = view(kp, vp, ks, vs, table, lengths, starts, q.size(0), status);
+  const at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(kp.device());
   const Tensor qr = rows_of(q.scalar_type() == torch::kBFloat16 ? q : q.to(torch::kBFloat16));
   Tensor out = torch::empty({q.size(0), Hq, q.size(2)}, kp.options().dtype(torch::kBFloat16));

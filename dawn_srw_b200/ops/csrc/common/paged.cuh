@@ -58,15 +58,16 @@ __device__ __forceinline__ int seq_length(const View& w, int b) {
   return max(len, 0);
 }
 
-// The sequence that packed row t belongs to, or -1 (rows before the first or behind the last one).
-__device__ __forceinline__ int seq_of_row(const View& w, int t) {
+// The sequence that packed row t belongs to, or -1 (rows before the first or behind the last one); by a whole warp.
+__device__ __forceinline__ int seq_of_row_warp(const View& w, int t, int lane) {
   if (w.c.starts == nullptr) return t;
-  int lo = 0, hi = w.c.B;                          // the last b with starts[b] <= t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (w.c.starts[mid + 1] <= t) lo = mid + 1; else hi = mid;
+  int b = 0;                                       // how many sequences end at or before t
+  for (int i = 0; i < w.c.B; i += 32) {
+    const unsigned past = __ballot_sync(0xffffffffu, i + lane < w.c.B && w.c.starts[i + lane + 1] <= t);
+    b += __popc(past);
+    if (past != 0xffffffffu) break;
   }
-  return lo < w.c.B && w.c.starts[lo] <= t ? lo : -1;
+  return b < w.c.B && w.c.starts[b] <= t ? b : -1;
 }
 
 // Page of position `pos` of sequence b, or -1 where the table names none of the pool.

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -445,11 +447,31 @@ inline long long workspace_bytes(long long workers, int rows, int dh) {
   return workers * static_cast<long long>(sizeof(int4)) + 2 * workers * rows * (dh + 2) * static_cast<long long>(sizeof(float));
 }
 
+// What a launcher asks of a device once, not in every call.
+constexpr int kDevices = 64;
+inline int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kDevices ? dev : 0;
+}
 inline int device_sms() {
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  static std::atomic<int> sms[kDevices];
+  const int dev = current_device();
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    n = n > 0 ? n : 148;
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+// Lets a kernel have up to `bytes` of dynamic shared memory; `most` is the kernel's own memory of what it may have.
+template <typename F>
+int allow_smem(F* kernel, int bytes, std::atomic<int> (&most)[kDevices]) {
+  const int dev = current_device();
+  if (most[dev].load(std::memory_order_relaxed) >= bytes) return 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 944;
+  most[dev].store(bytes, std::memory_order_relaxed);
+  return 0;
 }
 
 }  // namespace paged

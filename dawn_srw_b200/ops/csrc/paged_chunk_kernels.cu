@@ -962,9 +962,8 @@ int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
 
 template <int KIND, int NA>
 int launch(const ChunkParams& p, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(paged_chunk_kernel<KIND, NA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA>::kTotal) !=
-      cudaSuccess)
-    return 950;
+  static std::atomic<int> most[kDevices];
+  if (allow_smem(paged_chunk_kernel<KIND, NA>, Smem<NA>::kTotal, most)) return 950;
   return launch_early(paged_chunk_kernel<KIND, NA>, dim3(p.a.workers), kThreadsOf<KIND>, Smem<NA>::kTotal, p, stream) ? 951 : 0;
 }
 

@@ -579,17 +579,13 @@ Sharing sharing(const DsbPaged* c, int window, int sinks, int max_new, long long
   return s;
 }
 
-template <typename F>
-int with_smem(F* kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess ? 0 : 944;
-}
-
 template <int KIND, int KD, int NT>
 int launch(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
   using W = Warp<KIND, KD, NT>;
   if (how.blocks > 0) {
     const int bytes = how.warps * W::R::kBytes;
-    if (with_smem(paged_few_unit_kernel<KIND, KD, NT>, bytes)) return 944;
+    static std::atomic<int> most[kDevices];
+    if (allow_smem(paged_few_unit_kernel<KIND, KD, NT>, kMostWarps * W::R::kBytes, most)) return 944;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(max_rt * how.blocks, p.w.c.H, p.w.c.B);
     cfg.blockDim = dim3(32 * how.warps);
@@ -607,7 +603,8 @@ int launch(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, paged_few_unit_kernel<KIND, KD, NT>, p, how.blocks) == cudaSuccess ? 0 : 945;
   }
   constexpr int bytes = kWarps * W::R::kBytes;
-  if (with_smem(paged_few_run_kernel<KIND, KD, NT>, bytes)) return 944;
+  static std::atomic<int> most[kDevices];
+  if (allow_smem(paged_few_run_kernel<KIND, KD, NT>, bytes, most)) return 944;
   if (launch_early(paged_few_run_kernel<KIND, KD, NT>, dim3(p.workers / kWarps), 32 * kWarps, bytes, p, stream)) return 945;
   return launch_early(paged_merge_few_kernel<W::kRows>, dim3(p.workers), kMergeThreads, 0, p, stream);
 }

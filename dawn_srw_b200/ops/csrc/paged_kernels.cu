@@ -93,23 +93,29 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const View w, con
   const long long rows = static_cast<long long>(w.c.N) * w.c.H;
   int t = -1, h = 0, page = -1, pos = -1;
   if (g < rows) {
-    t = static_cast<int>(g / w.c.H);
+    t = static_cast<int>(rows >> 31 == 0 ? static_cast<uint32_t>(g) / static_cast<uint32_t>(w.c.H) : g / w.c.H);
     h = static_cast<int>(g - static_cast<long long>(t) * w.c.H);
-    const int b = seq_of_row(w, t);
-    if (b >= 0) {
-      const Rows r = seq_rows(w, b);
-      const int len = seq_length(w, b);
-      pos = len - r.count + (t - r.first);
-      if (pos >= 0 && pos < len) page = page_of(w, b, pos);
-    }
   }
-  const bool on = page >= 0 && col < w.c.dh;
+  // the rows are on their way while their places are looked up, in three loads that depend on one another
   Eight ek, ev;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ek.f[i] = ev.f[i] = 0.f;
-  if (on) {
+  if (t >= 0 && col < w.c.dh) {
     ek = load_src<SRC_BF16>(k, static_cast<size_t>(t) * k_st + static_cast<size_t>(h) * k_sh + col);
     ev = load_src<SRC_BF16>(v, static_cast<size_t>(t) * v_st + static_cast<size_t>(h) * v_sh + col);
+  }
+  int b = -1;
+  for (unsigned todo = __ballot_sync(0xffffffffu, t >= 0); todo != 0u;) {      // a token, or two, of a warp's rows
+    const int one = __shfl_sync(0xffffffffu, t, __ffs(todo) - 1);
+    const int x = seq_of_row_warp(w, one, threadIdx.x & 31);
+    if (t == one) b = x;
+    todo &= ~__ballot_sync(0xffffffffu, t == one);
+  }
+  if (b >= 0) {
+    const Rows r = seq_rows(w, b);
+    const int len = seq_length(w, b);
+    pos = len - r.count + (t - r.first);
+    if (pos >= 0 && pos < len) page = page_of(w, b, pos);
   }
   // every lane takes part in the shuffles; a group without a page stores nothing
   const size_t row = page >= 0 ? slot_row(w, page, h, pos) : 0;

@@ -115,7 +115,10 @@ def check_status_deferred() -> None:
 
 def _paged_status(pages):
     """Status word for the pages' device; of CPU pages a stand-in (the binding refuses them after all else)."""
-    return status_word(pages.device) if pages.is_cuda else torch.zeros(1, dtype=torch.int32)
+    word = _STATUS.get(pages.get_device())
+    if word is None:
+        word = status_word(pages.device) if pages.is_cuda else torch.zeros(1, dtype=torch.int32)
+    return word
 
 
 def _gate_list(spec: GateSpec) -> List[float]:
@@ -981,8 +984,7 @@ class CudaBackend:
         count_launches(2)
         return ext().prompt_attention(f(q), f(k), f(v), cache_k, cache_v, B, S, status_word(q.device))
 
-    # ---- paged key/value cache (layouts, types and bounds: ops/paged.py) ----
-    @torch.no_grad()
+    # ---- paged key/value cache (layouts, types and bounds: ops/paged.py; no gradients) ----
     def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
         """Keys and values [N, H, dh] (fp32 or bf16) of new tokens into their pages, rounded to the pages'
         type.  One launch; rows of no sequence, and positions whose table entry names no page, are left
@@ -990,7 +992,6 @@ class CudaBackend:
         count_launches(1)
         ext().paged_write(k, v, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, _paged_status(k_pages))
 
-    @torch.no_grad()
     def paged_read(self, k_pages, v_pages, table, lengths, max_len: int, k_scale=None, v_scale=None,
                    dtype=torch.float32):
         """Pages back to dense k, v [B, H, max_len, dh], zeros at and behind a sequence's length."""
@@ -1000,7 +1001,6 @@ class CudaBackend:
         return tuple(ext().paged_read(k_pages, v_pages, table, lengths, int(max_len), k_scale, v_scale,
                                       dtype == torch.bfloat16, _paged_status(k_pages)))
 
-    @torch.no_grad()
     def paged_attention(self, q, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None, *,
                         max_new: Optional[int] = None, window: Optional[int] = None, sinks: int = 0,
                         scale: Optional[float] = None):
