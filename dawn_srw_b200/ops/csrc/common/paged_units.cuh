@@ -115,10 +115,11 @@ __device__ __forceinline__ void unit_range(const AttnParams& p, Unit& u) {
 
 __device__ __forceinline__ void unit_sequence(const AttnParams& p, Unit& u, int b) {
   u.b = b;
+  const int len = seq_length(p.w, b);              // all loads at once
   const Rows r = seq_rows(p.w, b);
   u.first = r.first;
   u.n = r.count;
-  u.len = u.n > 0 ? seq_length(p.w, b) : 0;
+  u.len = u.n > 0 ? len : 0;
 }
 
 // Tiles of the units of one head of sequence i + lane: a lane's own arithmetic for a sequence of one row tile, the

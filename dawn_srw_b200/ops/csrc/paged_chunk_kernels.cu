@@ -53,6 +53,8 @@ struct Smem {
 
 struct ChunkParams {
   CUtensorMap k, v;                          // bf16 pages: [n_pages * H][page][dh]
+  CUtensorMap q;                             // queries: [N][Hq][dh], boxes of 128 rows (tokens x a group)
+  int q_tma;                                 // a group divides 128 rows: the queries come by TMA
   AttnParams a;
 };
 
@@ -262,7 +264,8 @@ __device__ __forceinline__ bool elect_one() {
 
 template <int S>
 struct Bars {
-  uint64_t q_full[2];       // queries of tile i are in shared memory (4 warps)
+  uint64_t q_full[2];       // queries of tile i are in shared memory (4 warps, or a TMA load)
+  uint64_t q_raw[2];        // they are, and are to be converted
   uint64_t k_full[S];       // K, and the tile's scales and absences
   uint64_t k_empty[S];      // both tiles' S of the stage are done
   uint64_t v_full[S];
@@ -315,10 +318,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   volatile uint32_t* absent = b.absent;
   const AttnParams& p = cp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.w.c.dh, ksteps = dh >> 4;
+  // a scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which would
+  // turn the -inf of hidden scores into NaN, into queries of zero
+  const bool as_is = !kF16 && p.scale_log2 > 0.f;      // queries as they are in memory
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b.q_full[i], 4);
+      mbar_init(&b.q_full[i], as_is && cp.q_tma ? 1 : 4);
+      mbar_init(&b.q_raw[i], 1);
       mbar_init(&b.s_full[i], 1);
       mbar_init(&b.s_free[i], 4);
       mbar_init(&b.p_half[i], 4);
@@ -663,12 +670,19 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
     const uint32_t q_tile = q_addr + i * NA * kAtom;
     const int first_row = 32 * (warp & 3), words = 2 * ksteps;  // of this warp; 16-byte words of a row
-    // a scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which
-    // would turn the -inf of hidden scores into NaN, into queries of zero
     const bool flat = p.scale_log2 == 0.f;
     // queries of the next segment on their way into the swizzled tile: a warp its 32 rows, neighbouring lanes the words
     // of a row
     auto fetch_q = [&]() {
+      if (cp.q_tma) {
+        if (row == 0) {
+          uint64_t* bar = as_is ? &b.q_full[i] : &b.q_raw[i];
+          mbar_expect_tx(bar, NA * kAtom);
+          const int t = u.first + p.by_g(u.rt * kUnitRows + i * kTileRows);
+          for (int a = 0; a < NA; ++a) tma_load_3d(q_tile + a * kAtom, &cp.q, bar, 64 * a, u.h * p.G, t);
+        }
+        return;
+      }
       constexpr int kRowLanes = 8 * NA, kRowStep = 32 / kRowLanes;
       const int word = lane % kRowLanes, sub_row = lane / kRowLanes;
       if (word < words) {
@@ -683,7 +697,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
       }
     };
-    uint32_t nk = 0, ns = 0;                       // tiles loaded, S of this tile so far
+    uint32_t nk = 0, ns = 0, nq = 0;               // tiles loaded, S of this tile, its segments with work so far
     bool ok = true, have = plans.next(u, lane);
     if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
     while (ok && have) {
@@ -695,11 +709,16 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       const int w0 = u.rt * kUnitRows + i * kTileRows + first_row;             // positions of this warp's rows
       const int pos_lo = u.len - u.n + p.by_g(min(w0, u.n * p.G - 1)), pos_hi = u.len - u.n + p.by_g(min(w0 + 31, u.n * p.G - 1));
       float f = flat ? 1.f : fabsf(p.scale_log2);
-      if (mine > 0) {
-        copies_wait_all();
+      if (mine > 0 && !(as_is && cp.q_tma)) {
+        if (cp.q_tma) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&b.q_raw[i], nq & 1, abort_flag));
+          if (!ok) break;
+        } else {
+          copies_wait_all();
+        }
         __syncwarp();
         const bool flip = p.scale_log2 < 0.f;
-        if (kF16 || flip) {
+        if (!as_is) {
           uint4 v[8 * NA];
           uint32_t top = 0;
 #pragma unroll
@@ -709,7 +728,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
           }
-          float up = flip ? -1.f : 1.f;
+          float up = flat ? 0.f : flip ? -1.f : 1.f;
           const uint32_t e = top >> 7;             // fp16 queries, scaled by a power of two (see the few-row kernel)
           if (kF16 && e >= 16u && e != 255u) {
             up *= __uint_as_float((261u - e) << 23);
@@ -724,7 +743,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
               st_shared_v4(swz(q_tile, row, c), pack_f16x2(t[0] * up, t[1] * up), pack_f16x2(t[2] * up, t[3] * up),
                            pack_f16x2(t[4] * up, t[5] * up), pack_f16x2(t[6] * up, t[7] * up));
             } else {
-              st_shared_v4(swz(q_tile, row, c), v[c].x ^ 0x80008000u, v[c].y ^ 0x80008000u, v[c].z ^ 0x80008000u, v[c].w ^ 0x80008000u);
+              const uint32_t sign = flip ? 0x80008000u : 0u, keep = flat ? 0u : 0xffffffffu;
+              st_shared_v4(swz(q_tile, row, c), (v[c].x ^ sign) & keep, (v[c].y ^ sign) & keep, (v[c].z ^ sign) & keep, (v[c].w ^ sign) & keep);
             }
           }
         }
@@ -732,6 +752,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.q_full[i]);
       }
+      if (mine > 0) ++nq;
       float m = kFloor, l = 0.f;
       for (int j = 0; j < mine; ++j, ++ns) {
         const uint32_t st = (nk + j) % kMeta<NA>;
@@ -960,6 +981,19 @@ int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
 }
 
+// Queries as [N][Hq][dh], boxes of 64 columns, a group of heads and as many tokens as 128 rows hold.
+int query_map(CUtensorMap* map, const AttnParams& a) {
+  auto enc = tensor_map_encoder();
+  if (enc == nullptr) return 1;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.w.c.dh), static_cast<cuuint64_t>(a.Hq), static_cast<cuuint64_t>(a.w.c.N)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q_sh) * 2, static_cast<cuuint64_t>(a.q_st) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.G), static_cast<cuuint32_t>(kTileRows / a.G)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(a.q), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
+}
+
 template <int KIND, int NA>
 int launch(const ChunkParams& p, cudaStream_t stream) {
   static std::atomic<int> most[kDevices];
@@ -982,6 +1016,10 @@ int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
   a.meta = static_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(a.meta + a.workers);
   p.a = a;
+  // strides that a tensor map takes (positive, below 2^40), a group that divides the rows of a tile: copies row by row
+  // otherwise
+  p.q_tma = a.G <= kTileRows && kTileRows % a.G == 0 && a.q_sh > 0 && a.q_st > 0 && a.q_sh < (1LL << 38) && a.q_st < (1LL << 38) &&
+            query_map(&p.q, a) == 0;
   int rc;
   if (a.w.c.kind == kBf16) {
     if (page_map(&p.k, a.w.c.k, a.w.c) || page_map(&p.v, a.w.c.v, a.w.c)) return 952;
