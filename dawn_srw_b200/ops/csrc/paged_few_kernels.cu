@@ -559,10 +559,14 @@ int few_workers() { return device_sms() * kBlocksPerSm * kWarps; }
 struct Sharing { int blocks, warps; };
 
 // The warps that the GPU holds (twelve an SM) are dealt to the units; a unit gets as many as its tiles at most.  What a
-// sequence really has is not known here, only what its table holds and a window leaves of it.  Above kLong positions
-// for a warp the differences between sequences cost more than the plan, the pieces and the merge of equal runs.
+// sequence really has is not known here, only what its table holds and a window leaves of it.  Above `longest`
+// positions for a warp the differences between sequences, and between SMs, cost more than the plan, the pieces and the
+// merge of equal runs.  Microseconds, clusters / equal runs:
+//   96 units, 18 warps each (bf16, 80):    4096 positions 34 / 33, 8192 58 / 54, 32768 229 / 179
+//   512 units, 3 warps (e4m3, 128):        512 positions 20 / 24, 1024 37 / 37, 2048 63 / 60, 8192 226 / 194
+//   512 units, lengths 16 times apart:     512 positions 14 / 23, 2048 35 / 28, 8192 98 / 75
+//   32 units, 48 warps (bf16, 128, G 4):   4096 positions 14 / 24, 16384 49 / 68, 32768 93 / 111
 Sharing sharing(const DsbPaged* c, int window, int sinks, int max_new, long long units) {
-  constexpr int kLong = 1024;
   long long most = static_cast<long long>(c->width) * c->page;
   if (window > 0 && static_cast<long long>(window) + sinks + max_new < most) most = static_cast<long long>(window) + sinks + max_new;
   long long w = static_cast<long long>(kMostWarps) * device_sms() / (units > 0 ? units : 1);
@@ -575,7 +579,8 @@ Sharing sharing(const DsbPaged* c, int window, int sinks, int max_new, long long
     s.warps = w / 6 <= 8 ? 6 : kMostWarps;
     s.blocks = static_cast<int>(w / s.warps);
   }
-  if (most > static_cast<long long>(kLong) * s.blocks * s.warps) s.blocks = 0;
+  const long long longest = s.blocks * s.warps > 36 ? 1024 : 448;
+  if (most > longest * s.blocks * s.warps) s.blocks = 0;
   return s;
 }
 
