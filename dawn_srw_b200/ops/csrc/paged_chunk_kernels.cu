@@ -25,14 +25,18 @@ namespace dsb {
 namespace paged {
 namespace {
 
-constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows, kTP = 128;
-constexpr int kAtom = kTP * 128;            // 128 rows x 64 16-bit columns
-template <int NA> constexpr int kStages = NA == 1 ? 4 : 2;      // tiles of K, and of V, in shared memory
+constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows;
+constexpr int kAtom = kTileRows * 128;      // 128 rows x 64 16-bit columns
+// Positions of a tile.  TMEM holds two O, two S and, for heads of up to 64, two P, so that the next S can be made while P
+// is.  For wider heads P takes the place of S, and the next S has to have another place: two S of 64 positions per
+// query tile (ragged prompts of 16 heads of 128: ? us for 97 with one of 128 and the wait for P that it takes).
+template <int NA> constexpr int kTP = NA == 1 ? 128 : 64;
+constexpr int kStages = 4;                  // tiles of K, and of V, in shared memory
 // Slots of scales and absences: written with K, read by a softmax that may be a tile behind the last use of the stage.
-template <int NA> constexpr int kMeta = 2 * kStages<NA>;
+constexpr int kMeta = 2 * kStages;
 constexpr int kPlans = 4;                   // segments that the planning warp is ahead of the others at most
 constexpr float kSlack = 8.f;               // how far (in powers of two) a maximum may grow before O is rescaled
-constexpr int kLeast = 2;                   // tiles of a run
+constexpr int kLeast = 2;                   // tiles of 128 positions of a run
 
 // Warpgroups 0 and 1: softmax of tiles 0 and 1.  Warps 8 and 9: their MMA.  Warps 10 and 11: TMA, the plan.
 // Warpgroup 3, 8-bit kinds: loaders.
@@ -42,10 +46,11 @@ constexpr int kThreadsOf = KIND == kBf16 ? 384 : 512;
 template <int NA>                            // 64-column atoms of a head
 struct Smem {
   static constexpr int kQ = 0;                                   // [2 tiles][NA atoms]
-  static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages][NA]
-  static constexpr int kV = kK + kStages<NA> * NA * kAtom;       // [kStages][NA]
-  static constexpr int kExp = kV + kStages<NA> * NA * kAtom;     // [kMeta][2][4] 2^e of the keys, e of the values
-  static constexpr int kPlan = kExp + kMeta<NA> * 32;            // [kPlans] segments ahead
+  static constexpr int kTile = NA * kTP<NA> * 128;               // K, or V, of a tile: NA atoms of kTP rows
+  static constexpr int kK = kQ + 2 * NA * kAtom;                 // [kStages]
+  static constexpr int kV = kK + kStages * kTile;                // [kStages]
+  static constexpr int kExp = kV + kStages * kTile;              // [kMeta][2][4] 2^e of the keys, e of the values
+  static constexpr int kPlan = kExp + kMeta * 32;            // [kPlans] segments ahead
   static constexpr int kBar = kPlan + kPlans * 128;
   static constexpr int kTotal = kBar + 512 + 1024;
   static_assert(kTotal <= 227 * 1024, "shared memory of an SM");
@@ -174,19 +179,21 @@ __host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(b_mn_major) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int kk) { return umma_desc(tile + (kk >> 2) * kAtom + (kk & 3) * 32, 16, 1024); }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int kk) { return umma_desc(tile + kk * 2048, kAtom, 1024); }
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile) { return umma_desc(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int atom) { return umma_desc(tile, atom, 1024); }
 // 16-byte word c8 (eight columns) of a row of a tile made of swizzled atoms.
+template <int ATOM = kAtom>
 __device__ __forceinline__ uint32_t swz(uint32_t tile, int row, int c8) {
-  return tile + (c8 >> 3) * kAtom + row * 128 + (((c8 & 7) ^ (row & 7)) << 4);
+  return tile + (c8 >> 3) * ATOM + row * 128 + (((c8 & 7) ^ (row & 7)) << 4);
 }
 
 // How many of a unit's tiles of positions query tile i works on (its rows see none of the later ones).
+template <int TP>
 __device__ __forceinline__ int tiles_of(const AttnParams& p, const Unit& u, int i) {
   const int r0 = i * kTileRows, r1 = min(u.rows, r0 + kTileRows);
   if (r0 >= u.rows) return 0;
   const int last = u.len - u.n + p.by_g(u.rt * kUnitRows + r1 - 1);
-  const int end = (max(last + 1, 0) + kTP - 1) / kTP;       // tiles of positions that begin at or before `last`
+  const int end = (max(last + 1, 0) + TP - 1) / TP;       // tiles of positions that begin at or before `last`
   return min(u.tiles, end <= u.st ? end : max(end - u.skip, u.st));
 }
 
@@ -201,7 +208,8 @@ struct Plan {
 };
 static_assert(sizeof(Plan) <= 128, "slot of a plan");
 
-__device__ __forceinline__ int place(const Plan& q, int j) { return (q.t0 + j < q.st ? q.t0 + j : q.t0 + j + q.skip) * kTP; }
+template <int TP>
+__device__ __forceinline__ int place(const Plan& q, int j) { return (q.t0 + j < q.st ? q.t0 + j : q.t0 + j + q.skip) * TP; }
 
 // Bit k: a row at position pos sees position x + k.
 __device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks) {
@@ -210,13 +218,13 @@ __device__ __forceinline__ uint32_t seen32(int x, int pos, int window, int sinks
   return by & ~old;
 }
 
-// D = A B^T over KS steps of sixteen columns, both K-major.
-template <int KS>
+// D = A B^T over KS steps of sixteen columns, both K-major; B's atoms are B_ATOM bytes apart.
+template <int KS, int B_ATOM>
 __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
   for (int kk = 0; kk < KS; ++kk) {
-    const uint32_t off = ((kk >> 2) * kAtom + (kk & 3) * 32) >> 4;
-    mma_bf16_ss(d, a + off, b + off, idesc, kk > 0 ? 1u : 0u);
+    mma_bf16_ss(d, a + (((kk >> 2) * kAtom + (kk & 3) * 32) >> 4), b + (((kk >> 2) * B_ATOM + (kk & 3) * 32) >> 4), idesc,
+                kk > 0 ? 1u : 0u);
   }
 }
 
@@ -271,9 +279,9 @@ struct Bars {
   uint64_t v_full[S];
   uint64_t v_empty[S];      // both tiles' O of the stage are done
   uint64_t v_fix;           // V has landed, rows behind the end still have to be cleared
-  uint64_t s_full[2];
+  uint64_t s_full[2][2];    // [query tile][place of S]
   uint64_t s_free[2];       // S has been read (4 warps); only where P has columns of its own
-  uint64_t p_half[2];       // the first 64 positions of P are in TMEM (4 warps)
+  uint64_t p_half[2];       // the first half of P is in TMEM (4 warps)
   uint64_t p_full[2];       // all of them
   uint64_t o_done[2];
   uint64_t plan_full[kPlans];
@@ -309,10 +317,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   constexpr bool kF16 = KIND != kBf16;
   constexpr bool kAhead = kF16;                 // columns of S loaded one step ahead (183 us for 194; bf16 103 for 101)
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
+  constexpr bool kKeep = kAlias && !kF16;       // a row of S stays in registers (a loaders' kernel has too few of them)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  constexpr int S = kStages<NA>;
-  static_assert(sizeof(Bars<S>) <= 512 && kMeta<NA> == 2 * S, "barriers");
+  constexpr int S = kStages, TP = kTP<NA>, kHalf = TP / 2, kTile = L::kTile, kKvAtom = TP * 128;
+  static_assert(sizeof(Bars<S>) <= 512 && kMeta == 2 * S, "barriers");
   Bars<S>& b = *reinterpret_cast<Bars<S>*>(smem + L::kBar);
   volatile int* abort_flag = &b.abort;
   volatile uint32_t* absent = b.absent;
@@ -326,7 +335,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b.q_full[i], as_is && cp.q_tma ? 1 : 4);
       mbar_init(&b.q_raw[i], 1);
-      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.s_full[i][0], 1);
+      mbar_init(&b.s_full[i][1], 1);
       mbar_init(&b.s_free[i], 4);
       mbar_init(&b.p_half[i], 4);
       mbar_init(&b.p_full[i], 4);
@@ -338,6 +348,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.v_full[i], kF16 ? 4 : 1);
       mbar_init(&b.v_empty[i], 2);
     }
+    for (int i = 0; i < kMeta; ++i) b.absent[i] = 0;
     mbar_init(&b.v_fix, 1);
     for (int i = 0; i < kPlans; ++i) {
       mbar_init(&b.plan_full[i], 1);
@@ -377,28 +388,28 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         // One lane does all of it, and no instruction stands under a condition of its own: a tcgen05.mma that became a
         // predicated one gave wrong results.  What does not change from tile to tile is made beforehand.
         const int I = warp - 8;
-        const uint32_t idesc_s = idesc16(!kF16, kTileRows, kTP, 0), idesc_o = idesc16(!kF16, kTileRows, dh, 1);
-        constexpr uint32_t kStage16 = NA * kAtom >> 4;        // a stage, or a query tile, in a descriptor's units
-        const uint64_t q_desc = desc_k(q_addr, 0) + I * kStage16, k_desc = desc_k(k_addr, 0), v_desc = desc_mn(v_addr, 0);
+        const uint32_t idesc_s = idesc16(!kF16, kTileRows, TP, 0), idesc_o = idesc16(!kF16, kTileRows, dh, 1);
+        const uint64_t q_desc = desc_k(q_addr + I * NA * kAtom), k_desc = desc_k(k_addr), v_desc = desc_mn(v_addr, kKvAtom);
         const uint32_t s_at = s_col(I), o_at = o_col(I), p_at = p_col(I);
         // uses of the stages, segments with work and tiles so far.  Whoever waits for a phase of a barrier has seen the
         // phase before it, or something later, so that no wait is two phases off.
         uint32_t nk = 0, nq = 0, nt = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && wait_hot(bar, phase & 1, abort_flag); };
-        auto issue_s = [&](int j) {
-          const uint32_t st = (nk + j) % S;
+        // S of the segment's j-th tile, the x-th of this query tile
+        auto issue_s = [&](int j, uint32_t x) {
+          const uint32_t st = (nk + j) % S, place = kAlias ? x & 1u : 0u;
           wait(&b.k_full[st], (nk + j) / S);
           if (!ok) return;
           tc_fence_after();
-          const uint64_t ka = k_desc + st * kStage16;
+          const uint64_t ka = k_desc + st * (kTile >> 4);
           switch (ksteps - 4 * (NA - 1)) {
-            case 1: issue_qk<4 * NA - 3>(s_at, q_desc, ka, idesc_s); break;
-            case 2: issue_qk<4 * NA - 2>(s_at, q_desc, ka, idesc_s); break;
-            case 3: issue_qk<4 * NA - 1>(s_at, q_desc, ka, idesc_s); break;
-            default: issue_qk<4 * NA>(s_at, q_desc, ka, idesc_s);
+            case 1: issue_qk<4 * NA - 3, kKvAtom>(s_at + place * TP, q_desc, ka, idesc_s); break;
+            case 2: issue_qk<4 * NA - 2, kKvAtom>(s_at + place * TP, q_desc, ka, idesc_s); break;
+            case 3: issue_qk<4 * NA - 1, kKvAtom>(s_at + place * TP, q_desc, ka, idesc_s); break;
+            default: issue_qk<4 * NA, kKvAtom>(s_at + place * TP, q_desc, ka, idesc_s);
           }
-          mma_commit(&b.s_full[I]);
+          mma_commit(&b.s_full[I][place]);
           mma_commit(&b.k_empty[st]);
         };
         for (uint32_t k = 0; ok; ++k) {
@@ -411,32 +422,35 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           const int n = max(n0, n1), mine = I == 0 ? n0 : n1;
           if (mine > 0) {
             wait(&b.q_full[I], nq++);
-            if (ok) issue_s(0);
+            if (ok) issue_s(0, nt);
+            if (kAlias && mine > 1 && ok) issue_s(1, nt + 1);
           }
           for (int j = 0; j < mine && ok; ++j, ++nt) {
             const uint32_t st = (nk + j) % S;
             if (!kAlias && j + 1 < mine) {         // the next S while the weights of this one are still being made
               wait(&b.s_free[I], nt);
-              if (ok) issue_s(j + 1);
+              if (ok) issue_s(j + 1, nt + 1);
             }
             wait(&b.v_full[st], (nk + j) / S);
-            wait(&b.p_half[I], nt);
+            if (!kAlias) wait(&b.p_half[I], nt);
+            if (kAlias) wait(&b.p_full[I], nt);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t va = v_desc + st * kStage16;
-            mma_ts(o_at, p_at, va, idesc_o, j > 0);
+            const uint64_t va = v_desc + st * (kTile >> 4);
+            const uint32_t pa = p_at + (kAlias ? (nt & 1u) * TP : 0u);
+            mma_ts(o_at, pa, va, idesc_o, j > 0);
 #pragma unroll
-            for (int kk = 1; kk < kTP / 32; ++kk) mma_ts(o_at, p_at + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
-            wait(&b.p_full[I], nt);
+            for (int kk = 1; kk < kHalf / 16; ++kk) mma_ts(o_at, pa + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
+            if (!kAlias) wait(&b.p_full[I], nt);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int kk = kTP / 32; kk < kTP / 16; ++kk) mma_ts(o_at, p_at + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
+            for (int kk = kHalf / 16; kk < TP / 16; ++kk) mma_ts(o_at, pa + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
             mma_commit(&b.o_done[I]);
             mma_commit(&b.v_empty[st]);
-            if (kAlias && j + 1 < mine) {          // the next S takes the columns that this P is being read from
+            if (kAlias) {                          // the S after the next takes the columns that this P is read from
               wait(&b.o_done[I], nt);
-              if (ok) issue_s(j + 1);
+              if (j + 2 < mine && ok) issue_s(j + 2, nt + 2);
             }
           }
           for (int j = mine; j < n && ok; ++j) {   // the other tile's alone
@@ -453,33 +467,33 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       // ------------------------------------------------------------ TMA loads of bf16 pages
       uint32_t nk = 0, fixes = 0;
       bool ok = true;
-      const int shift = p.w.shift, box = min(p.w.c.page, kTP);
+      const int shift = p.w.shift, box = min(p.w.c.page, TP);
       while (ok && plans.next(u, lane)) {
         const int n = max(u.n0, u.n1);
         const int* table = p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width;
         for (int j = 0; j < n && ok; ++j, ++nk) {
           const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1;
-          const int x0 = place(u, j);
-          // lane i < 8: the page of sixteen positions i, -1 where no row sees any of them
+          const int x0 = place<TP>(u, j);
+          // lane i < TP / 16: the page of sixteen positions i, -1 where no row sees any of them
           int id = -1;
           const int x = x0 + 16 * lane;
-          if (lane < 8 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
+          if (lane < TP / 16 && x < u.hi && (x + 16 > u.lo || x < u.s_end)) {
             id = __ldg(table + (x >> shift));
             if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.w.c.n_pages)) {
               atomicExch(p.w.c.status, kStatusBadPage);
               id = -1;
             }
           }
-          const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & 0xffu;
+          const uint32_t gone = __ballot_sync(0xffffffffu, id < 0) & ((1u << TP / 16) - 1u);
           auto unseen = [&](int y) { return y >= u.hi || (y < u.lo && y >= u.s_end); };
           // rows of V to clear
-          const bool cut = gone != 0u || x0 + kTP > u.hi || (x0 < u.lo && min(x0 + kTP, u.lo) > u.s_end);
+          const bool cut = gone != 0u || x0 + TP > u.hi || (x0 < u.lo && min(x0 + TP, u.lo) > u.s_end);
           // lanes that start a box: the first sixteen of each that the tile has
           const int per = box >> 4;
-          const bool mine = lane < 8 && lane % per == 0;
+          const bool mine = lane < TP / 16 && lane % per == 0;
           // a box is fetched if its page is there at all: its sixteens are of one page
           const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
-          const uint32_t group = lane < 8 ? (have >> (lane / per * per)) & ((1u << per) - 1u) : 0u;
+          const uint32_t group = lane < TP / 16 ? (have >> (lane / per * per)) & ((1u << per) - 1u) : 0u;
           const int src_lane = group ? lane / per * per + __ffs(group) - 1 : 0;
           const int page = __shfl_sync(0xffffffffu, id, src_lane);
           const bool fetch = mine && group != 0u;
@@ -488,13 +502,13 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
           if (!ok) break;
           if (lane == 0) {
-            absent[nk % kMeta<NA>] = (gone & 3u) | (gone & 12u) << 6 | (gone & 48u) << 12 | (gone & 192u) << 18;
+            absent[nk % kMeta] = (gone & 3u) | (gone & 12u) << 6 | (gone & 48u) << 12 | (gone & 192u) << 18;
             mbar_expect_tx(&b.k_full[st], boxes * NA * box * 128);
           }
           __syncwarp();
           if (fetch)
             for (int a = 0; a < NA; ++a)
-              tma_load_3d(k_addr + (st * NA + a) * kAtom + lane * 2048, &cp.k, &b.k_full[st], 64 * a, c1, c2);
+              tma_load_3d(k_addr + st * kTile + a * kKvAtom + lane * 2048, &cp.k, &b.k_full[st], 64 * a, c1, c2);
           ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
           if (!ok) break;
           uint64_t* bar = cut ? &b.v_fix : &b.v_full[st];
@@ -502,16 +516,16 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           __syncwarp();
           if (fetch)
             for (int a = 0; a < NA; ++a)
-              tma_load_3d(v_addr + (st * NA + a) * kAtom + lane * 2048, &cp.v, bar, 64 * a, c1, c2);
+              tma_load_3d(v_addr + st * kTile + a * kKvAtom + lane * 2048, &cp.v, bar, 64 * a, c1, c2);
           if (cut) {
             ok = __all_sync(0xffffffffu, mbar_wait(&b.v_fix, fixes & 1, abort_flag));
             if (!ok) break;
             ++fixes;
-            for (int w = lane; w < kTP * 8; w += 32) {
+            for (int w = lane; w < TP * 8; w += 32) {
               const int row = w >> 3;
               if (unseen(x0 + row) || ((gone >> (row >> 4)) & 1u))
                 for (int a = 0; a < NA; ++a)
-                  st_shared_v4(v_addr + (st * NA + a) * kAtom + row * 128 + (w & 7) * 16, 0u, 0u, 0u, 0u);
+                  st_shared_v4(v_addr + st * kTile + a * kKvAtom + row * 128 + (w & 7) * 16, 0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -522,11 +536,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     }
     else if (warp == 11) {
       // ------------------------------------------------------------ the plan, and notes for the merge
-      Segments<kUnitRows, kTP> seg;
+      Segments<kUnitRows, TP> seg;
       int4 meta = make_int4(-1, 0, 0, 0);
       uint32_t k = 0;
       bool ok = true;
-      for (seg.begin(p, lane, blockIdx.x, kLeast); ok; ++k) {
+      for (seg.begin(p, lane, blockIdx.x, kLeast * 128 / TP); ok; ++k) {
         const bool more = seg.on();
         const uint32_t slot = k % kPlans;
         ok = __all_sync(0xffffffffu, mbar_wait(&b.plan_empty[slot], ((k / kPlans) & 1) ^ 1, abort_flag));
@@ -536,7 +550,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           if (more) {
             const Unit& x = seg.u;
             q = {x.b, x.h, x.rt, x.len, x.n, x.first, x.rows, x.lo, x.hi, x.s_end, x.st, x.skip, seg.t0,
-                 max(0, min(seg.t1, tiles_of(p, x, 0)) - seg.t0), max(0, min(seg.t1, tiles_of(p, x, 1)) - seg.t0),
+                 max(0, min(seg.t1, tiles_of<TP>(p, x, 0)) - seg.t0), max(0, min(seg.t1, tiles_of<TP>(p, x, 1)) - seg.t0),
                  seg.whole() ? 1 : 0, seg.slot()};
           }
           plan_ring[slot] = q;
@@ -553,7 +567,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   } else if (warp >= 12) {
     // -------------------------------------------------------------- loaders of 8-bit pages
     if (kF16) {
-      const int tid = threadIdx.x - 384, shift = p.w.shift;              // a thread per position: a row of K and of V
+      // 128 threads per tile: kParts of them for a position, each every kParts-th word of its rows of K and V
+      constexpr int kParts = kTileRows / TP, kWords = 4 * NA / kParts;
+      const int tid = (threadIdx.x - 384) % TP, part = (threadIdx.x - 384) / TP, shift = p.w.shift;
+      const int chunk = tid >> 5;                                        // 32 positions of this warp
       // the tile that is fetched, one ahead of the one that is stored
       int j = 0, n = 0;
       auto more = [&]() {                                                // skips segments without work
@@ -566,7 +583,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       };
       struct Row { bool on, gone; size_t at; float ks, vs; };
       auto find = [&]() {
-        const int x = place(u, j) + tid, x16 = x & ~15;
+        const int x = place<TP>(u, j) + tid, x16 = x & ~15;
         int id = -1;
         if (x16 < u.hi && (x16 + 16 > u.lo || x16 < u.s_end)) {
           id = __ldg(p.w.c.table + static_cast<size_t>(u.b) * p.w.c.width + (x >> shift));
@@ -583,10 +600,11 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         r.vs = r.on ? __ldg(p.w.c.v_scale + r.at) : 0.f;
         return r;
       };
-      auto fetch = [&](const void* pool, const Row& r, uint4 (&raw)[4 * NA]) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + r.at * dh);
+      auto fetch = [&](const void* pool, const Row& r, uint4 (&raw)[kWords]) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + r.at * dh) + part;
 #pragma unroll
-        for (int c = 0; c < 4 * NA; ++c) raw[c] = r.on && c < ksteps ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < kWords; ++c)
+          raw[c] = r.on && kParts * c + part < ksteps ? __ldg(src + kParts * c) : make_uint4(0u, 0u, 0u, 0u);
       };
       // biased exponent of the warp's largest finite scale: that of 1 where there is none, and of 2^-107 at least, so
       // that its products with a score's factor do not vanish
@@ -597,7 +615,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         return e == 0u ? 127u : max(e, 20u);
       };
       // codes * r as fp16, r in two parts: the product is rounded once
-      auto store = [&](const uint4 (&raw)[4 * NA], uint32_t tile, float r) {
+      auto store = [&](const uint4 (&raw)[kWords], uint32_t tile, float r) {
         const __half hi = __float2half_rn(r), lo = __float2half_rn(r - __half2float(hi));
         const __half2 h2 = __half2half2(hi), l2 = __half2half2(lo);
         auto scaled = [&](uint32_t x) {
@@ -606,16 +624,17 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           return *reinterpret_cast<const uint32_t*>(&y);
         };
 #pragma unroll
-        for (int c = 0; c < 4 * NA; ++c) {                                // sixteen codes: two words of eight columns
-          if (c < ksteps) {
+        for (int c = 0; c < kWords; ++c) {                                // sixteen codes: two words of eight columns
+          const int word = 2 * (kParts * c + part);
+          if (word < 2 * ksteps) {
             const uint2 a = codes_to_f16<KIND, false>(raw[c].x), d = codes_to_f16<KIND, false>(raw[c].y),
                         e = codes_to_f16<KIND, false>(raw[c].z), f = codes_to_f16<KIND, false>(raw[c].w);
-            st_shared_v4(swz(tile, tid, 2 * c), scaled(a.x), scaled(a.y), scaled(d.x), scaled(d.y));
-            st_shared_v4(swz(tile, tid, 2 * c + 1), scaled(e.x), scaled(e.y), scaled(f.x), scaled(f.y));
+            st_shared_v4(swz<kKvAtom>(tile, tid, word), scaled(a.x), scaled(a.y), scaled(d.x), scaled(d.y));
+            st_shared_v4(swz<kKvAtom>(tile, tid, word + 1), scaled(e.x), scaled(e.y), scaled(f.x), scaled(f.y));
           }
         }
       };
-      uint4 kraw[4 * NA], vraw[4 * NA];
+      uint4 kraw[kWords], vraw[kWords];
       Row r = {false, true, 0, 0.f, 0.f};
       bool have = more(), ok = true;
       if (have) {
@@ -624,7 +643,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         fetch(p.w.c.v, r, vraw);
       }
       for (uint32_t nk = 0; have && ok; ++nk) {
-        const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1, slot = nk % kMeta<NA>;
+        const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1, slot = nk % kMeta;
         const uint32_t none = __ballot_sync(0xffffffffu, r.gone);         // two sixteens of this warp
         const uint32_t ek = largest(r.ks), ev = largest(r.vs);
         // 2^(127 - e) as a float: e of 254 at most
@@ -636,13 +655,13 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&b.k_empty[st], par, abort_flag));
         if (!ok) break;
-        if (lane == 0) {
-          float* e = reinterpret_cast<float*>(smem + L::kExp) + slot * 8 + (warp - 12);
+        if (lane == 0 && part == 0) {
+          float* e = reinterpret_cast<float*>(smem + L::kExp) + slot * 8 + chunk;
           e[0] = __uint_as_float(ek << 23);
           e[4] = static_cast<float>(static_cast<int>(ev) - 127);
-          reinterpret_cast<volatile uint8_t*>(absent + slot)[warp - 12] = (none & 0xffffu ? 1 : 0) | (none >> 16 ? 2 : 0);
+          reinterpret_cast<volatile uint8_t*>(absent + slot)[chunk] = (none & 0xffffu ? 1 : 0) | (none >> 16 ? 2 : 0);
         }
-        store(kraw, k_addr + st * NA * kAtom, rk);
+        store(kraw, k_addr + st * kTile, rk);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.k_full[st]);
@@ -655,7 +674,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&b.v_empty[st], par, abort_flag));
         if (!ok) break;
-        store(vraw, v_addr + st * NA * kAtom, rv);
+        store(vraw, v_addr + st * kTile, rv);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.v_full[st]);
@@ -667,7 +686,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     // -------------------------------------------------------------- softmax, a thread per query row
     const int i = warp >> 2, row = threadIdx.x - 128 * i;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = s_col(i) + lanes, o_at = o_col(i) + lanes, p_at = p_col(i) + lanes;
+    const uint32_t s_base = s_col(i) + lanes, o_at = o_col(i) + lanes, p_base = p_col(i) + lanes;
     const uint32_t q_tile = q_addr + i * NA * kAtom;
     const int first_row = 32 * (warp & 3), words = 2 * ksteps;  // of this warp; 16-byte words of a row
     const bool flat = p.scale_log2 == 0.f;
@@ -697,6 +716,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
       }
     };
+    constexpr int kParts = TP / 32;                // of a row of S
     uint32_t nk = 0, ns = 0, nq = 0;               // tiles loaded, S of this tile, its segments with work so far
     bool ok = true, have = plans.next(u, lane);
     if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
@@ -755,28 +775,28 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       if (mine > 0) ++nq;
       float m = kFloor, l = 0.f;
       for (int j = 0; j < mine; ++j, ++ns) {
-        const uint32_t st = (nk + j) % kMeta<NA>;
-        ok = __all_sync(0xffffffffu, wait_hot(&b.s_full[i], ns & 1, abort_flag));
+        const uint32_t st = (nk + j) % kMeta;
+        const uint32_t at = kAlias ? ns & 1u : 0u;         // which S
+        ok = __all_sync(0xffffffffu, wait_hot(&b.s_full[i][at], (kAlias ? ns >> 1 : ns) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
+        const uint32_t s_at = s_base + at * TP, p_at = kAlias ? s_at : p_base;
         const uint32_t gone = absent[st];
-        const int x0 = place(u, j);
-        const bool hidden = gone != 0u || x0 + kTP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
+        const int x0 = place<TP>(u, j);
+        const bool hidden = gone != 0u || x0 + TP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
         // of columns 32 c ..: score (in powers of two) = product * fc + ev
-        float fc[4] = {f, f, f, f}, ev[4] = {0.f, 0.f, 0.f, 0.f};
-        if (kF16) {
-          const float* e = reinterpret_cast<const float*>(smem + L::kExp) + st * 8;
+        float fc[kParts], ev[kParts];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            fc[c] *= e[c];
-            ev[c] = e[4 + c];
-          }
+        for (int c = 0; c < kParts; ++c) {
+          const float* e = reinterpret_cast<const float*>(smem + L::kExp) + st * 8 + c;
+          fc[c] = kF16 ? f * e[0] : f;
+          ev[c] = kF16 ? e[4] : 0.f;
         }
         // what a row does not see is -inf and weighs nothing: in TMEM, so that the tiles in between, most of them, have
         // nothing to do with it
         if (hidden) {
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < TP / 16; ++c) {
             const int x = x0 + 16 * c;                 // sixteen columns: most are seen, or not, by all rows of a warp
             const uint32_t away = gone >> (8 * (c >> 1) + (c & 1)) & 1u;
             if (away == 0u && x + 15 <= pos_lo && (x > pos_hi - p.window || x + 15 < p.sinks)) continue;
@@ -795,15 +815,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           }
           tmem_st_wait();
         }
-        // two passes over S, 64 and 32 columns at a time: a row of 128 would not fit the registers
-        float top = kFloor;
+        // a row of 64 stays in registers where they suffice; two passes over S elsewhere
+        float keep[64], top = kFloor;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[64];
-          tmem_ld64_now(s_at + 64 * h, x);
+        for (int h = 0; h < TP / 64; ++h) {
+          tmem_ld64_now(s_at + 64 * h, keep);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float* y = x + 32 * c;
+            const float* y = keep + 32 * c;
             float t0 = fmaxf(y[0], y[1]), t1 = fmaxf(y[2], y[3]);
 #pragma unroll
             for (int k = 4; k < 32; k += 4) {
@@ -813,14 +832,22 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             top = fmaxf(top, fmaf(fmaxf(t0, t1), fc[2 * h + c], ev[2 * h + c]));       // fc >= 0
           }
         }
-        if (!kAlias && j > 0) {                    // O, and the columns of P (elsewhere S could not be here otherwise)
+        // O complete up to the tile before, and the columns of a P of its own free
+        auto o_ready = [&]() {
           ok = __all_sync(0xffffffffu, wait_hot(&b.o_done[i], (ns - 1) & 1, abort_flag));
-          if (!ok) break;
           tc_fence_after();
+        };
+        if (!kAlias && j > 0) {
+          o_ready();
+          if (!ok) break;
         }
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
+          if (kAlias) {
+            o_ready();
+            if (!ok) break;
+          }
           const float m_new = fmaxf(m, top), d = exp2_fast(m - m_new);
           for (int c = 0; c < ksteps; ++c) {
             float o[16];
@@ -839,15 +866,15 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         float xs[2][32];
         if (kAhead) tmem_ld32(s_at, xs[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float* x = xs[kAhead ? c & 1 : 0];
+        for (int c = 0; c < kParts; ++c) {
+          float* x = kKeep ? keep + 32 * (c & 1) : xs[kAhead ? c & 1 : 0];
           if (kAhead) {
             tmem_ld_wait_dep32(x);
-            if (c < 3) tmem_ld32(s_at + 32 * (c + 1), xs[(c + 1) & 1]);
-          } else {
+            if (c < kParts - 1) tmem_ld32(s_at + 32 * (c + 1), xs[(c + 1) & 1]);
+          } else if (!kKeep) {
             tmem_ld32_now(s_at + 32 * c, x);
           }
-          if (!kAlias && c == 3) {
+          if (!kAlias && c == kParts - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&b.s_free[i]);
@@ -867,11 +894,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           l += kF16 ? part * exp2_fast(-ev[c]) : part;
           if (c & 1) {
             tmem_st_wait();
+            // seen for every tile, so that no wait for this barrier, here or behind the loop, is two phases off
+            if (kAlias && j > 0) o_ready();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(c == 1 ? &b.p_half[i] : &b.p_full[i]);
+            if (lane == 0) mbar_arrive(c == kParts - 1 ? &b.p_full[i] : &b.p_half[i]);
           }
         }
+        if (!ok) break;
       }
       nk += n;
       if (!ok) break;
@@ -966,14 +996,15 @@ __global__ void __launch_bounds__(256) paged_merge_chunk_kernel(const AttnParams
   st_global_v8(dst, w);
 }
 
-// Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (128 rows at most).
+// Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (a tile's positions at most).
 int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
+  const int most = c.dh <= 64 ? kTP<1> : kTP<2>;
   auto enc = tensor_map_encoder();
   if (enc == nullptr) return 1;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.dh), static_cast<cuuint64_t>(c.page),
                         static_cast<cuuint64_t>(c.n_pages) * static_cast<cuuint64_t>(c.H)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.dh) * 2, static_cast<cuuint64_t>(c.dh) * 2 * c.page};
-  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(c.page < kTP ? c.page : kTP), 1};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(c.page < most ? c.page : most), 1};
   cuuint32_t estr[3] = {1, 1, 1};
   if (dims[2] == 0) dims[2] = 1;              // no page: nothing is fetched
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(pool), dims, strides, box, estr,
