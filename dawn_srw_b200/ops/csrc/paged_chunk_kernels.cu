@@ -29,7 +29,10 @@ constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows;
 constexpr int kAtom = kTileRows * 128;      // 128 rows x 64 16-bit columns
 // Positions of a tile.  TMEM holds two O, two S and, for heads of up to 64, two P, so that the next S can be made while P
 // is.  For wider heads P takes the place of S, and the next S has to have another place: two S of 64 positions per
-// query tile (ragged prompts of 16 heads of 128: ? us for 97 with one of 128 and the wait for P that it takes).
+// query tile.  Heads of 128 against one S of 128, whose softmax waits for the products: 5 sequences x 512 tokens 27 us
+// for 31, ragged prompts 91 for 97.  For heads of 64 two S of 64 are slower than S and P beside each other: 148 heads,
+// 256 tokens over 4352 positions 78 us for 67 (int8 98 for 74), since a product of 64 columns keeps the tensor core
+// busy for 48 cycles where half of one of 128 takes 32: it reads Q from shared memory all the same.
 template <int NA> constexpr int kTP = NA == 1 ? 128 : 64;
 constexpr int kStages = 4;                  // tiles of K, and of V, in shared memory
 // Slots of scales and absences: written with K, read by a softmax that may be a tile behind the last use of the stage.
@@ -283,7 +286,7 @@ struct Bars {
   uint64_t s_free[2];       // S has been read (4 warps); only where P has columns of its own
   uint64_t p_half[2];       // the first half of P is in TMEM (4 warps)
   uint64_t p_full[2];       // all of them
-  uint64_t o_done[2];
+  uint64_t o_done[2][2];    // [query tile][place of the S that became its weights]
   uint64_t plan_full[kPlans];
   uint64_t plan_empty[kPlans];  // every warp that works by the plan has read it
   uint32_t tmem;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   constexpr bool kF16 = KIND != kBf16;
   constexpr bool kAhead = kF16;                 // columns of S loaded one step ahead (183 us for 194; bf16 103 for 101)
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
-  constexpr bool kKeep = kAlias && !kF16;       // a row of S stays in registers (a loaders' kernel has too few of them)
+  constexpr bool kKeep = kAlias && !kF16;       // a row of S stays in registers (beside loaders there are too few of them)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr int S = kStages, TP = kTP<NA>, kHalf = TP / 2, kTile = L::kTile, kKvAtom = TP * 128;
@@ -340,7 +343,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.s_free[i], 4);
       mbar_init(&b.p_half[i], 4);
       mbar_init(&b.p_full[i], 4);
-      mbar_init(&b.o_done[i], 1);
+      mbar_init(&b.o_done[i][0], 1);
+      mbar_init(&b.o_done[i][1], 1);
     }
     for (int i = 0; i < S; ++i) {
       mbar_init(&b.k_full[i], kF16 ? 4 : 1);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   tc_fence_after();
   const uint32_t tmem = b.tmem;
   const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
-  // S: columns 0 and 128;  O: 256 and 256 + 64 NA;  P: where S is, or behind O
+  // S: columns 0 and 128 (two of 64 each, or one);  O: 256 and 256 + 64 NA;  P: where S is, or behind O
   auto s_col = [&](int i) { return tmem + 128 * i; };
   auto o_col = [&](int i) { return tmem + 256 + 64 * NA * i; };
   auto p_col = [&](int i) { return kAlias ? s_col(i) : tmem + 384 + 64 * i; };
@@ -446,10 +450,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             tc_fence_after();
 #pragma unroll
             for (int kk = kHalf / 16; kk < TP / 16; ++kk) mma_ts(o_at, pa + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
-            mma_commit(&b.o_done[I]);
+            mma_commit(&b.o_done[I][kAlias ? nt & 1u : 0u]);
             mma_commit(&b.v_empty[st]);
             if (kAlias) {                          // the S after the next takes the columns that this P is read from
-              wait(&b.o_done[I], nt);
+              wait(&b.o_done[I][nt & 1u], nt >> 1);
               if (j + 2 < mine && ok) issue_s(j + 2, nt + 2);
             }
           }
@@ -717,6 +721,9 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       }
     };
     constexpr int kParts = TP / 32;                // of a row of S
+    // until the x-th tile's product with V is in O.  With two places the barrier's phase before it, of tile x - 2, is past:
+    // S of tile x has been seen, which was made behind that product.
+    auto o_wait = [&](uint32_t x) { return wait_hot(&b.o_done[i][kAlias ? x & 1u : 0u], (kAlias ? x >> 1 : x) & 1, abort_flag); };
     uint32_t nk = 0, ns = 0, nq = 0;               // tiles loaded, S of this tile, its segments with work so far
     bool ok = true, have = plans.next(u, lane);
     if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
@@ -781,7 +788,15 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_at = s_base + at * TP, p_at = kAlias ? s_at : p_base;
+        // The two tiles' softmaxes, one of each per quarter of the SM, take turns with the exponential unit and with what
+        // is in front of it: the second starts half a tile later (ragged prompts, 91 us for 96).  Not for a few tiles.
+        if (kKeep && i == 1 && j == 0 && mine > 4) {
+          const long long t0 = clock64();
+          while (clock64() - t0 < 700) { }
+        }
         const uint32_t gone = absent[st];
+        float keep[64];
+        if (kKeep) tmem_ld64_now(s_at, keep);              // before it is known whether anything is hidden: rarely
         const int x0 = place<TP>(u, j);
         const bool hidden = gone != 0u || x0 + TP > pos_lo + 1 || x0 < pos_hi - p.window + 1;
         // of columns 32 c ..: score (in powers of two) = product * fc + ev
@@ -814,12 +829,13 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             tmem_st16(s_at + 16 * c, w);
           }
           tmem_st_wait();
+          if (kKeep) tmem_ld64_now(s_at, keep);
         }
         // a row of 64 stays in registers where they suffice; two passes over S elsewhere
-        float keep[64], top = kFloor;
+        float top = kFloor;
 #pragma unroll
         for (int h = 0; h < TP / 64; ++h) {
-          tmem_ld64_now(s_at + 64 * h, keep);
+          if (!kKeep) tmem_ld64_now(s_at + 64 * h, keep);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float* y = keep + 32 * c;
@@ -834,7 +850,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         // O complete up to the tile before, and the columns of a P of its own free
         auto o_ready = [&]() {
-          ok = __all_sync(0xffffffffu, wait_hot(&b.o_done[i], (ns - 1) & 1, abort_flag));
+          ok = __all_sync(0xffffffffu, o_wait(ns - 1));
           tc_fence_after();
         };
         if (!kAlias && j > 0) {
@@ -894,8 +910,6 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           l += kF16 ? part * exp2_fast(-ev[c]) : part;
           if (c & 1) {
             tmem_st_wait();
-            // seen for every tile, so that no wait for this barrier, here or behind the loop, is two phases off
-            if (kAlias && j > 0) o_ready();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(c == kParts - 1 ? &b.p_full[i] : &b.p_half[i]);
@@ -913,7 +927,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       have = plans.next(u, lane);
       if (have && (i == 0 ? u.n0 : u.n1) > 0) fetch_q();
       if (mine > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&b.o_done[i], (ns - 1) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, o_wait(ns - 1));
         if (!ok) break;
         tc_fence_after();
       }
