@@ -391,6 +391,11 @@ class PagedSession:
         if not 0 <= seq < self.max_seqs or self.pages[seq] is None:
             raise ValueError(f"sequence {seq} is not open")
 
+    def _check_ids(self, ids: torch.Tensor) -> None:
+        """Before anything changes: an index outside the embedding would end the process's use of a GPU."""
+        if ids.numel() and bool(((ids < 0) | (ids >= self.model.vocab_size)).any()):
+            raise ValueError(f"a token id is outside the vocabulary of {self.model.vocab_size}")
+
     def _grow(self, new: Dict[int, int]) -> None:
         """Room for ``new`` tokens of each sequence, or an error that changes nothing."""
         need = 0
@@ -477,6 +482,8 @@ class PagedSession:
         dev = self._table.device
         ids = {s: torch.as_tensor(t, dtype=torch.long, device=dev).reshape(-1) for s, t in new.items()}
         counts = {s: t.numel() for s, t in ids.items()}
+        packed = torch.cat(list(ids.values()))
+        self._check_ids(packed)
         self._grow(counts)
         self._refresh()
         seqs, ns = list(ids), list(counts.values())
@@ -485,7 +492,7 @@ class PagedSession:
         lengths = torch.tensor([self.lengths[s] for s in seqs], dtype=torch.int32, device=dev)
         starts = torch.tensor([0] + ns, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
         pos = torch.cat([torch.arange(self.lengths[s] - n, self.lengths[s]) for s, n in zip(seqs, ns)]).to(dev)
-        h = self._forward(self._embed(torch.cat([ids[s] for s in seqs]), pos), table, lengths, starts, max(ns))
+        h = self._forward(self._embed(packed, pos), table, lengths, starts, max(ns))
         self._forget(seqs)
         if all_logits:
             return list(self.be.logits(h, self.model.token_emb.weight).split(ns))
@@ -503,6 +510,7 @@ class PagedSession:
         if not tokens:
             raise ValueError("no sequence to extend")
         tokens = {s: int(t) for s, t in tokens.items()}
+        self._check_ids(torch.tensor(list(tokens.values())))
         self._grow({s: 1 for s in tokens})
         self._refresh()
         dev = self._table.device

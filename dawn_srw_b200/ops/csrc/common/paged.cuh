@@ -1,5 +1,5 @@
 // Device-side view of a paged key/value cache: which sequence a packed row belongs to, where a
-// position lives, and 8-bit codes as bf16.
+// position lives, and 8-bit codes as bf16 (for reading back; the attention's conversions are in paged_units.cuh).
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
@@ -35,7 +35,7 @@ inline bool bad_cache(const DsbPaged* c) {
   if (c->H <= 0 || c->n_pages < 0 || c->B < 0 || c->width < 0 || c->N < 0) return true;
   if (c->N > kMostPositions || static_cast<long long>(c->width) * c->page > kMostPositions) return true;
   if (c->starts == nullptr && c->N != c->B) return true;
-  if (c->kind != kBf16 && (c->k_scale == nullptr || c->v_scale == nullptr)) return true;
+  if (c->kind != kBf16 && c->n_pages > 0 && (c->k_scale == nullptr || c->v_scale == nullptr)) return true;
   return ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) != 0;
 }
 
@@ -89,7 +89,7 @@ __device__ __forceinline__ size_t slot_row(const View& w, int page, int h, int p
 // int8: 128 + (low seven bits) and 128 or 256 (by the sign bit) are bf16 values whose bits are the code's
 // own; their difference is the number.  e4m3: exponent and fraction moved into bf16's places read as the
 // value times 2^-120 (the biases differ by 120, subnormals included), so one product puts it right.  The
-// NaN codes 0x7f, 0xff, which no write here makes, read as +-480.
+// NaN codes 0x7f, 0xff, which no write here makes, read back as +-480 (the attention takes them as NaN).
 template <int KIND>
 __device__ __forceinline__ uint2 codes_to_bf16(uint32_t x) {
   uint2 r = {__byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342)};
@@ -108,15 +108,6 @@ __device__ __forceinline__ uint2 codes_to_bf16(uint32_t x) {
   r.x = one(r.x);
   r.y = one(r.y);
   return r;
-}
-
-// Eight elements at `row * dh + col` of a pool as four registers of bf16 pairs.
-template <int KIND>
-__device__ __forceinline__ uint4 load8(const void* pool, size_t elem) {
-  if (KIND == kBf16) return __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + elem));
-  const uint2 c = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + elem));
-  const uint2 a = codes_to_bf16<KIND>(c.x), b = codes_to_bf16<KIND>(c.y);
-  return make_uint4(a.x, a.y, b.x, b.y);
 }
 
 __device__ __forceinline__ void bf16x8_to_f32(const uint4& u, float* f) {

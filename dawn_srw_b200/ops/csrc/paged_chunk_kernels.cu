@@ -8,9 +8,9 @@
 //
 // bf16 pages come by TMA, one box per page and 64 columns, into the 128-byte-swizzled tiles that the instructions
 // read: K-major for K, MN-major for V.  8-bit codes are read by four warps and go to the same layout as fp16 numbers,
-// code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: rounded once, by 2^-11 at
-// most (an eighth of a weight's rounding and far below the codes' own; a scale per column in the softmax would cost
-// each thread three shared-memory reads per column).  2^e of the keys goes to the scores, 2^e of the values, as in
+// code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: exact for e4m3, whose scales
+// are powers of two, and rounded once, by 2^-11 at most, for int8 (as a weight is, and far below the codes' own
+// rounding; a scale per column in the softmax would cost each thread three shared-memory reads per column).  2^e of the keys goes to the scores, 2^e of the values, as in
 // the few-row kernel, to the exponents and out of the sum.  Rows of V that no query row sees are zeros, whatever the
 // page holds there; a scale that is no number makes the scores of its position NaN.
 //
@@ -285,7 +285,9 @@ struct Bars {
   uint64_t s_full[2][2];    // [query tile][place of S]
   uint64_t s_free[2];       // S has been read (4 warps); only where P has columns of its own
   uint64_t p_half[2];       // the first half of P is in TMEM (4 warps)
-  uint64_t p_full[2];       // all of them
+  // [query tile][place of S]  all of them.  A warp may be through with the next tile's S while another still makes this
+  // one's P, so that with two places one barrier would count the first warp twice.
+  uint64_t p_full[2][2];
   uint64_t o_done[2][2];    // [query tile][place of the S that became its weights]
   uint64_t plan_full[kPlans];
   uint64_t plan_empty[kPlans];  // every warp that works by the plan has read it
@@ -342,7 +344,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.s_full[i][1], 1);
       mbar_init(&b.s_free[i], 4);
       mbar_init(&b.p_half[i], 4);
-      mbar_init(&b.p_full[i], 4);
+      mbar_init(&b.p_full[i][0], 4);
+      mbar_init(&b.p_full[i][1], 4);
       mbar_init(&b.o_done[i][0], 1);
       mbar_init(&b.o_done[i][1], 1);
     }
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             }
             wait(&b.v_full[st], (nk + j) / S);
             if (!kAlias) wait(&b.p_half[I], nt);
-            if (kAlias) wait(&b.p_full[I], nt);
+            if (kAlias) wait(&b.p_full[I][nt & 1u], nt >> 1);
             if (!ok) break;
             tc_fence_after();
             const uint64_t va = v_desc + st * (kTile >> 4);
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             mma_ts(o_at, pa, va, idesc_o, j > 0);
 #pragma unroll
             for (int kk = 1; kk < kHalf / 16; ++kk) mma_ts(o_at, pa + 8 * kk, va + (kk * 2048 >> 4), idesc_o, 1u);
-            if (!kAlias) wait(&b.p_full[I], nt);
+            if (!kAlias) wait(&b.p_full[I][0], nt);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -912,7 +915,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(c == kParts - 1 ? &b.p_full[i] : &b.p_half[i]);
+            if (lane == 0) mbar_arrive(c == kParts - 1 ? &b.p_full[i][at] : &b.p_half[i]);
           }
         }
         if (!ok) break;
@@ -1011,7 +1014,8 @@ __global__ void __launch_bounds__(256) paged_merge_chunk_kernel(const AttnParams
 }
 
 // Pages as [n_pages * H][page][dh], boxes of 64 columns by one page (a tile's positions at most).
-int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
+int page_map(CUtensorMap* map, const void* pool, const AttnParams& a) {
+  const DsbPaged& c = a.w.c;
   const int most = c.dh <= 64 ? kTP<1> : kTP<2>;
   auto enc = tensor_map_encoder();
   if (enc == nullptr) return 1;
@@ -1020,7 +1024,10 @@ int page_map(CUtensorMap* map, const void* pool, const DsbPaged& c) {
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.dh) * 2, static_cast<cuuint64_t>(c.dh) * 2 * c.page};
   cuuint32_t box[3] = {64, static_cast<cuuint32_t>(c.page < most ? c.page : most), 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  if (dims[2] == 0) dims[2] = 1;              // no page: nothing is fetched
+  if (dims[2] == 0) {                         // no page: nothing is fetched, but a map wants an address
+    dims[2] = 1;
+    pool = a.q;
+  }
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(pool), dims, strides, box, estr,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : 2;
@@ -1067,7 +1074,7 @@ int launch_chunk(AttnParams& a, void* workspace, cudaStream_t stream) {
             query_map(&p.q, a) == 0;
   int rc;
   if (a.w.c.kind == kBf16) {
-    if (page_map(&p.k, a.w.c.k, a.w.c) || page_map(&p.v, a.w.c.v, a.w.c)) return 952;
+    if (page_map(&p.k, a.w.c.k, a) || page_map(&p.v, a.w.c.v, a)) return 952;
     rc = launch_dim<kBf16>(p, stream);
   } else if (a.w.c.kind == kE4m3) {
     rc = launch_dim<kE4m3>(p, stream);

@@ -5,7 +5,8 @@ Pages of keys and values are ``[n_pages, H, page, dh]``: bf16, or 8-bit codes (`
 ``int8``) with fp32 scales ``[n_pages, H, page]``, one for each position and head.  ``table [B, width]``
 (int32) names the page of positions ``i * page .. (i + 1) * page`` of a sequence, ``lengths [B]`` (int32)
 its positions, new tokens included.  The new tokens of all sequences are packed: rows ``starts[b] ..
-starts[b + 1]`` are the last tokens of sequence ``b``; ``starts`` is None where every sequence has one.
+starts[b + 1]`` (ascending) are the last tokens of sequence ``b``; ``starts`` is None where every sequence
+has one.  Sequences may share pages that they read; what one call writes twice to a place is either value.
 
 A row of keys or values is stored with one rounding: bf16; e4m3 after division by the smallest power of
 two that brings the row's largest magnitude to 448 or less; or int8, ``round(x * (127 / largest))`` with
@@ -32,7 +33,8 @@ def _refuse_unless(ok: bool, msg: str) -> None:
 
 
 def check_cache(k_pages, v_pages, table, lengths, starts, k_scale, v_scale, rows: int) -> None:
-    """What the kernels' bindings check too, but for the head dimensions that only they cannot take."""
+    """What the kernels' bindings check too, but for the head dimensions and sizes (more than 65535 sequences or
+    heads, 2^30 rows or positions) that only they cannot take."""
     _refuse_unless(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
                    "k and v pages must have one shape [n_pages, heads, page, dim] and one type")
     _refuse_unless(k_pages.is_contiguous() and v_pages.is_contiguous(), "pages must be contiguous")

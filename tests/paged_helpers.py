@@ -87,12 +87,34 @@ def attention64(q, c, new, window=None, sinks=0, scale=None):
     return out, mag
 
 
-def assert_attention(got, ref, mag):
+def largest_score(q, c, new, scale=None):
+    """The largest scale * sum |q| |k| of any row and any position of its sequence."""
+    H, G = c["k_pages"].shape[1], q.shape[1] // c["k_pages"].shape[1]
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else abs(scale)
+    most, at = 0.0, 0
+    for b, n in enumerate(new):
+        if n and int(c["lengths"][b]):
+            k = held64(c, b, int(c["lengths"][b]), "k").abs()
+            s = torch.einsum("rhgd,nhd->rhgn", q[at: at + n].double().abs().view(n, H, G, -1), k)
+            most = max(most, float(s.max()) * scale)
+        at += n
+    return most
+
+
+def assert_attention(got, ref, mag, rounded_scores=0.0):
     """A bf16 result of bf16 operands: each weight is rounded to bf16 once (2^-8 of it at most, so 2^-8 of
     sum p |v|), the result once (2^-8 of it); what is left is fp32 (scores of magnitude below 100 from sums of
-    at most 128 products: below 2^-12 of a weight)."""
+    at most 128 products: below 2^-12 of a weight).
+
+    Over 8-bit pages the weights are fp16 (2^-11), and a chunk's int8 keys and values, code * scale, are rounded
+    to fp16 too: 2^-11 of sum p |v| for the values, and a score moves by 2^-11 of scale * sum |q| |k| =: A at most,
+    a weight by that and, through the sum of all, by that again.  2^-11 (2 + 2 A) is within the 2^-8 above while
+    A <= 3 even if all roundings have one sign; rows of random numbers, whose roundings have not, stay far below it
+    at A of 10.  Where scores are made large on purpose, ``rounded_scores`` = A adds the term 2 * 2^-11 A, with
+    another 1 + 2^-11 A for the exponential's second order (A below 100)."""
     assert got.dtype == torch.bfloat16
     err = (got.double() - ref).abs()
     tol = ref.abs() * 2.0 ** -8 + mag * (2.0 ** -8 + 2.0 ** -12) * (1 + 2.0 ** -8)
+    tol = tol + mag * 2.0 ** -10 * rounded_scores * (1 + 2.0 ** -11 * rounded_scores)
     bad = ~(err <= tol)
     assert not bool(bad.any()), (int(bad.sum()), float((err - tol)[bad].max()), bad.nonzero()[:4].tolist())

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dawn_srw_b200.ops import paged as P
-from paged_helpers import KINDS, args, assert_attention, attention64, make_cache, scales, starts_of
+from paged_helpers import KINDS, args, assert_attention, attention64, largest_score, make_cache, scales, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -367,3 +367,57 @@ def test_a_prompt_in_chunks_then_tokens(cb, be, kind):
             want = P.decode_rows(*P.encode_rows(x[b], c["k_pages"].dtype)).transpose(0, 1)
             assert torch.equal(got[b, :, :t], want) and not bool(got[b, :, t:].any())
     cb.check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [48, 80, 128])
+@pytest.mark.parametrize("new", [[1, 1], [300, 40]])
+def test_the_running_maximum_moves_in_every_tile(cb, be, kind, dh, new):
+    """Scores that rise (first sequence) or fall along the context, by several powers of two from tile to tile."""
+    lengths = [1100, 333]
+    c = make_cache(kind, lengths, 2, dh, 16, "cuda", garbage=False)
+    for b, up in enumerate((1.0, -1.0)):
+        for i in range(-(-lengths[b] // 16)):
+            page = int(c["table"][b, i])
+            x = torch.randn(2, 16, dh, device="cuda", generator=torch.Generator("cuda").manual_seed(i)) * 0.1
+            x[..., 0] += up * (i - 30)
+            codes, scale = P.encode_rows(x, P.PAGE_DTYPES[kind])
+            c["k_pages"][page] = codes
+            if scale is not None:
+                c["k_scale"][page] = scale
+    q = _rand(sum(new), 4, dh, dtype=torch.bfloat16, seed=5)
+    q[..., 0] = q[..., 0].abs() + 2.0
+    starts = None if new == [1, 1] else starts_of(new, "cuda")
+    got = be.paged_attention(q, *args(c), starts, **scales(c))
+    for _ in range(30):                                           # the order of a block's warps changes nothing
+        assert torch.equal(be.paged_attention(q, *args(c), starts, **scales(c)), got)
+    ref, mag = attention64(q, c, new)
+    assert_attention(got, ref, mag, largest_score(q, c, new) if kind == "int8" and new != [1, 1] else 0.0)
+    cb.check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+def test_a_pool_without_pages(cb, be, kind, new):
+    c = make_cache(kind, [0, 0], 2, 64, 16, "cuda", spare=0)
+    assert c["k_pages"].shape[0] == 0
+    q = _rand(sum(new), 2, 64, dtype=torch.bfloat16)
+    starts = None if new == [1, 1] else starts_of(new, "cuda")
+    assert not bool(be.paged_attention(q, *args(c), starts, **scales(c)).any())
+    be.paged_write(q, q, *args(c), starts, **scales(c))
+    assert not bool(be.paged_read(*args(c), 9, **scales(c))[0].any())
+    cb.check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh,G", [(64, 1), (128, 2), (112, 3)])
+def test_chunks_of_many_shapes(cb, be, kind, dh, G):
+    """Runs of one tile, of a few and of many, units that blocks share, row tiles with and without work."""
+    gen = torch.Generator().manual_seed(dh)
+    for i in range(6):
+        B = int(torch.randint(1, 5, (1,), generator=gen))
+        lengths = torch.randint(1, (64, 500, 1500)[i % 3], (B,), generator=gen).tolist()
+        new = [int(torch.randint(1, min(n, 400) + 1, (1,), generator=gen)) for n in lengths]
+        window = (None, 150, 33)[(i // 2) % 3]
+        _check(cb, be, kind, 2, G, dh, (16, 64, 256)[i % 3], lengths, new, window, 0 if window is None else 5, seed=i,
+               max_new=1000)

@@ -196,3 +196,16 @@ def test_refusals():
     with pytest.raises(ValueError, match="max_seq_len"):
         s.extend({a: torch.ones(91, dtype=torch.long)})
     assert s.lengths == [0, 0] and len(s.free_pages) == 12
+
+
+@pytest.mark.parametrize("bad", [-1, 200, 2 ** 40])
+def test_ids_outside_the_vocabulary_are_refused(bad):
+    m = _model("dense")
+    s = I.PagedSession(m, 2)
+    a, b = s.open(), s.open()
+    with pytest.raises(ValueError, match="vocabulary"):
+        s.extend({a: torch.tensor([5]), b: torch.tensor([3, bad, 4])})
+    with pytest.raises(ValueError, match="vocabulary"):
+        s.step({a: 7, b: bad})
+    assert s.lengths == [0, 0] and s.pages[a] == s.pages[b] == []
+    assert s.extend({a: torch.tensor([0, 199])}).shape == (1, 200)
