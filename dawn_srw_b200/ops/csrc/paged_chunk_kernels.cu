@@ -16,6 +16,16 @@
 //
 // The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
+//
+// What bounds it.  The products alone, at the rate of a large matrix product (1.66 PFLOP/s), are a third of the time:
+// five bf16 prompts of 301 to 2048 tokens, 16 heads of 128, 96 us for 31; 4099 tokens over 16000 int8 positions, 16
+// heads of 64 that share 4 and a window of 4096, 181 us for 61.  128 positions of a unit take about 4000 cycles.  By
+// arithmetic the exponential unit has 1700 of them to do, shared memory at 128 bytes a cycle 1800 (heads of 64) to 2800
+// (heads of 128) for the products' operands and 512 for the loads; the clock inside the kernel shows some 700 cycles
+// per tile and warp that are waits, and latencies of TMEM and shared memory, in the open: the two softmax warps of a
+// quarter of the SM run in step.  Starting one of them later changed nothing; more exponentials on the FMA units lost.
+// A small call, 512 tokens over 2100 e4m3 positions, 16 heads of 80, takes 27 us for 3: its plan (2.5 us), two runs a
+// block, the pieces and their merge (8 us).
 #include <type_traits>
 
 #include "common/host_utils.cuh"
@@ -29,8 +39,8 @@ constexpr int kTileRows = 128, kUnitRows = 2 * kTileRows;
 constexpr int kAtom = kTileRows * 128;      // 128 rows x 64 16-bit columns
 // Positions of a tile.  TMEM holds two O, two S and, for heads of up to 64, two P, so that the next S can be made while P
 // is.  For wider heads P takes the place of S, and the next S has to have another place: two S of 64 positions per
-// query tile.  Heads of 128 against one S of 128, whose softmax waits for the products: 5 sequences x 512 tokens 27 us
-// for 31, ragged prompts 91 for 97.  For heads of 64 two S of 64 are slower than S and P beside each other: 148 heads,
+// query tile.  Against one S of 128, whose softmax waits for the products: 512 tokens over 2100 e4m3 positions, 16
+// heads of 80, 27 us for 31, ragged bf16 prompts with heads of 128 96 for 97.  For heads of 64 two S of 64 are slower than S and P beside each other: 148 heads,
 // 256 tokens over 4352 positions 78 us for 67 (int8 98 for 74), since a product of 64 columns keeps the tensor core
 // busy for 48 cycles where half of one of 128 takes 32: it reads Q from shared memory all the same.
 template <int NA> constexpr int kTP = NA == 1 ? 128 : 64;
@@ -791,12 +801,6 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_at = s_base + at * TP, p_at = kAlias ? s_at : p_base;
-        // The two tiles' softmaxes, one of each per quarter of the SM, take turns with the exponential unit and with what
-        // is in front of it: the second starts half a tile later (ragged prompts, 91 us for 96).  Not for a few tiles.
-        if (kKeep && i == 1 && j == 0 && mine > 4) {
-          const long long t0 = clock64();
-          while (clock64() - t0 < 700) { }
-        }
         const uint32_t gone = absent[st];
         float keep[64];
         if (kKeep) tmem_ld64_now(s_at, keep);              // before it is known whether anything is hidden: rarely
