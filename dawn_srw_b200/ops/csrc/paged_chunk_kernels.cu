@@ -590,13 +590,16 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       const int chunk = tid >> 5;                                        // 32 positions of this warp
       // the tile that is fetched, one ahead of the one that is stored
       int j = 0, n = 0;
-      auto more = [&]() {                                                // skips segments without work
+      // 1: there is one, 0: none.  -1, unless `far`: the next segment has none.  Further plans come only when those who
+      // work by the first have gone on, for which they may still want the values of the tile that is being stored.
+      auto more = [&](bool far) {
         while (j >= n) {
-          if (!plans.next(u, lane)) return false;
+          if (!plans.next(u, lane)) return 0;
           n = max(u.n0, u.n1);
           j = 0;
+          if (n == 0 && !far) return -1;
         }
-        return true;
+        return 1;
       };
       struct Row { bool on, gone; size_t at; float ks, vs; };
       auto find = [&]() {
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       };
       uint4 kraw[kWords], vraw[kWords];
       Row r = {false, true, 0, 0.f, 0.f};
-      bool have = more(), ok = true;
+      bool have = more(true) > 0, ok = true;
       if (have) {
         r = find();
         fetch(p.w.c.k, r, kraw);
@@ -683,9 +686,9 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.k_full[st]);
         ++j;
-        have = more();
+        int got = more(false);
         Row next = {false, true, 0, 0.f, 0.f};
-        if (have) {
+        if (got > 0) {
           next = find();
           fetch(p.w.c.k, next, kraw);
         }
@@ -695,6 +698,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.v_full[st]);
+        if (got < 0) {
+          got = more(true);
+          if (got > 0) {
+            next = find();
+            fetch(p.w.c.k, next, kraw);
+          }
+        }
+        have = got > 0;
         if (have) fetch(p.w.c.v, next, vraw);
         r = next;
       }

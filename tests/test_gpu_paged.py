@@ -421,3 +421,14 @@ def test_chunks_of_many_shapes(cb, be, kind, dh, G):
         window = (None, 150, 33)[(i // 2) % 3]
         _check(cb, be, kind, 2, G, dh, (16, 64, 256)[i % 3], lengths, new, window, 0 if window is None else 5, seed=i,
                max_new=1000)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("window", [None, 100])
+def test_many_sequences_without_work_between_others(cb, be, kind, dh, window):
+    """Runs of units that have rows and no positions, longer than what a block plans ahead, behind a unit with some."""
+    lengths = [1, 79, 1, 0, 1, 300, 0, 1, 0, 1, 200, 0, 0, 0, 40]
+    new = [0, 50, 1, 1, 1, 262, 0, 3, 1, 4, 200, 2, 1, 9, 40]
+    _check(cb, be, kind, 8, 8, dh, 16, lengths, new, window, extra=3)
+    _check(cb, be, kind, 8, 1, dh, 16, lengths, [min(n, 1) for n in new], window, extra=1)
