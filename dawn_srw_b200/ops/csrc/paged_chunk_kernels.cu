@@ -23,7 +23,7 @@
 // arithmetic the exponential unit has 1700 of them to do, shared memory at 128 bytes a cycle 1800 (heads of 64) to 2800
 // (heads of 128) for the products' operands and 512 for the loads; the clock inside the kernel shows some 700 cycles
 // per tile and warp that are waits, and latencies of TMEM and shared memory, in the open: the two softmax warps of a
-// quarter of the SM run in step.  Starting one of them later changed nothing; more exponentials on the FMA units lost.
+// quarter of the SM run in step.  Starting one of them later changed nothing; exponentials on the FMA units help by 3 % at most (see kPoly).
 // A small call, 512 tokens over 2100 e4m3 positions, 16 heads of 80, takes 27 us for 3: its plan (2.5 us), two runs a
 // block, the pieces and their merge (8 us).
 #include <type_traits>
@@ -184,8 +184,9 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 }
 // How many of sixteen exponentials are made this way.  With four loading warps beside the softmax the issue slots are
 // what is short, not the exponential unit: 4099 tokens over 16000 int8 positions took 183 us with none, 196 with four
-// and 220 with eight; ragged bf16 prompts of up to 2048 tokens 105, 101 (three), 102 and 107 us.
-template <int KIND> constexpr int kPoly = KIND == kBf16 ? 3 : 0;
+// and 220 with eight.  bf16, heads of 64, 24 x 4096 tokens: 96.5 with none, 93.6 with three; heads of 128, whose softmax
+// waits for other things, ragged prompts: 95.6 with none, 97.4 with three.
+template <int KIND, int NA> constexpr int kPoly = KIND == kBf16 && NA == 1 ? 3 : 0;
 
 // Instruction descriptor, kind::f16, fp32 accumulators: A and B both bf16 or both fp16.
 __host__ __device__ constexpr uint32_t idesc16(bool bf16, int m, int n, int b_mn_major) {
@@ -330,7 +331,7 @@ template <int KIND, int NA>
 __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
   using L = Smem<NA>;
   constexpr bool kF16 = KIND != kBf16;
-  constexpr bool kAhead = kF16;                 // columns of S loaded one step ahead (183 us for 194; bf16 103 for 101)
+  constexpr bool kAhead = kF16;                 // columns of S loaded one step ahead (int8: 183 us for 194; bf16 lost 2 of 101)
   constexpr bool kAlias = NA > 1;               // no room for P beside S and O: it takes the place of S
   constexpr bool kKeep = kAlias && !kF16;       // a row of S stays in registers (beside loaders there are too few of them)
   extern __shared__ uint8_t smem_raw[];
@@ -919,7 +920,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             float2 y = fma2(make_float2(x[k], x[k + 1]), make_float2(fc[c], fc[c]), make_float2(off, off));
-            y = (k / 2) % 16 < kPoly<KIND> ? exp2_poly(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            y = (k / 2) % 16 < kPoly<KIND, NA> ? exp2_poly(y) : make_float2(exp2_fast(y.x), exp2_fast(y.y));
             sum = add2(sum, y);
             w[k / 2] = kF16 ? pack_f16x2(y.x, y.y) : pack_bf16x2(y.x, y.y);
           }
