@@ -60,8 +60,9 @@ DsbPaged view(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTe
   REFUSE_UNLESS(N <= (1 << 30) && B <= 65535, "more than 65535 sequences, or too many rows");
   REFUSE_UNLESS(v.device() == k.device() && table.device() == k.device() && lengths.device() == k.device(),
                 "pages, table and lengths must be on one device");
+  REFUSE_UNLESS(aligned(k) && aligned(v) && (!scaled || (aligned(*ks) && aligned(*vs))),
+                "pages and scales must be 16-byte aligned for the kernels");
   REFUSE_UNLESS(k.is_cuda(), "the kernels need CUDA tensors");
-  REFUSE_UNLESS(aligned(k) && aligned(v), "pages must be 16-byte aligned");
   REFUSE_UNLESS(status.device() == k.device(), "status word on another device");
   c.k = k.data_ptr();
   c.v = v.data_ptr();

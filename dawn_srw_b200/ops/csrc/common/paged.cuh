@@ -36,6 +36,8 @@ inline bool bad_cache(const DsbPaged* c) {
   if (c->N > kMostPositions || static_cast<long long>(c->width) * c->page > kMostPositions) return true;
   if (c->starts == nullptr && c->N != c->B) return true;
   if (c->kind != kBf16 && c->n_pages > 0 && (c->k_scale == nullptr || c->v_scale == nullptr)) return true;
+  // scales are copied four at a time
+  if (c->kind != kBf16 && ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15) != 0) return true;
   return ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) != 0;
 }
 

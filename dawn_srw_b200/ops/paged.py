@@ -33,8 +33,8 @@ def _refuse_unless(ok: bool, msg: str) -> None:
 
 
 def check_cache(k_pages, v_pages, table, lengths, starts, k_scale, v_scale, rows: int) -> None:
-    """What the kernels' bindings check too, but for the head dimensions and sizes (more than 65535 sequences or
-    heads, 2^30 rows or positions) that only they cannot take."""
+    """What the kernels' bindings check too, but for the head dimensions, sizes (more than 65535 sequences or
+    heads, 2^30 rows or positions) and pages or scales off a 16-byte border that only they cannot take."""
     _refuse_unless(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype,
                    "k and v pages must have one shape [n_pages, heads, page, dim] and one type")
     _refuse_unless(k_pages.is_contiguous() and v_pages.is_contiguous(), "pages must be contiguous")
