@@ -14,7 +14,8 @@ extern "C" {
 //   starts [B + 1] or null: rows starts[b] .. starts[b + 1] of the N packed rows are the last tokens of
 //   sequence b (null: row b is the last token of sequence b, N == B).  starts ascends; no two rows that are written
 //   in one call have one place.
-// Page size: a power of two, 16 .. 256; dh a multiple of 16, at most 128; everything 16-byte aligned.
+// Page size: a power of two, 16 .. 256; dh a multiple of 16, at most 128; everything 16-byte aligned, the
+// attention's result 32-byte.
 // A length above width * page or a page outside the pool sets *status to 4; what it names counts as absent.
 struct DsbPaged {
   void* k;

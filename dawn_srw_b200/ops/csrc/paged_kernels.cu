@@ -247,7 +247,7 @@ extern "C" int dsb_paged_write(const DsbPaged* c, const void* k, const void* v, 
 }
 
 extern "C" int dsb_paged_read(const DsbPaged* c, void* k, void* v, int dst_bf16, int max_len, cudaStream_t stream) {
-  if (bad_cache(c) || max_len < 0) return 934;
+  if (bad_cache(c) || max_len < 0 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) return 934;
   if (c->B == 0 || max_len == 0) return 0;
   const View w = make_view(c);
 #define DSB_KIND(K) (dst_bf16 ? launch_read<K, true>(w, k, v, max_len, stream) : launch_read<K, false>(w, k, v, max_len, stream))
@@ -281,6 +281,8 @@ extern "C" int dsb_paged_attention(const DsbPaged* c, const void* q, long long q
   if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_st % 8 || q_sh % 8 || c->H > 65535 || c->B > 65535 ||
       static_cast<long long>(c->N) * (Hq / c->H) > kMostPositions)
     return 941;
+  // results leave in words of 32 bytes, pieces come and go in words of 16
+  if ((reinterpret_cast<uintptr_t>(out) & 31) != 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return 941;
   if (c->N == 0) return 0;
   if (c->B == 0) {
     const size_t bytes = static_cast<size_t>(c->N) * Hq * c->dh * sizeof(__nv_bfloat16);

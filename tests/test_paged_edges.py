@@ -61,3 +61,14 @@ def c_calls(c, out=4096):
 @pytest.mark.parametrize("what", ["k", "v", "k_scale", "v_scale"])
 def test_c_entry_points_refuse_addresses_off_a_border(what):
     assert c_calls(c_view(**{what: 4100})) == {"write": 930, "read": 934, "attention": 940}
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what is not refused would be launched")
+def test_c_entry_points_refuse_results_off_a_border():
+    """Reading back stores words of 16 bytes, the attention of 32; a result on a border gets as far as the launch, or
+    the want of a workspace."""
+    c = c_view()
+    assert c_calls(c, out=4100)["read"] == 934 and c_calls(c, out=4104)["read"] == 934
+    assert c_calls(c, out=4100)["attention"] == 941 and c_calls(c, out=4096 + 16)["attention"] == 941
+    assert c_calls(c, out=4096 + 16)["read"] == 936
+    assert c_calls(c)["attention"] not in (0, 940, 941)
