@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
   const AttnParams& p = cp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dh = p.w.c.dh, ksteps = dh >> 4;
   // a scale's sign goes to the queries, so that the largest product has the largest score; a scale of zero, which would
-  // turn the -inf of hidden scores into NaN, into queries of zero
+  // turn the -inf of hidden scores into NaN, into queries of zero (a factor of the scores that underflows, of small
+  // queries and small keys, is kept at 2^-126: products are below 2^25, so that their scores are 0 all the same)
   const bool as_is = !kF16 && p.scale_log2 > 0.f;      // queries as they are in memory
 
   if (threadIdx.x == 0) {
@@ -824,6 +825,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         for (int c = 0; c < kParts; ++c) {
           const float* e = reinterpret_cast<const float*>(smem + L::kExp) + st * 8 + c;
           fc[c] = kF16 ? f * e[0] : f;
+          fc[c] = fc[c] < kLeastScale ? kLeastScale : fc[c];     // 0 would make NaN of a hidden score; NaN stays
           ev[c] = kF16 ? e[4] : 0.f;
         }
         // what a row does not see is -inf and weighs nothing: in TMEM, so that the tiles in between, most of them, have
