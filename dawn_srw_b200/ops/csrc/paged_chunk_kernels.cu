@@ -166,10 +166,22 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// The largest, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // 2^x for two x below 100 on the FMA units: the exponential unit, a sixteenth of a lane per cycle, is what the softmax
 // waits for, so it makes only some of them.  Cody and Waite's reduction to n + f, f in [-1/2, 1/2], and a polynomial in
 // f of degree 4 with value 1 at 0, fitted here to the least relative error (3e-6); n goes into the exponent's bits.
-// Below -127, and at -inf, the result is 0.
+// Below -127, and at -inf, the result is 0; at NaN it is some number.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   x.x = fmaxf(x.x, -127.f);
   x.y = fmaxf(x.y, -127.f);
@@ -860,15 +872,18 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const float* y = keep + 32 * c;
-            float t0 = fmaxf(y[0], y[1]), t1 = fmaxf(y[2], y[3]);
+            float t0 = max_nan(y[0], y[1]), t1 = max_nan(y[2], y[3]);
 #pragma unroll
             for (int k = 4; k < 32; k += 4) {
-              t0 = fmaxf(fmaxf(t0, y[k]), y[k + 1]);
-              t1 = fmaxf(fmaxf(t1, y[k + 2]), y[k + 3]);
+              t0 = max_nan(t0, y[k], y[k + 1]);
+              t1 = max_nan(t1, y[k + 2], y[k + 3]);
             }
-            top = fmaxf(top, fmaf(fmaxf(t0, t1), fc[2 * h + c], ev[2 * h + c]));       // fc >= 0
+            top = max_nan(top, fmaf(max_nan(t0, t1), fc[2 * h + c], ev[2 * h + c]));   // fc >= 0
           }
         }
+        // a score that is NaN, or inf, less itself NaN too: the row's result is. It goes by the maximum, since exp2_poly
+        // does not hand on NaN
+        top = top < INFINITY ? top : __uint_as_float(0x7fc00000u);
         // O complete up to the tile before, and the columns of a P of its own free
         auto o_ready = [&]() {
           ok = __all_sync(0xffffffffu, o_wait(ns - 1));
@@ -880,12 +895,12 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         if (j == 0) {
           m = top;
-        } else if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        } else if (__any_sync(0xffffffffu, !(top <= m + kSlack))) {
           if (kAlias) {
             o_ready();
             if (!ok) break;
           }
-          const float m_new = fmaxf(m, top), d = exp2_fast(m - m_new);
+          const float m_new = max_nan(m, top), d = exp2_fast(m - m_new);
           for (int c = 0; c < ksteps; ++c) {
             float o[16];
             tmem_ld16_now(o_at + 16 * c, o);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dawn_srw_b200.ops import paged as P
-from paged_helpers import KINDS, args, assert_attention, attention64, make_cache, scales, starts_of
+from paged_helpers import KINDS, args, assert_attention, attention64, held64, make_cache, scales, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -37,6 +37,40 @@ def _run(be, c, q, new, **kw):
     return be.paged_attention(q, *args(c), starts, **scales(c), **kw)
 
 
+def smallest_weights(q, c, new, window=None, sinks=0):
+    """What the fp16 weights of 8-bit pages may add to a result.  A weight goes to fp16 as p_j S_j, S_j being the power
+    of two next to (in a chunk: at) the largest scale of the values among 32 positions, p_j the softmax; the
+    row's largest, W, stands at 2^6 or more.  A weight below fp16's normal numbers is off by half of its smallest step,
+    2^-25, which is 2^-31 W: by sum_j 2^-31 W |v_j| / S_j in all, and S_j is more than half of the scale of j."""
+    out = torch.zeros(q.shape, dtype=torch.double, device=q.device)
+    if c["v_scale"] is None:
+        return out
+    H, G = c["k_pages"].shape[1], q.shape[1] // c["k_pages"].shape[1]
+    at = 0
+    for b, n in enumerate(new):
+        length = int(c["lengths"][b])
+        k, v = held64(c, b, length, "k"), held64(c, b, length, "v")
+        pos = torch.arange(length, device=q.device)
+        ids = c["table"][b].long()[pos // c["k_pages"].shape[2]]
+        s = c["v_scale"][ids, :, pos % c["k_pages"].shape[2]].double()              # [length, H]
+        s = torch.where((v == 0).all(-1) | ~s.isfinite(), torch.zeros_like(s), s)
+        group = torch.zeros_like(s)
+        for x in range(0, length, 32):
+            top, least = s[x: x + 32].amax(0), torch.where(s > 0, s, torch.full_like(s, math.inf))[x: x + 32].amin(0)
+            group[x: x + 32] = torch.where(top <= 2.0 ** 15 * least, top, s[x: x + 32])
+        codes = torch.where(s[..., None] > 0, v.abs() / s[..., None], torch.zeros_like(v)).nan_to_num(0.0)
+        for i in range(n):
+            p = length - n + i
+            j = torch.arange(p + 1, device=q.device)
+            if window is not None:
+                j = j[(j > p - window) | (j < sinks)]
+            a = torch.einsum("hgd,nhd->hgn", q[at + i].double().view(H, G, -1), k[j]) / math.sqrt(q.shape[2])
+            most = (torch.softmax(a, -1) * group[j].T[:, None]).amax(-1)                # [H, G]
+            out[at + i] = (2.0 ** -30 * most[..., None] * codes[j].sum(0)[:, None]).reshape(q.shape[1:])
+        at += n
+    return out.nan_to_num(0.0)
+
+
 def _compare(cb, be, c, q, new, window=None, sinks=0, nan_rows=False):
     """Finite results as the definition has them, the others where it has them and of the same kind; with ``nan_rows``
     a row with one that is not finite is NaN throughout."""
@@ -49,6 +83,7 @@ def _compare(cb, be, c, q, new, window=None, sinks=0, nan_rows=False):
     assert torch.equal(got.isnan(), ref.isnan())
     assert torch.equal(got[~fine].nan_to_num(0.0).double(), ref[~fine].bfloat16().nan_to_num(0.0).double())
     zero = torch.zeros_like
+    mag = mag + 2.0 ** 8 * smallest_weights(q, c, new, window, sinks)                   # assert_attention takes 2^-8 of it
     assert_attention(torch.where(fine, got, zero(got)), torch.where(fine, ref, zero(ref)), torch.where(fine, mag, zero(mag)))
     cb.check_status()
     return ref
@@ -66,3 +101,24 @@ def test_small_queries_and_keys(cb, be, kind, dh, q_mag, k_mag, window, sinks):
         q = _rand(sum(new), 4, dh, seed=3) * 2.0 ** q_mag
         ref = _compare(cb, be, c, q, new, window, sinks)
         assert bool(ref.isfinite().all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dh", [64, 80, 128])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+@pytest.mark.parametrize("at", [0, 5, 6, 31, 37, 64, 69, 100])
+def test_a_key_that_is_no_number(cb, be, kind, dh, odd, at):
+    """NaN for the rows that see it, wherever it stands in a tile, and nothing for those that do not."""
+    for lengths, new, window in (([220, 40], [180, 40], None), ([220, 40], [180, 40], 60), ([104, 40], [5, 3], None),
+                                 ([220, 40], [1, 1], None), ([220, 40], [1, 1], 30)):
+        c = make_cache(kind, lengths, 2, dh, 16, "cuda", seed=at)
+        page, slot = _at(c, 0, at)
+        if kind == "bf16":
+            c["k_pages"][page, 0, slot, 0] = odd
+        else:                                                    # as a row with such a value is stored
+            c["k_scale"][page, 0, slot] = math.nan
+        q = _rand(sum(new), 4, dh, seed=at + 1)
+        q[..., 0] = q[..., 0].abs() + 0.1
+        ref = _compare(cb, be, c, q, new, window, 0, nan_rows=True)
+        sees = torch.tensor([p >= at and (window is None or at > p - window) for p in range(lengths[0] - new[0], lengths[0])])
+        assert torch.equal(ref[: new[0], 0, 0].isnan().cpu(), sees)
