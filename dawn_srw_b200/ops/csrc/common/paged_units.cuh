@@ -11,7 +11,8 @@
 namespace dsb {
 namespace paged {
 
-constexpr float kFloor = -3.0e38f;               // below every score
+// A row's maximum: kFloor before it has seen a position, kSeen at least after it; scores at or below kSeen weigh nothing.
+constexpr float kFloor = -3.40282347e38f, kSeen = -3.39e38f;
 constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -23,6 +24,11 @@ __device__ __forceinline__ float log2_fast(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// What a row's result is multiplied with. No weight: zero for a row that sees nothing, NaN (nothing over nothing) for one
+// whose scores are all -inf.
+__device__ __forceinline__ float over_sum(float sum, float top) {
+  return sum != 0.f ? 1.f / sum : top > kFloor ? __uint_as_float(0x7fc00000u) : 0.f;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_few_kernel(const At
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     if (lane == 0) {
       s_top[r] = top;
-      s_inv[r] = sum == 0.f ? 0.f : 1.f / sum;
+      s_inv[r] = over_sum(sum, top);
     }
   }
   const int tasks = u.rows * per;                      // float4s of the unit

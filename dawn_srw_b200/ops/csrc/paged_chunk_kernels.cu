@@ -842,12 +842,17 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         }
         // what a row does not see is -inf and weighs nothing: in TMEM, so that the tiles in between, most of them, have
         // nothing to do with it
+        float top = kSeen;
         if (hidden) {
+          bool any = false;
 #pragma unroll 1
           for (int c = 0; c < TP / 16; ++c) {
             const int x = x0 + 16 * c;                 // sixteen columns: most are seen, or not, by all rows of a warp
             const uint32_t away = gone >> (8 * (c >> 1) + (c & 1)) & 1u;
-            if (away == 0u && x + 15 <= pos_lo && (x > pos_hi - p.window || x + 15 < p.sinks)) continue;
+            if (away == 0u && x + 15 <= pos_lo && (x > pos_hi - p.window || x + 15 < p.sinks)) {
+              any = true;
+              continue;
+            }
             uint32_t w[16];
             if (away != 0u || x > pos_hi || (x + 15 <= pos_lo - p.window && x >= p.sinks)) {
 #pragma unroll
@@ -856,6 +861,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
               float y[16];
               tmem_ld16_now(s_at + 16 * c, y);
               const uint32_t seen = seen32(x, pos, p.window, p.sinks);
+              any = any || (seen & 0xffffu) != 0u;
 #pragma unroll
               for (int k = 0; k < 16; ++k) w[k] = (seen >> k) & 1u ? __float_as_uint(y[k]) : 0xff800000u;
             }
@@ -863,9 +869,9 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           }
           tmem_st_wait();
           if (kKeep) tmem_ld64_now(s_at, keep);
+          top = any ? kSeen : kFloor;
         }
         // a row of 64 stays in registers where they suffice; two passes over S elsewhere
-        float top = kFloor;
 #pragma unroll
         for (int h = 0; h < TP / 64; ++h) {
           if (!kKeep) tmem_ld64_now(s_at + 64 * h, keep);
@@ -957,7 +963,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       if (!ok) break;
       // every S of the unit is done: its queries make room for the next ones
       const bool whole = u.whole != 0;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = over_sum(l, m);
       float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + u.slot) * piece_floats<kUnitRows>(dh);
       __nv_bfloat16* dst = real ? out_row(p, u.first, u.h, r) : nullptr;
       have = plans.next(u, lane);
@@ -1038,7 +1044,7 @@ __global__ void __launch_bounds__(256) paged_merge_chunk_kernel(const AttnParams
       a[4 * k + 3] = fmaf(a[4 * k + 3], x, w * o[k].w);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = over_sum(sum, top);
   uint32_t w[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) w[k] = pack_bf16x2(a[2 * k] * inv, a[2 * k + 1] * inv);

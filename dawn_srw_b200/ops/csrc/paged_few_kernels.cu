@@ -312,7 +312,6 @@ struct Warp {
       uint32_t pt[NT][kMT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top[2] = {kFloor, kFloor};
         uint32_t vis = 0xffffffffu;
         if (!open) {
           vis = 0;
@@ -325,6 +324,7 @@ struct Warp {
               vis |= static_cast<uint32_t>(on) << (4 * mt + c);
             }
         }
+        float top[2] = {vis & 0x55555555u ? kSeen : kFloor, vis & 0xaaaaaaaau ? kSeen : kFloor};
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(cons
           s_all[r][1] = sum;
         }
       } else {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = over_sum(sum, top);
         *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
             make_uint2(pack_bf16x2(f.x * inv, f.y * inv), pack_bf16x2(f.z * inv, f.w * inv));
       }
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(cons
           f.z = fmaf(x, v.z, f.z);
           f.w = fmaf(x, v.w, f.w);
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = over_sum(sum, top);
         *reinterpret_cast<uint2*>(out_row(p, u, u.rt * W::kRows + r) + c) =
             make_uint2(pack_bf16x2(f.x * inv, f.y * inv), pack_bf16x2(f.z * inv, f.w * inv));
       }
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * nt + 2 * t + e;
         if (r >= u.rows) continue;
-        const float inv = s.l[nt][e] == 0.f ? 0.f : 1.f / s.l[nt][e];
+        const float inv = over_sum(s.l[nt][e], s.m[nt][e]);
         if (!seg.whole() && g == 0) *reinterpret_cast<float2*>(piece + 2 * r) = make_float2(s.m[nt][e], s.l[nt][e]);
         float* row = piece + 2 * W::kRows + r * dh;
         __nv_bfloat16* dst = out_row(p, u, u.rt * W::kRows + r);

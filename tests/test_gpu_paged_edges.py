@@ -122,3 +122,17 @@ def test_a_key_that_is_no_number(cb, be, kind, dh, odd, at):
         ref = _compare(cb, be, c, q, new, window, 0, nan_rows=True)
         sees = torch.tensor([p >= at and (window is None or at > p - window) for p in range(lengths[0] - new[0], lengths[0])])
         assert torch.equal(ref[: new[0], 0, 0].isnan().cpu(), sees)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("lengths,new,window", [([1, 30], [1, 1], None), ([1, 9], [1, 9], None), ([40, 300], [40, 300], None),
+                                                ([40, 300], [40, 300], 1), ([4, 300], [4, 290], 3), ([40, 20], [3, 1], 2)])
+def test_rows_that_see_only_scores_of_minus_infinity(cb, be, dh, lengths, new, window):
+    """Nothing over nothing: NaN by the definition, unlike a row that sees no key."""
+    c = make_cache("bf16", lengths, 2, dh, 16, "cuda")
+    for b, pos in ((0, 0), (0, lengths[0] - 1), (1, 0), (1, lengths[1] - 1)):
+        page, slot = _at(c, b, pos)
+        c["k_pages"][page, 0, slot, 3] = -math.inf
+    q = _rand(sum(new), 4, dh, seed=2)
+    q[..., 3] = q[..., 3].abs() + 0.1
+    _compare(cb, be, c, q, new, window, nan_rows=True)
