@@ -30,6 +30,17 @@ __device__ __forceinline__ float log2_fast(float x) {
 __device__ __forceinline__ float over_sum(float sum, float top) {
   return sum != 0.f ? 1.f / sum : top > kFloor ? __uint_as_float(0x7fc00000u) : 0.f;
 }
+// The largest, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -319,6 +330,137 @@ struct Segments {
     t1 = static_cast<int>(min(static_cast<long long>(u.tiles), end - at));
   }
 };
+
+// ---- Units computed again.  Products of whole tiles hand a value that is no number on to rows that do not see it: a weight
+// of zero times NaN or inf is NaN.  It shows in an O that is not finite beside a finite sum of weights; then the positions
+// that only some of the unit's rows see are looked through, and if one holds such a value the work is done again row by row,
+// position by position, without touching what a row does not see.  Hundreds of times slower, and for diverged caches alone.
+
+// NaN if x, or a term before it, is not finite.
+__device__ __forceinline__ float track_odd(float odd, float x) { return fmaf(x, 0.f, odd); }
+
+template <int KIND>
+__device__ __forceinline__ bool odd_codes(uint32_t x) {
+  return KIND == kBf16 ? (((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u) != 0u      // exponents of ones carry
+                       : (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;     // e4m3: and fractions
+}
+
+// Does a position that only some of the unit's rows see hold a value that is no number?  Threads `who` of `of`.
+template <int KIND>
+__device__ __noinline__ bool odd_values(const AttnParams& p, const Unit u, int who, int of) {
+  if (KIND == kInt8) return false;
+  const int words = p.w.c.dh * (KIND == kBf16 ? 2 : 1) >> 4;
+  const int early = min(u.lo_all, u.hi) - u.lo, late = max(u.hi_all, u.lo);        // [lo, lo_all), [hi_all, hi)
+  const long long n = static_cast<long long>(max(early, 0) + max(u.hi - late, 0)) * words;
+  for (long long i = who; i < n; i += of) {
+    const int x = static_cast<int>(i / words), word = static_cast<int>(i % words);
+    const int pos = x < early ? u.lo + x : late + x - max(early, 0), page = page_of(p.w, u.b, pos);
+    if (page < 0) continue;
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.w.c.v) +
+                                                         slot_row(p.w, page, u.h, pos) * (16 * words)) + word);
+    if (odd_codes<KIND>(v.x) || odd_codes<KIND>(v.y) || odd_codes<KIND>(v.z) || odd_codes<KIND>(v.w)) return true;
+  }
+  return false;
+}
+
+// Eight values from element `at` of a pool on, without their scale.
+template <int KIND>
+__device__ __forceinline__ void held8(const void* pool, size_t at, float* f) {
+  if (KIND == kBf16) {
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(pool) + at)), f);
+    return;
+  }
+  const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at));
+  const uint2 a = codes_to_f16<KIND, false>(x.x), c = codes_to_f16<KIND, false>(x.y);
+  const uint32_t h[4] = {a.x, a.y, c.x, c.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(h + i));
+    f[2 * i] = y.x;
+    f[2 * i + 1] = y.y;
+  }
+}
+
+// Rows r0, r0 + r_step, .. of a unit over its tiles t0, t0 + step, .. below t1, by a warp, in fp32.  ml null: the results, in
+// bf16.  Otherwise maximum and sum of row r at ml + 2 r, its columns 4 c .. at o + r * row_stride + c * col_stride, sum and O
+// times `up`.
+template <int KIND, int ROWS, int TP>
+__device__ __noinline__ void rows_again(const AttnParams& p, const Unit u, int t0, int t1, int step, int r0, int r_step,
+                                        int lane, float* ml, float* to, int row_stride, int col_stride, float up) {
+  const int dh = p.w.c.dh, half = lane >> 4, col = 8 * (lane & 15);
+  for (int r = r0; r < u.rows; r += r_step) {
+    const int row = u.rt * ROWS + r, t = p.by_g(row), pos = u.len - u.n + t;
+    const __nv_bfloat16* q = p.q + static_cast<long long>(u.first + t) * p.q_st + static_cast<long long>(u.h * p.G + row - t * p.G) * p.q_sh;
+    float m = kFloor, l = 0.f, o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    for (int tile = t0; tile < t1; tile += step)
+      for (int x0 = (tile < u.st ? tile : tile + u.skip) * TP, x1 = x0 + TP; x0 < x1; x0 += 32) {
+        const int j = x0 + lane;
+        const int page = j < x1 && j <= pos && (j > pos - p.window || j < p.sinks) ? page_of(p.w, u.b, j) : -1;
+        const bool on = page >= 0;
+        const unsigned seen = __ballot_sync(0xffffffffu, on);
+        if (seen == 0u) continue;
+        const size_t at = on ? slot_row(p.w, page, u.h, j) : 0;
+        float s = 0.f, vs = 1.f;
+        if (on) {
+          for (int c = 0; c < dh; c += 8) {
+            float a[8], k[8];
+            bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(q + c)), a);
+            held8<KIND>(p.w.c.k, at * dh + c, k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(a[e], k[e], s);
+          }
+          if (KIND != kBf16) {
+            s *= __ldg(p.w.c.k_scale + at);
+            vs = __ldg(p.w.c.v_scale + at);
+          }
+          s *= p.scale_log2;
+        }
+        float top = on ? max_nan(s, kSeen) : kFloor;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float m_new = max_nan(m, top), d = exp2_fast(m - m_new), w = on ? exp2_fast(s - m_new) : 0.f;
+        l = fmaf(l, d, w);
+        m = m_new;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] *= d;
+        for (int k = 0; k < 32; k += 2) {              // half a warp a position
+          const int from = k + half;
+          const float y = __shfl_sync(0xffffffffu, w, from), z = __shfl_sync(0xffffffffu, vs, from);
+          const unsigned long long at_k = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
+          if (((seen >> from) & 1u) && col < dh) {
+            float v[8];
+            held8<KIND>(p.w.c.v, at_k * dh + col, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(y, v[e] * z, o[e]);
+          }
+        }
+      }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] += __shfl_xor_sync(0xffffffffu, o[k], 16);
+    if (half != 0 || col >= dh) continue;
+    if (ml == nullptr) {
+      const float inv = over_sum(l, m);
+      *reinterpret_cast<uint4*>(out_row(p, u, row) + col) =
+          make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                     pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
+    } else {
+      if (lane == 0) {
+        ml[2 * r] = m;
+        ml[2 * r + 1] = l * up;
+      }
+      float* x = to + static_cast<size_t>(r) * row_stride + static_cast<size_t>(col / 4) * col_stride;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = o[k] * up;
+        x[col_stride + k] = o[4 + k] * up;
+      }
+    }
+  }
+}
 
 constexpr int kMergeThreads = 256;
 constexpr int kMergeChunk = 64;        // pieces whose weights are at hand at a time

@@ -10,9 +10,10 @@
 // read: K-major for K, MN-major for V.  8-bit codes are read by four warps and go to the same layout as fp16 numbers,
 // code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: exact for e4m3, whose scales
 // are powers of two, and rounded once, by 2^-11 at most, for int8 (as a weight is, and far below the codes' own
-// rounding; a scale per column in the softmax would cost each thread three shared-memory reads per column).  2^e of the keys goes to the scores, 2^e of the values, as in
-// the few-row kernel, to the exponents and out of the sum.  Rows of V that no query row sees are zeros, whatever the
-// page holds there; a scale that is no number makes the scores of its position NaN.
+// rounding; a scale per column in the softmax would cost each thread three shared-memory reads per column).  2^e of the
+// keys goes to the scores, 2^e of the values, as in the few-row kernel, to the exponents and out of the sum.  Rows of V that
+// no query row sees are zeros, whatever the page holds there; a scale that is no number makes the scores of its position
+// NaN; a value that is none, seen by some rows of a unit alone, has the block's work done again (rows_again).
 //
 // The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
@@ -166,18 +167,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// The largest, NaN if one is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // 2^x for two x below 100 on the FMA units: the exponential unit, a sixteenth of a lane per cycle, is what the softmax
 // waits for, so it makes only some of them.  Cody and Waite's reduction to n + f, f in [-1/2, 1/2], and a polynomial in
 // f of degree 4 with value 1 at 0, fitted here to the least relative error (3e-6); n goes into the exponent's bits.
@@ -316,6 +305,7 @@ struct Bars {
   uint64_t plan_empty[kPlans];  // every warp that works by the plan has read it
   uint32_t tmem;
   int abort;
+  int again;                // an O is not finite although the sum of its weights is
   uint32_t absent[2 * S];   // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
 };
 
@@ -338,6 +328,20 @@ struct Plans {
     return q.b >= 0;
   }
 };
+
+// A block's segments again, where that is called for.
+template <int KIND, int TP>
+__device__ __noinline__ void segments_again(const AttnParams& p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Segments<kUnitRows, TP> seg;
+  for (seg.begin(p, lane, blockIdx.x, kLeast * 128 / TP); seg.on(); seg.next(p)) {
+    if (!__syncthreads_or(odd_values<KIND>(p, seg.u, threadIdx.x, kThreadsOf<KIND>))) continue;
+    float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + seg.slot()) * piece_floats<kUnitRows>(p.w.c.dh);
+    // the kernel's fp16 weights are 2^6 times the others
+    rows_again<KIND, kUnitRows, TP>(p, seg.u, seg.t0, seg.t1, 1, warp, kThreadsOf<KIND> / 32, lane, seg.whole() ? nullptr : piece,
+                                    piece + 2 * kUnitRows, 4, 4 * kUnitRows, KIND == kBf16 ? 1.f : 64.f);
+  }
+}
 
 template <int KIND, int NA>
 __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams cp) {
@@ -386,6 +390,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.plan_empty[i], kF16 ? 14 : 11);      // softmax, MMA, and TMA or loaders
     }
     b.abort = 0;
+    b.again = 0;
     fence_barrier_init();
     if (!kF16) {
       tma_prefetch_desc(&cp.k);
@@ -975,6 +980,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       }
       if (real && !whole) reinterpret_cast<float2*>(piece)[ru] = make_float2(m, l);
       float4* to = reinterpret_cast<float4*>(piece + 2 * kUnitRows) + ru;
+      float odd = 0.f;
       for (int c = 0; c < ksteps; ++c) {
         float o[16];
         if (mine > 0) {
@@ -984,6 +990,10 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           for (int k = 0; k < 16; ++k) o[k] = 0.f;
         }
         if (!real) continue;
+        if (KIND != kInt8) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) odd = track_odd(odd, o[k]);
+        }
         if (whole) {
           uint32_t w[8];
 #pragma unroll
@@ -995,6 +1005,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
             to[(4 * c + k) * kUnitRows] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
       }
+      if (odd != odd && l < INFINITY) *static_cast<volatile int*>(&b.again) = 1;
       tc_fence_before();                           // O has been read: the next unit's P may follow
     }
   }
@@ -1011,6 +1022,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (KIND != kInt8 && *static_cast<volatile int*>(&b.again) && *abort_flag == 0) segments_again<KIND, TP>(p);
 }
 
 // What several blocks left of a unit, in order: a block takes 32 rows, a lane per row, a warp per sixteen columns.

@@ -408,6 +408,25 @@ struct Warp {
   }
 };
 
+// All lanes of a warp: an O is not finite although the sum of its weights is, and the unit's rows see different positions,
+// one of which holds a value that is no number.
+template <int KIND, int KD, int NT>
+__device__ __forceinline__ bool work_again(const AttnParams& p, const Warp<KIND, KD, NT>& s, const Unit& u, int lane) {
+  if (KIND == kInt8 || (u.lo == u.lo_all && u.hi == u.hi_all)) return false;            // single tokens
+  bool odd = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = 0.f;
+#pragma unroll
+      for (int c = 0; c < KD; ++c) x = track_odd(track_odd(x, s.o[nt][c][e]), s.o[nt][c][2 + e]);
+      odd = odd || (x != x && s.l[nt][e] < INFINITY);
+    }
+  return __any_sync(0xffffffffu, odd) && __any_sync(0xffffffffu, odd_values<KIND>(p, u, lane, 32));
+}
+template <int KIND> constexpr float kUp = KIND == kBf16 ? 1.f : 16384.f;   // weights here are 2^14 times those of rows_again
+
 constexpr int kMostWarps = 12;          // of a block: what fits an SM
 
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
@@ -419,7 +438,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 // A cluster of blocks per unit, every warp every n-th tile: grid (blocks of a cluster x row tiles, heads, sequences);
 // more row tiles than the grid has are taken in turn.
 template <int KIND, int KD, int NT>
-__global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(const AttnParams p, int blocks) {
+__global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(const __grid_constant__ AttnParams p, int blocks) {
   using W = Warp<KIND, KD, NT>;
   static_assert(2 * W::kRows * (16 * KD + 4) * 4 <= W::R::kBytes, "two O fit a warp's ring");
   extern __shared__ __align__(128) unsigned char smem[];
@@ -458,6 +477,10 @@ __global__ void __launch_bounds__(32 * kMostWarps, 1) paged_few_unit_kernel(cons
           s_ml[warp][r][1] = s.l[nt][e];
         }
       }
+    if (work_again(p, s, u, lane)) {
+      __syncwarp();
+      rows_again<KIND, W::kRows, W::kTP>(p, u, rank * warps + warp, u.tiles, blocks * warps, 0, 1, lane, &s_ml[warp][0][0], mine, ld, 4, kUp<KIND>);
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < u.rows * per; i += blockDim.x) {
       const int r = i / per, c = 4 * (i - r * per);
@@ -517,7 +540,7 @@ constexpr int kLeastTiles = 8;
 
 // Equal runs of tiles for every warp.
 template <int KIND, int KD, int NT>
-__global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const __grid_constant__ AttnParams p) {
   using W = Warp<KIND, KD, NT>;
   extern __shared__ __align__(128) unsigned char smem[];
   const uint32_t ring = smem_u32(smem) + (threadIdx.x >> 5) * W::R::kBytes;
@@ -555,6 +578,10 @@ __global__ void __launch_bounds__(32 * kWarps, 3) paged_few_run_kernel(const Att
             }
           }
       }
+    if (work_again(p, s, u, lane)) {
+      __syncwarp();
+      rows_again<KIND, W::kRows, W::kTP>(p, u, seg.t0, seg.t1, 1, 0, 1, lane, seg.whole() ? nullptr : piece, piece + 2 * W::kRows, dh, 4, kUp<KIND>);
+    }
   }
   if (lane == 0) p.meta[worker] = meta;
 }

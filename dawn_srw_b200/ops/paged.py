@@ -210,5 +210,11 @@ def attention(q, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_
         s = torch.einsum("hrgd,hnd->hrgn", rows, kv[0]) * scale
         s = s.masked_fill(~sees[None, :, None], -math.inf)
         w = torch.softmax(s, -1)
-        out[mine] = torch.einsum("hrgn,hnd->hrgd", w, kv[1]).transpose(0, 1).reshape(len(p), Hq, -1)
+        # a weight of zero does not keep a value that is no number away from a row that does not see it
+        odd = ~torch.isfinite(kv[1])
+        o = torch.einsum("hrgn,hnd->hrgd", w, torch.where(odd, 0.0, kv[1]))
+        for j in odd.any(-1).any(0).nonzero().flatten().tolist():
+            part = w[..., j, None] * kv[1][:, None, None, j]
+            o += torch.where(odd[:, None, None, j] & sees[None, :, None, j, None], part, 0.0)
+        out[mine] = o.transpose(0, 1).reshape(len(p), Hq, -1)
     return out.to(q.dtype)

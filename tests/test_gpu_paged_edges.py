@@ -136,3 +136,40 @@ def test_rows_that_see_only_scores_of_minus_infinity(cb, be, dh, lengths, new, w
     q = _rand(sum(new), 4, dh, seed=2)
     q[..., 3] = q[..., 3].abs() + 0.1
     _compare(cb, be, c, q, new, window, nan_rows=True)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dh", [64, 80, 128])
+@pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 0), (70, 20)])
+def test_a_value_that_is_no_number(cb, be, kind, dh, odd, window, sinks):
+    """It reaches the rows that see it, in its column, and no other."""
+    for lengths, new, at in (([220, 40], [180, 40], 100), ([220, 40], [180, 40], 10), ([600, 40], [500, 30], 333),
+                             ([104, 40], [5, 3], 102), ([105, 40], [9, 3], 40), ([300, 40], [8, 3], 256)):
+        c = make_cache(kind, lengths, 2, dh, 16, "cuda", seed=at)
+        page, slot = _at(c, 0, at)
+        if kind == "bf16":
+            c["v_pages"][page, 0, slot, 7] = odd
+        else:
+            c["v_pages"].view(torch.uint8)[page, 0, slot, 7] = 0x7f if odd > 0 or odd != odd else 0xff     # both are NaN
+        q = _rand(sum(new), 4, dh, seed=at + 1)
+        ref = _compare(cb, be, c, q, new, window, sinks)
+        bad = (~ref.isfinite()).nonzero()
+        assert bool((bad[:, 2] == 7).all()) and bool((bad[:, 1] < 2).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20000, 3)])
+def test_a_value_that_is_no_number_in_a_long_context(cb, be, kind, window, sinks):
+    """Drafted tokens whose warps take equal runs of all units, and leave pieces."""
+    lengths, new = [40000, 300, 7, 1000, 9, 70, 200, 1], [5, 3, 5, 1, 4, 0, 5, 1]
+    for at in (39997, 39999, 20000, 19998, 5):
+        c = make_cache(kind, lengths, 8, 64, 64, "cuda", seed=at)
+        for b, pos in ((0, at), (2, 4)):
+            page, slot = _at(c, b, pos)
+            if kind == "bf16":
+                c["v_pages"][page, 0, slot, 7] = math.inf
+            else:
+                c["v_pages"].view(torch.uint8)[page, 0, slot, 7] = 0x7f
+        q = _rand(sum(new), 16, 64, seed=at + 1) * 0.2
+        _compare(cb, be, c, q, new, window, sinks)

@@ -1,13 +1,15 @@
 """Paged key/value cache at the edges of its range, on the CPU: alignment, and values that are no numbers."""
 import ctypes
+import math
 
 import pytest
 import torch
 
 from dawn_srw_b200.ops import build
+from dawn_srw_b200.ops.backend import ReferenceBackend
 from dawn_srw_b200.ops.cuda_backend import CudaBackend
 
-from paged_helpers import args, make_cache, scales
+from paged_helpers import args, attention64, make_cache, scales, starts_of
 
 CPU = torch.device("cpu")
 
@@ -72,3 +74,19 @@ def test_c_entry_points_refuse_results_off_a_border():
     assert c_calls(c, out=4100)["attention"] == 941 and c_calls(c, out=4096 + 16)["attention"] == 941
     assert c_calls(c, out=4096 + 16)["read"] == 936
     assert c_calls(c)["attention"] not in (0, 940, 941)
+
+
+@pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (4, 0), (5, 2)])
+def test_a_value_that_is_no_number_reaches_the_rows_that_see_it(odd, window, sinks):
+    """The plain path, fp32 throughout: 1e-5 of the sum of magnitudes."""
+    c = make_cache("bf16", [20, 5], 2, 16, 16, CPU)
+    c["v_pages"][int(c["table"][0, 0]), 1, 9, 3] = odd
+    new = [18, 5]
+    q = torch.randn(23, 4, 16, generator=torch.Generator().manual_seed(1))
+    got = ReferenceBackend().paged_attention(q, *args(c), starts_of(new, CPU), window=window, sinks=sinks)
+    ref, mag = attention64(q, c, new, window, sinks)
+    fine = ref.isfinite()
+    assert int((~fine).sum()) == 2 * (11 if window is None else window)              # two query heads of the group, a column
+    assert torch.equal(got.isfinite(), fine) and torch.equal(got[~fine].double().nan_to_num(), ref[~fine].float().double().nan_to_num())
+    assert bool(((got.double() - ref).abs() <= 1e-5 * mag + 1e-12)[fine].all())
