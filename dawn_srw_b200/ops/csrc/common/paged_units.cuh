@@ -84,6 +84,14 @@ inline Divisor make_divisor(int d) {
   return {static_cast<uint32_t>(((1ULL << (31 + s)) + d - 1) / d), 31 + s};
 }
 
+// Rows of zeros are stored under a scale of 1, which says nothing of their size: beside rows with small scales it would set
+// the measure that fp16 numbers are relative to. Where a scale of 1 is met the codes are looked at.
+constexpr float kZeroRow = 1.f;
+template <int KIND>
+__device__ __forceinline__ bool zero_codes(uint32_t x) { return (KIND == kE4m3 ? x & 0x7f7f7f7fu : x) == 0u; }
+template <int KIND>
+__device__ __forceinline__ bool zero_codes(const uint4& x) { return zero_codes<KIND>(x.x | x.y | x.z | x.w); }
+
 struct AttnParams {
   View w;
   const __nv_bfloat16* q;           // [N, Hq, dh], strides in elements

@@ -9,11 +9,14 @@
 // bf16 pages come by TMA, one box per page and 64 columns, into the 128-byte-swizzled tiles that the instructions
 // read: K-major for K, MN-major for V.  8-bit codes are read by four warps and go to the same layout as fp16 numbers,
 // code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: exact for e4m3, whose scales
-// are powers of two, and rounded once, by 2^-11 at most, for int8 (as a weight is, and far below the codes' own
-// rounding; a scale per column in the softmax would cost each thread three shared-memory reads per column).  2^e of the
-// keys goes to the scores, 2^e of the values, as in the few-row kernel, to the exponents and out of the sum.  Rows of V that
-// no query row sees are zeros, whatever the page holds there; a scale that is no number makes the scores of its position
-// NaN; a value that is none, seen by some rows of a unit alone, has the block's work done again (rows_again).
+// are powers of two and whose codes are multiples of 2^-9, and rounded once, by 2^-11 at most, for int8 (as a weight is,
+// and far below the codes' own rounding; a scale per column in the softmax would cost each thread three shared-memory
+// reads per column).  That is while no scale is smaller by more than 2^15: where one is, the block's work is done again
+// in fp32 (rows_again).  Rows of zeros have no part in it.  2^e of the keys goes to the scores, 2^e of the values, as in
+// the few-row kernel, to the exponents and out of the sum.
+//
+// Rows of V that no query row sees are zeros, whatever the page holds there; a scale that is no number makes the scores
+// of its position NaN; a value that is none, seen by some rows of a unit alone, has the block's work done again too.
 //
 // The blocks, one per SM, take equal runs of tiles of all units, so neither ragged lengths nor causal triangles leave
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
@@ -306,6 +309,7 @@ struct Bars {
   uint32_t tmem;
   int abort;
   int again;                // an O is not finite although the sum of its weights is
+  int apart;                // scales of 32 positions are too far apart for fp16 numbers
   uint32_t absent[2 * S];   // [kMeta] bits 8 w + i: no row sees sixteen positions 2 w + i, or they have no page
 };
 
@@ -329,13 +333,50 @@ struct Plans {
   }
 };
 
+// The scale that counts of a row's 8-bit codes: 0 of a row of zeros.
+template <int KIND>
+__device__ __forceinline__ float used_scale(float s, const void* pool, size_t row, int dh) {
+  if (s != kZeroRow) return s;
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + row * dh);
+  bool zero = true;
+  for (int c = 0; c < dh / 16; ++c) zero = zero && zero_codes<KIND>(__ldg(x + c));
+  return zero ? 0.f : s;
+}
+
+// Of a warp's scales: biased exponent of the largest finite one, that of 2^-107 at least, so that its products with a score's
+// factor do not vanish; `none` where there is none.  apart: this lane's is less by more than 2^15.
+__device__ __forceinline__ uint32_t largest_exponent(float x, uint32_t none, bool& apart) {
+  const uint32_t e = (__float_as_uint(x) >> 23) & 0xffu;
+  uint32_t most = __reduce_max_sync(0xffffffffu, e == 255u ? 0u : e);
+  if (most == 0u) return none;
+  most = max(most, 20u);
+  apart = apart || (e != 0u && most > e + 15u);
+  return most;
+}
+
+// Are scales of 32 positions of a segment too far apart?  Warp `warp` of `warps`.
+template <int KIND, int TP>
+__device__ __noinline__ bool scales_apart(const AttnParams& p, const Unit u, int t0, int t1, int warp, int warps, int lane) {
+  bool apart = false;
+  for (int i = warp; i < (t1 - t0) * (TP / 32); i += warps) {
+    const int tile = t0 + i / (TP / 32), x = (tile < u.st ? tile : tile + u.skip) * TP + i % (TP / 32) * 32 + lane;
+    const int page = x < u.hi && (x >= u.lo || x < u.s_end) ? page_of(p.w, u.b, x) : -1;
+    const size_t at = page >= 0 ? slot_row(p.w, page, u.h, x) : 0;
+    largest_exponent(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.k_scale + at), p.w.c.k, at, p.w.c.dh) : 0.f, 0u, apart);
+    largest_exponent(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.v_scale + at), p.w.c.v, at, p.w.c.dh) : 0.f, 0u, apart);
+  }
+  return apart;
+}
+
 // A block's segments again, where that is called for.
 template <int KIND, int TP>
 __device__ __noinline__ void segments_again(const AttnParams& p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Segments<kUnitRows, TP> seg;
   for (seg.begin(p, lane, blockIdx.x, kLeast * 128 / TP); seg.on(); seg.next(p)) {
-    if (!__syncthreads_or(odd_values<KIND>(p, seg.u, threadIdx.x, kThreadsOf<KIND>))) continue;
+    bool redo = odd_values<KIND>(p, seg.u, threadIdx.x, kThreadsOf<KIND>);
+    if (KIND != kBf16) redo = scales_apart<KIND, TP>(p, seg.u, seg.t0, seg.t1, warp, kThreadsOf<KIND> / 32, lane) || redo;
+    if (!__syncthreads_or(redo)) continue;
     float* piece = p.part + (2 * static_cast<size_t>(blockIdx.x) + seg.slot()) * piece_floats<kUnitRows>(p.w.c.dh);
     // the kernel's fp16 weights are 2^6 times the others
     rows_again<KIND, kUnitRows, TP>(p, seg.u, seg.t0, seg.t1, 1, warp, kThreadsOf<KIND> / 32, lane, seg.whole() ? nullptr : piece,
@@ -390,7 +431,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       mbar_init(&b.plan_empty[i], kF16 ? 14 : 11);      // softmax, MMA, and TMA or loaders
     }
     b.abort = 0;
-    b.again = 0;
+    b.again = b.apart = 0;
     fence_barrier_init();
     if (!kF16) {
       tma_prefetch_desc(&cp.k);
@@ -645,14 +686,6 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         for (int c = 0; c < kWords; ++c)
           raw[c] = r.on && kParts * c + part < ksteps ? __ldg(src + kParts * c) : make_uint4(0u, 0u, 0u, 0u);
       };
-      // biased exponent of the warp's largest finite scale: that of 1 where there is none, and of 2^-107 at least, so
-      // that its products with a score's factor do not vanish
-      auto largest = [&](float x) {
-        uint32_t e = (__float_as_uint(x) >> 23) & 0xffu;
-        e = e == 255u ? 0u : e;
-        e = __reduce_max_sync(0xffffffffu, e);
-        return e == 0u ? 127u : max(e, 20u);
-      };
       // codes * r as fp16, r in two parts: the product is rounded once
       auto store = [&](const uint4 (&raw)[kWords], uint32_t tile, float r) {
         const __half hi = __float2half_rn(r), lo = __float2half_rn(r - __half2float(hi));
@@ -684,7 +717,14 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
       for (uint32_t nk = 0; have && ok; ++nk) {
         const uint32_t st = nk % S, par = ((nk / S) & 1) ^ 1, slot = nk % kMeta;
         const uint32_t none = __ballot_sync(0xffffffffu, r.gone);         // two sixteens of this warp
-        const uint32_t ek = largest(r.ks), ev = largest(r.vs);
+        // where there is no scale, of keys that of 1; of values 2^-60: rows of zeros have their weight in the sum alone
+        bool apart = false;
+        if (r.ks == kZeroRow || r.vs == kZeroRow) {
+          r.ks = used_scale<KIND>(r.ks, p.w.c.k, r.at, dh);
+          r.vs = used_scale<KIND>(r.vs, p.w.c.v, r.at, dh);
+        }
+        const uint32_t ek = largest_exponent(r.ks, 127u, apart), ev = largest_exponent(r.vs, 67u, apart);
+        if (apart) *static_cast<volatile int*>(&b.apart) = 1;
         // 2^(127 - e) as a float: e of 254 at most
         float rk = r.ks * __uint_as_float((254u - ek) << 23), rv = r.vs * __uint_as_float((254u - ev) << 23);
         const bool odd = !(fabsf(r.ks) < INFINITY) || !(fabsf(r.vs) < INFINITY);
@@ -1022,7 +1062,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (KIND != kInt8 && *static_cast<volatile int*>(&b.again) && *abort_flag == 0) segments_again<KIND, TP>(p);
+  const bool redo = (KIND != kInt8 && *static_cast<volatile int*>(&b.again)) || (kF16 && *static_cast<volatile int*>(&b.apart));
+  if (redo && *abort_flag == 0) segments_again<KIND, TP>(p);
 }
 
 // What several blocks left of a unit, in order: a block takes 32 rows, a lane per row, a warp per sixteen columns.

@@ -31,6 +31,7 @@ namespace paged {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr float kZeroScale = 8.67361738e-19f;    // 2^-60: counts as the scale of a row of zeros, whose weight is only in the sum
 
 template <bool F16>
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -57,6 +58,11 @@ __device__ __forceinline__ void ldmatrix(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void ldmatrix_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 // 16 bytes to shared memory; zeros where `on` is false (nothing is read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
@@ -296,14 +302,30 @@ struct Warp {
       // off at most, or 2^-39 of the largest; the sum takes the scale out again.  A scale of zero counts as 2^-126.
       float ks[kMT][2], lv[kMT][2], rv[kMT][2];
       if (kF16) {
+        bool ones = false;
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float v;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks[mt][e]) : "r"(sst + (16 * mt + 8 * e + g) * 4) : "memory");
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(sst + (kTP + 16 * mt + 8 * e + g) * 4) : "memory");
-            v = v < kLeastScale ? kLeastScale : v;       // keeps NaN
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(lv[mt][e]) : "r"(sst + (kTP + 16 * mt + 8 * e + g) * 4) : "memory");
+            ones = ones || lv[mt][e] == kZeroRow;
+          }
+        if (ones) {
+#pragma unroll
+          for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              bool zero = lv[mt][e] == kZeroRow;
+              for (int w = 0; zero && w < wpr; ++w) zero = zero_codes<KIND>(ld_shared_v4(vst + (16 * mt + 8 * e + g) * row_b + 16 * w));
+              if (zero) lv[mt][e] = kZeroScale;
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float v = lv[mt][e] < kLeastScale ? kLeastScale : lv[mt][e];       // keeps NaN
             lv[mt][e] = log2_fast(v);
             rv[mt][e] = __fdividef(1.f, v);
           }

@@ -173,3 +173,26 @@ def test_a_value_that_is_no_number_in_a_long_context(cb, be, kind, window, sinks
                 c["v_pages"].view(torch.uint8)[page, 0, slot, 7] = 0x7f
         q = _rand(sum(new), 16, 64, seed=at + 1) * 0.2
         _compare(cb, be, c, q, new, window, sinks)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("which,mag", [("v", 30), ("v", -40), ("k", 26), ("v zero", -40), ("k zero", -20)])
+def test_neighbours_of_another_magnitude(cb, be, kind, dh, which, mag):
+    """Keys or values whose scales differ by more than fp16 numbers do, beside each other in a tile; rows before the
+    large one do not see it.  ``zero``: rows of zeros, which are stored under a scale of 1, among small ones."""
+    for lengths, new, at in (([200, 30], [200, 30], 150), ([700, 30], [400, 30], 500), ([155, 30], [8, 3], 150)):
+        c = make_cache(kind, lengths, 2, dh, 16, "cuda", seed=at)
+        name = which[0]
+        page, slot = _at(c, 0, at)
+        q = _rand(sum(new), 4, dh, seed=at + 1)
+        if which.endswith("zero"):
+            c[name + "_scale"] *= 2.0 ** mag
+            c[name + "_scale"][page, :, slot] = 1.0
+            c[name + "_pages"].view(torch.uint8)[page, :, slot] = 0
+            if name == "k":
+                q = q * 2.0 ** -mag
+        else:
+            c[name + "_scale"][page, :, slot] *= 2.0 ** mag
+        ref = _compare(cb, be, c, q, new)
+        assert bool(ref.isfinite().all())
