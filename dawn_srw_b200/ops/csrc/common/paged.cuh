@@ -91,7 +91,7 @@ __device__ __forceinline__ size_t slot_row(const View& w, int page, int h, int p
 // int8: 128 + (low seven bits) and 128 or 256 (by the sign bit) are bf16 values whose bits are the code's
 // own; their difference is the number.  e4m3: exponent and fraction moved into bf16's places read as the
 // value times 2^-120 (the biases differ by 120, subnormals included), so one product puts it right.  The
-// NaN codes 0x7f, 0xff, which no write here makes, read back as +-480 (the attention takes them as NaN).
+// NaN codes 0x7f, 0xff, which no write here makes, come out as +-480: the caller looks for them.
 template <int KIND>
 __device__ __forceinline__ uint2 codes_to_bf16(uint32_t x) {
   uint2 r = {__byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342)};

@@ -143,6 +143,11 @@ __device__ __forceinline__ Eight read8(const void* pool, const float* scales, si
   const float s = __ldg(scales + row);
   bf16x8_to_f32(make_uint4(codes_to_bf16<KIND>(c.x).x, codes_to_bf16<KIND>(c.x).y, codes_to_bf16<KIND>(c.y).x,
                            codes_to_bf16<KIND>(c.y).y), e.f);
+  if (KIND == kE4m3 && (odd_codes<kE4m3>(c.x) || odd_codes<kE4m3>(c.y))) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0x7fu) == 0x7fu) e.f[i] = __uint_as_float(0x7fc00000u);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) e.f[i] *= s;
   return e;

@@ -196,3 +196,15 @@ def test_neighbours_of_another_magnitude(cb, be, kind, dh, which, mag):
             c[name + "_scale"][page, :, slot] *= 2.0 ** mag
         ref = _compare(cb, be, c, q, new)
         assert bool(ref.isfinite().all())
+
+
+def test_nan_codes_read_back_as_nan(cb, be):
+    """0x7f and 0xff of e4m3, which no write here makes but a page may hold."""
+    c = make_cache("e4m3", [20], 2, 64, 16, "cuda", garbage=False)
+    raw = c["k_pages"].view(torch.uint8)
+    raw[:, 0, 3, 5], raw[:, 1, 2, 63] = 0x7f, 0xff
+    for dtype in (torch.float32, torch.bfloat16):
+        got, want = be.paged_read(*args(c), 20, **scales(c), dtype=dtype)[0], P.read(*args(c), 20, **scales(c), dtype=dtype)[0]
+        assert int(want.isnan().sum()) == 4 and torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
+    cb.check_status()
