@@ -316,6 +316,20 @@ class DecodeSession:
         return self.out.clone()
 
 
+class _Watched:
+    """A model's parameters and buffers as they are now.  It holds their storages, so that an address is never that of
+    another one in the meantime."""
+
+    def __init__(self, model):
+        self.links = [(d, list(d.items())) for m in model.modules() for d in (m._modules, m._parameters, m._buffers) if d]
+        self.seen = [(p, p.detach(), p._version) for p in (*model.parameters(), *model.buffers())]
+
+    def same(self) -> bool:
+        """Nothing written to, pointed elsewhere (``p.data = ..``) or replaced since."""
+        return (all(len(d) == len(items) and all(d.get(k) is v for k, v in items) for d, items in self.links)
+                and all(p._version == n and p.data_ptr() == t.data_ptr() for p, t, n in self.seen))
+
+
 class PagedSession:
     """Decoding of up to ``max_seqs`` sequences, each of its own length, over one paged key/value cache.
 
@@ -368,8 +382,7 @@ class PagedSession:
         z = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=dev)
         self._table, self._len, self._tok = z(max_seqs, self.width), z(max_seqs), z(max_seqs).long()
         self._graph = self._out = None
-        self._pools = self._key = None
-        self._params = list(model.parameters())
+        self._pools = self._watched = None
         self.use_graph = dev.type == "cuda" if use_graph is None else bool(use_graph)
 
     # ---- sequences and pages -------------------------------------------
@@ -465,12 +478,12 @@ class PagedSession:
         return (m.token_emb.weight.index_select(0, ids) + m.pos_emb.weight.index_select(0, pos)).float()
 
     def _refresh(self) -> None:
-        """What is made from the parameters, made again after a write to one: a captured step reads the copies
-        that it was captured with."""
-        key = tuple(p._version for p in self._params) + (self._params[0].data_ptr(),)
-        if key != self._key:
-            self._key, self._graph, self._out = key, None, None
+        """What is made from the parameters, made again after one was written to or replaced: a captured step reads
+        the copies that it was captured with."""
+        if self._watched is None or not self._watched.same():
+            self._graph = self._out = self._watched = None
             self._pools = None if _is_dense(self.model) else _pools(self.model, self.be)
+            self._watched = _Watched(self.model)
 
     @torch.no_grad()
     def extend(self, new: Dict[int, torch.Tensor], all_logits: bool = False):
