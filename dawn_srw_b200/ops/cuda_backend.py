@@ -898,12 +898,14 @@ class CudaBackend:
 
     # ---- dense ops -----------------------------------------------------
     def _w(self, w):
-        """bf16 compute copy of a master weight, refreshed when the weight changes.  The entry knows its
-        weight (weakly): a new tensor may get the id, and the version, of one that is gone."""
+        """bf16 compute copy of a master weight, refreshed when the weight changes or gets another storage
+        (``w.data = ..`` moves no version).  The entry knows its weight (weakly): a new tensor may get the
+        id, and the version, of one that is gone."""
         key = id(w)
         hit = self._wcache.get(key)
-        if hit is None or hit[0] != w._version or hit[1].device != w.device or hit[2]() is not w:
-            hit = (w._version, w.detach().to(torch.bfloat16), weakref.ref(w))
+        if (hit is None or hit[0] != (w._version, w.data_ptr()) or hit[1].device != w.device
+                or hit[2]() is not w):
+            hit = ((w._version, w.data_ptr()), w.detach().to(torch.bfloat16), weakref.ref(w))
             self._wcache[key] = hit
         return hit[1]
 
