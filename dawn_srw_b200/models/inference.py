@@ -31,6 +31,7 @@ backend (sm_100a kernels on a GPU, plain torch on CPU).
 from __future__ import annotations
 
 import math
+from contextlib import contextmanager
 from typing import Callable, Dict, Iterable, List, Optional, Tuple
 
 import torch
@@ -409,8 +410,22 @@ class PagedSession:
         if ids.numel() and bool(((ids < 0) | (ids >= self.model.vocab_size)).any()):
             raise ValueError(f"a token id is outside the vocabulary of {self.model.vocab_size}")
 
-    def _grow(self, new: Dict[int, int]) -> None:
-        """Room for ``new`` tokens of each sequence, or an error that changes nothing."""
+    @contextmanager
+    def _grown(self, new: Dict[int, int]):
+        """Room for ``new`` tokens of each sequence while what is inside succeeds; an error changes nothing."""
+        before = {s: self.lengths[s] for s in new if 0 <= s < self.max_seqs}
+        taken = self._grow(new)
+        try:
+            yield
+        except BaseException:
+            for s, n in before.items():
+                self.lengths[s] = n
+                del self.pages[s][-(-n // self.page_size):]
+            self.free_pages.extend(reversed(taken))
+            raise
+
+    def _grow(self, new: Dict[int, int]) -> List[int]:
+        """Room for ``new`` tokens of each sequence, or an error that changes nothing; the pages that it took."""
         need = 0
         for s, n in new.items():
             self._check(s)
@@ -421,10 +436,13 @@ class PagedSession:
             need += -(-(self.lengths[s] + n) // self.page_size) - len(self.pages[s])
         if need > len(self.free_pages):
             raise RuntimeError(f"paged cache is full: {need} pages wanted, {len(self.free_pages)} free")
+        taken = []
         for s, n in new.items():
             self.lengths[s] += n
             while len(self.pages[s]) * self.page_size < self.lengths[s]:
-                self.pages[s].append(self.free_pages.pop())
+                taken.append(self.free_pages.pop())
+                self.pages[s].append(taken[-1])
+        return taken
 
     def _forget(self, seqs) -> None:
         """Pages that no later token sees go back to the pool."""
@@ -497,19 +515,21 @@ class PagedSession:
         counts = {s: t.numel() for s, t in ids.items()}
         packed = torch.cat(list(ids.values()))
         self._check_ids(packed)
-        self._grow(counts)
-        self._refresh()
-        seqs, ns = list(ids), list(counts.values())
-        width = max(len(self.pages[s]) for s in seqs)
-        table = self._table_of(seqs, width).to(dev)
-        lengths = torch.tensor([self.lengths[s] for s in seqs], dtype=torch.int32, device=dev)
-        starts = torch.tensor([0] + ns, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
-        pos = torch.cat([torch.arange(self.lengths[s] - n, self.lengths[s]) for s, n in zip(seqs, ns)]).to(dev)
-        h = self._forward(self._embed(packed, pos), table, lengths, starts, max(ns))
+        with self._grown(counts):
+            self._refresh()
+            seqs, ns = list(ids), list(counts.values())
+            width = max(len(self.pages[s]) for s in seqs)
+            table = self._table_of(seqs, width).to(dev)
+            lengths = torch.tensor([self.lengths[s] for s in seqs], dtype=torch.int32, device=dev)
+            starts = torch.tensor([0] + ns, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+            pos = torch.cat([torch.arange(self.lengths[s] - n, self.lengths[s]) for s, n in zip(seqs, ns)]).to(dev)
+            h = self._forward(self._embed(packed, pos), table, lengths, starts, max(ns))
+            if all_logits:
+                out = list(self.be.logits(h, self.model.token_emb.weight).split(ns))
+            else:
+                out = self.be.logits(h[starts[1:].long() - 1].contiguous(), self.model.token_emb.weight)
         self._forget(seqs)
-        if all_logits:
-            return list(self.be.logits(h, self.model.token_emb.weight).split(ns))
-        return self.be.logits(h[starts[1:].long() - 1].contiguous(), self.model.token_emb.weight)
+        return out
 
     def _step_static(self):
         pos = (self._len.long() - 1).clamp(min=0)              # an idle slot has no position and attends to nothing
@@ -524,31 +544,34 @@ class PagedSession:
             raise ValueError("no sequence to extend")
         tokens = {s: int(t) for s, t in tokens.items()}
         self._check_ids(torch.tensor(list(tokens.values())))
-        self._grow({s: 1 for s in tokens})
-        self._refresh()
-        dev = self._table.device
-        active = list(range(self.max_seqs))
-        self._table.copy_(self._table_of(active, self.width))
-        self._len.copy_(torch.tensor([self.lengths[s] if s in tokens else 0 for s in active], dtype=torch.int32))
-        self._tok.copy_(torch.tensor([tokens.get(s, 0) for s in active]))
-        if not self.use_graph:
-            out = self._step_static()
-        else:
-            if self._graph is None:
-                # outside the capture first (lazy initialisation); it writes the slots that the replay writes again
-                side = torch.cuda.Stream(device=dev)
-                side.wait_stream(torch.cuda.current_stream(dev))
-                with torch.cuda.stream(side):
-                    for _ in range(2):
-                        self._step_static()
-                torch.cuda.current_stream(dev).wait_stream(side)
-                self._graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self._graph):
-                    self._out = self._step_static()
-            self._graph.replay()
-            out = self._out
+        with self._grown({s: 1 for s in tokens}):
+            self._refresh()
+            dev = self._table.device
+            active = list(range(self.max_seqs))
+            self._table.copy_(self._table_of(active, self.width))
+            self._len.copy_(torch.tensor([self.lengths[s] if s in tokens else 0 for s in active], dtype=torch.int32))
+            self._tok.copy_(torch.tensor([tokens.get(s, 0) for s in active]))
+            out = self._replay(dev) if self.use_graph else self._step_static()
+            out = out[torch.tensor(list(tokens), device=dev)]
         self._forget(tokens)
-        return out[torch.tensor(list(tokens), device=dev)]
+        return out
+
+    def _replay(self, dev) -> torch.Tensor:
+        """The captured step, captured first where there is none."""
+        if self._graph is None:
+            # outside the capture first (lazy initialisation); it writes the slots that the replay writes again
+            side = torch.cuda.Stream(device=dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                for _ in range(2):
+                    self._step_static()
+            torch.cuda.current_stream(dev).wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = self._step_static()
+            self._graph, self._out = graph, out           # only now: a failed capture leaves none
+        self._graph.replay()
+        return self._out
 
     @torch.no_grad()
     def dense(self, seqs: Iterable[int]) -> Tuple[torch.Tensor, torch.Tensor]:

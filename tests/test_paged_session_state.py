@@ -59,3 +59,46 @@ def test_parameters_that_are_pointed_elsewhere_or_replaced(kind, change):
     assert s._watched is not watched                              # a captured step is captured again
     want = _expected(m, torch.cat([IDS, torch.tensor([3])]), "bf16")
     assert _close(after[0], want[20]) and not torch.allclose(before, after, atol=1e-3)
+
+
+class Failing:
+    """A backend whose n-th call of an operator from now on fails."""
+
+    def __init__(self, be, name, n):
+        self._be, self._name, self._left = be, name, n
+
+    def __getattr__(self, name):
+        f = getattr(self._be, name)
+        if name != self._name:
+            return f
+
+        def call(*a, **kw):
+            self._left -= 1
+            if self._left == 0:
+                raise RuntimeError("out of memory")
+            return f(*a, **kw)
+        return call
+
+
+@pytest.mark.parametrize("name,n", [("paged_write", 1), ("paged_attention", 2), ("logits", 1), ("layer_norm", 3)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (9, 2)])
+def test_a_call_that_fails_changes_nothing(name, n, window, sinks):
+    """Lengths, pages and what is free stay, and the call made again gives the logits of a session without the failure."""
+    m = _model("spatial-r1-v4.1")
+    ids = torch.randint(1, 200, (60,), generator=torch.Generator().manual_seed(7))
+    s = I.PagedSession(m, 2, window=window, sinks=sinks)
+    a, b = s.open(), s.open()
+    s.extend({a: ids[:30], b: ids[:16]})
+    be, state = s.be, lambda: (list(s.lengths), copy.deepcopy(s.pages), list(s.free_pages))
+    for new in (lambda: s.extend({b: ids[16:50], a: ids[30:33]}), lambda: s.extend({a: ids[33:35], b: ids[50:51]}, all_logits=True),
+                lambda: s.step({a: ids[35], b: ids[51]})):
+        before = state()
+        s.be = Failing(be, name, n)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            new()
+        assert state() == before
+        s.be = be
+        last = new()
+    assert s.lengths == [36, 52]
+    assert _close(last[0], _expected(m, ids[:36], "bf16", window, sinks)[35])
+    assert _close(last[1], _expected(m, ids[:52], "bf16", window, sinks)[51])
