@@ -358,6 +358,8 @@ class PagedSession:
             raise ValueError("max_seqs must be positive and page_size a power of two from 16 to 256")
         if window is not None and window < 1 or sinks < 0:
             raise ValueError("window must be at least 1 (None: no window), sinks not negative")
+        if sinks and window is None:
+            raise ValueError("sinks belong to a window")
         if not _is_dense(model) and model.shard_group is not None:
             raise ValueError("a paged session needs unsharded pools")
         self.model, self.page_size, self.window, self.sinks = model, page_size, window, sinks

@@ -102,3 +102,12 @@ def test_a_call_that_fails_changes_nothing(name, n, window, sinks):
     assert s.lengths == [36, 52]
     assert _close(last[0], _expected(m, ids[:36], "bf16", window, sinks)[35])
     assert _close(last[1], _expected(m, ids[:52], "bf16", window, sinks)[51])
+
+
+def test_sinks_without_a_window_are_refused():
+    """As with dense caches; they were left out without a word."""
+    m = _model("dense")
+    with pytest.raises(ValueError, match="sinks belong to a window"):
+        I.PagedSession(m, 1, sinks=2)
+    with pytest.raises(ValueError, match="sinks belong to a window"):
+        I.generate(m, IDS[None], max_new_tokens=2, kv_dtype="bf16", sinks=1)
