@@ -368,6 +368,7 @@ class PagedSession:
         L, H = model.n_layers, model.n_heads
         dh = model.d_model // H
         self.width = -(-model.max_seq_len // page_size)
+        self.be.paged_supported(H, dh, max_seqs, self.width * page_size)
         n_pages = max_seqs * self.width if n_pages is None else int(n_pages)
         dtype = PAGE_DTYPES[kv_dtype]
         shape = (L, n_pages, H, page_size, dh)

@@ -84,6 +84,9 @@ class ReferenceBackend:
         return R.pool_diversity(tensors)
 
     # ---- paged key/value cache -----------------------------------------
+    def paged_supported(self, heads, dim, sequences, positions):
+        """Raises ValueError for a cache that the operators here cannot take; the plain path takes any."""
+
     @torch.no_grad()
     def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
         paged.write(k, v, k_pages, v_pages, table, lengths, starts, k_scale, v_scale)

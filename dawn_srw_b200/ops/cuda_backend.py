@@ -987,6 +987,15 @@ class CudaBackend:
         return ext().prompt_attention(f(q), f(k), f(v), cache_k, cache_v, B, S, status_word(q.device))
 
     # ---- paged key/value cache (layouts, types and bounds: ops/paged.py; no gradients) ----
+    def paged_supported(self, heads: int, dim: int, sequences: int, positions: int):
+        """Raises ValueError for a cache that the kernels cannot take (the bindings refuse each call of one)."""
+        if dim < 16 or dim > 128 or dim % 16 != 0:
+            raise ValueError(f"paged cache: head dimension {dim} is not supported by the kernels "
+                             "(multiple of 16, at most 128)")
+        if heads > 65535 or sequences > 65535 or positions > 2 ** 30:
+            raise ValueError(f"paged cache: {heads} heads, {sequences} sequences or {positions} positions are too "
+                             "many for the kernels (65535, 65535, 2^30)")
+
     def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
         """Keys and values [N, H, dh] (fp32 or bf16) of new tokens into their pages, rounded to the pages'
         type.  One launch; rows of no sequence, and positions whose table entry names no page, are left

@@ -111,3 +111,17 @@ def test_sinks_without_a_window_are_refused():
         I.PagedSession(m, 1, sinks=2)
     with pytest.raises(ValueError, match="sinks belong to a window"):
         I.generate(m, IDS[None], max_new_tokens=2, kv_dtype="bf16", sinks=1)
+
+
+@pytest.mark.parametrize("d_model,heads", [(32, 4), (96, 4), (320, 2)])
+def test_heads_that_the_kernels_cannot_take_are_refused_by_the_constructor(d_model, heads):
+    """Of 8, 24 and 160; the plain path takes them."""
+    from dawn_srw_b200.models.baseline import VanillaTransformer
+    from dawn_srw_b200.ops.cuda_backend import CudaBackend
+    m = VanillaTransformer(vocab_size=50, d_model=d_model, n_layers=1, n_heads=heads, max_seq_len=40, d_ff=16).eval()
+    I.PagedSession(m, 1)
+    m.backend = CudaBackend()
+    with pytest.raises(ValueError, match="not supported by the kernels"):
+        I.PagedSession(m, 1)
+    with pytest.raises(ValueError, match="too many"):
+        m.backend.paged_supported(2, 64, 65536, 512)
