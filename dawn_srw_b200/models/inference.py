@@ -347,7 +347,8 @@ class PagedSession:
         s.close(a)
 
     Attention reads what the pages hold, so the logits are those of the rounded cache.  Dense and SRW models;
-    pools must not be sharded."""
+    pools must not be sharded.  A kernel that gives up (a wait that ran out, a page outside the pool) is reported
+    by RuntimeError in the call after the one that launched it, or by ``check()``, which waits for the GPU."""
 
     def __init__(self, model, max_seqs: int, *, n_pages: Optional[int] = None, page_size: int = 16,
                  kv_dtype: str = "bf16", window: Optional[int] = None, sinks: int = 0,
@@ -531,6 +532,7 @@ class PagedSession:
                 out = list(self.be.logits(h, self.model.token_emb.weight).split(ns))
             else:
                 out = self.be.logits(h[starts[1:].long() - 1].contiguous(), self.model.token_emb.weight)
+            self.be.finish_step()
         self._forget(seqs)
         return out
 
@@ -556,6 +558,7 @@ class PagedSession:
             self._tok.copy_(torch.tensor([tokens.get(s, 0) for s in active]))
             out = self._replay(dev) if self.use_graph else self._step_static()
             out = out[torch.tensor(list(tokens), device=dev)]
+            self.be.finish_step()
         self._forget(tokens)
         return out
 
@@ -575,6 +578,10 @@ class PagedSession:
             self._graph, self._out = graph, out           # only now: a failed capture leaves none
         self._graph.replay()
         return self._out
+
+    def check(self) -> None:
+        """Waits for the GPU and raises RuntimeError if a kernel reported a failure."""
+        self.be.finish_run()
 
     @torch.no_grad()
     def dense(self, seqs: Iterable[int]) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -669,6 +676,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, temperatu
             t1 = time.perf_counter()
     sync()
     t2 = time.perf_counter()
+    _be(model, input_ids.device).finish_run()          # raises if a kernel gave up
     B = input_ids.shape[0]
     stats = {"new_tokens": n, "tokens_per_sec": n * B / max(t2 - t0, 1e-9),
              "first_step_s": (t1 - t0) if t1 is not None else 0.0, "graph": session.use_graph}

@@ -54,3 +54,29 @@ def test_a_failed_capture_leaves_no_graph():
     assert s._graph is not None and s.lengths == [40]
     assert torch.equal(got, _logits(I.PagedSession(m, 1, use_graph=False), ids))
     s.be.finish_run()
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_a_page_outside_the_pool_is_reported_to_the_caller(use_graph):
+    m = _model("dense")
+    s = I.PagedSession(m, 1, use_graph=use_graph)
+    a = s.open()
+    s.extend({a: torch.arange(1, 40)})
+    s.step({a: 3})
+    s.check()
+    good, s.pages[a][1] = s.pages[a][1], 10 ** 6                 # counts as absent; the status word tells of it
+    s.step({a: 3})
+    with pytest.raises(RuntimeError, match="status 4"):
+        s.step({a: 3})
+    assert s.lengths == [41]
+    s.pages[a][1] = good
+    try:
+        s.check()                                                # of the step that raised, which ran all the same
+    except RuntimeError:
+        pass
+    s.step({a: 3})
+    s.check()
+    s.pages[a][1] = 10 ** 6
+    s.extend({a: torch.arange(1, 20)})
+    with pytest.raises(RuntimeError, match="status 4"):
+        s.check()

@@ -125,3 +125,42 @@ def test_heads_that_the_kernels_cannot_take_are_refused_by_the_constructor(d_mod
         I.PagedSession(m, 1)
     with pytest.raises(ValueError, match="too many"):
         m.backend.paged_supported(2, 64, 65536, 512)
+
+
+class Reporting(Failing):
+    """A backend that counts how often its failures are asked for, and can have one to report."""
+    failure = None
+
+    def __init__(self, be):
+        super().__init__(be, "", 0)
+        self.steps = self.runs = 0
+
+    def finish_step(self):
+        self.steps += 1
+        if self.failure:
+            raise RuntimeError(self.failure)
+
+    def finish_run(self):
+        self.runs += 1
+
+
+def test_failures_of_kernels_are_asked_for():
+    m = _model("dense")
+    s = I.PagedSession(m, 1)
+    s.be = Reporting(s.be)
+    a = s.open()
+    s.extend({a: IDS})
+    s.step({a: 3})
+    assert (s.be.steps, s.be.runs) == (2, 0)
+    s.be.failure = "status 4"
+    for call in (lambda: s.step({a: 3}), lambda: s.extend({a: IDS})):
+        with pytest.raises(RuntimeError, match="status 4"):
+            call()
+        assert s.lengths == [21]
+    s.check()
+    assert s.be.runs == 1
+    m.backend = Reporting(m._backend(torch.device("cpu")))
+    for kw in ({}, {"kv_dtype": "int8"}):
+        runs = m.backend.runs
+        I.generate(m, IDS[None], max_new_tokens=2, **kw)
+        assert m.backend.runs == runs + 1
