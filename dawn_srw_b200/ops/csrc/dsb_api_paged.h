@@ -13,7 +13,7 @@ extern "C" {
 //   lengths [B]: positions of a sequence, its new tokens included;
 //   starts [B + 1] or null: rows starts[b] .. starts[b + 1] of the N packed rows are the last tokens of
 //   sequence b (null: row b is the last token of sequence b, N == B).  starts ascends; no two rows that are written
-//   in one call have one place.
+//   in one call may have one place (not checked: their words, codes and scales would mix).
 // Page size: a power of two, 16 .. 256; dh a multiple of 16, at most 128; everything 16-byte aligned, the
 // attention's result 32-byte.
 // A length above width * page or a page outside the pool sets *status to 4; what it names counts as absent.

@@ -998,7 +998,7 @@ class CudaBackend:
 
     def paged_write(self, k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None):
         """Keys and values [N, H, dh] (fp32 or bf16) of new tokens into their pages, rounded to the pages'
-        type.  One launch; rows of no sequence, and positions whose table entry names no page, are left
+        type.  No two rows may have one place.  One launch; rows of no sequence, and positions whose table entry names no page, are left
         out (the latter sets the status word)."""
         count_launches(1)
         ext().paged_write(k, v, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, _paged_status(k_pages))

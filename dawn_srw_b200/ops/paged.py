@@ -6,7 +6,8 @@ Pages of keys and values are ``[n_pages, H, page, dh]``: bf16, or 8-bit codes (`
 (int32) names the page of positions ``i * page .. (i + 1) * page`` of a sequence, ``lengths [B]`` (int32)
 its positions, new tokens included.  The new tokens of all sequences are packed: rows ``starts[b] ..
 starts[b + 1]`` (ascending) are the last tokens of sequence ``b``; ``starts`` is None where every sequence
-has one.  Sequences may share pages that they read; what one call writes twice to a place is either value.
+has one.  Sequences may share pages that they read.  No two rows that one call writes may have one place: the
+plain path refuses them, the kernels do not look and would mix the two.
 
 A row of keys or values is stored with one rounding: bf16; e4m3 after division by the smallest power of
 two that brings the row's largest magnitude to 448 or less; or int8, ``round(x * (127 / largest))`` with
@@ -136,6 +137,7 @@ def write(k, v, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_s
     ids = table[seq, pos // page].long()
     _refuse_unless(bool(((ids >= 0) & (ids < k_pages.shape[0])).all()), "a table entry names no page")
     slot = pos % page
+    _refuse_unless(len((ids * page + slot).unique()) == len(ids), "two rows have one place")
     for x, pages, scales in ((k, k_pages, k_scale), (v, v_pages, v_scale)):
         codes, scale = encode_rows(x[there], pages.dtype)
         _raw(pages)[ids, :, slot] = _raw(codes)

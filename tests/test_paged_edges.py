@@ -90,3 +90,13 @@ def test_a_value_that_is_no_number_reaches_the_rows_that_see_it(odd, window, sin
     assert int((~fine).sum()) == 2 * (11 if window is None else window)              # two query heads of the group, a column
     assert torch.equal(got.isfinite(), fine) and torch.equal(got[~fine].double().nan_to_num(), ref[~fine].float().double().nan_to_num())
     assert bool(((got.double() - ref).abs() <= 1e-5 * mag + 1e-12)[fine].all())
+
+
+def test_two_rows_with_one_place_are_refused_by_the_plain_path():
+    c = make_cache("int8", [20, 7], 2, 16, 16, CPU, garbage=False)
+    c["table"][1, 0] = c["table"][0, 0]                          # a page that both read is fine
+    x = torch.zeros(2, 2, 16)
+    ReferenceBackend().paged_write(x, x, *args(c), **scales(c))
+    c["lengths"][:] = 7
+    with pytest.raises(ValueError, match="one place"):
+        ReferenceBackend().paged_write(x, x, *args(c), **scales(c))
