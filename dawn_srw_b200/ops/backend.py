@@ -99,6 +99,7 @@ class ReferenceBackend:
     @torch.no_grad()
     def paged_attention(self, q, k_pages, v_pages, table, lengths, starts=None, k_scale=None, v_scale=None, *,
                         max_new=None, window=None, sinks=0, scale=None):
+        """In the queries' type, as ``attention`` here; the kernels return bf16, as theirs."""
         return paged.attention(q, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, max_new=max_new,
                                window=window, sinks=sinks, scale=scale)
 
