@@ -412,6 +412,7 @@ __device__ __noinline__ void rows_again(const AttnParams& p, const Unit u, int t
         const size_t at = on ? slot_row(p.w, page, u.h, j) : 0;
         float s = 0.f, vs = 1.f;
         if (on) {
+#pragma unroll 4
           for (int c = 0; c < dh; c += 8) {
             float a[8], k[8];
             bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(q + c)), a);
@@ -433,16 +434,18 @@ __device__ __noinline__ void rows_again(const AttnParams& p, const Unit u, int t
         m = m_new;
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] *= d;
+#pragma unroll 8
         for (int k = 0; k < 32; k += 2) {              // half a warp a position
           const int from = k + half;
           const float y = __shfl_sync(0xffffffffu, w, from), z = __shfl_sync(0xffffffffu, vs, from);
           const unsigned long long at_k = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), from);
-          if (((seen >> from) & 1u) && col < dh) {
-            float v[8];
-            held8<KIND>(p.w.c.v, at_k * dh + col, v);
+          const bool mine = ((seen >> from) & 1u) && col < dh;
+          float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = fmaf(y, v[e] * z, o[e]);
-          }
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+          if (mine) held8<KIND>(p.w.c.v, at_k * dh + col, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = mine ? fmaf(y, v[e] * z, o[e]) : o[e];
         }
       }
 #pragma unroll

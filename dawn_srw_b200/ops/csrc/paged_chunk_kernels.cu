@@ -8,12 +8,13 @@
 //
 // bf16 pages come by TMA, one box per page and 64 columns, into the 128-byte-swizzled tiles that the instructions
 // read: K-major for K, MN-major for V.  8-bit codes are read by four warps and go to the same layout as fp16 numbers,
-// code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: exact for e4m3, whose scales
-// are powers of two and whose codes are multiples of 2^-9, and rounded once, by 2^-11 at most, for int8 (as a weight is,
-// and far below the codes' own rounding; a scale per column in the softmax would cost each thread three shared-memory
-// reads per column).  That is while no scale is smaller by more than 2^15: where one is, the block's work is done again
-// in fp32 (rows_again).  Rows of zeros have no part in it.  2^e of the keys goes to the scores, 2^e of the values, as in
-// the few-row kernel, to the exponents and out of the sum.
+// code * scale / 2^e, e the exponent of the largest scale among the 32 positions of a warp: for int8 rounded once, by
+// 2^-11 at most (as a weight is, and far below the codes' own rounding; a scale per column in the softmax would cost each
+// thread three shared-memory reads per column), for e4m3, whose scales are powers of two and whose codes are multiples of
+// 2^-9, exact while the scale is not smaller than the largest by more than 2^15.  At 2^20 fp16's smallest step is 2^-12 of
+// such a row's largest value, of int8's at 2^13 the rounding of the scale; where one is smaller still, the block's work is
+// done again in fp32 (rows_again).  Rows of zeros have no part in it.  2^e of the keys goes to the scores, 2^e of the
+// values, as in the few-row kernel, to the exponents and out of the sum.
 //
 // Rows of V that no query row sees are zeros, whatever the page holds there; a scale that is no number makes the scores
 // of its position NaN; a value that is none, seen by some rows of a unit alone, has the block's work done again too.
@@ -344,13 +345,15 @@ __device__ __forceinline__ float used_scale(float s, const void* pool, size_t ro
 }
 
 // Of a warp's scales: biased exponent of the largest finite one, that of 2^-107 at least, so that its products with a score's
-// factor do not vanish; `none` where there is none.  apart: this lane's is less by more than 2^15.
+// factor do not vanish; `none` where there is none.  apart: this lane's is less by more than 2^20 (e4m3 and a power of two) or
+// 2^13.
+template <int KIND>
 __device__ __forceinline__ uint32_t largest_exponent(float x, uint32_t none, bool& apart) {
   const uint32_t e = (__float_as_uint(x) >> 23) & 0xffu;
   uint32_t most = __reduce_max_sync(0xffffffffu, e == 255u ? 0u : e);
   if (most == 0u) return none;
   most = max(most, 20u);
-  apart = apart || (e != 0u && most > e + 15u);
+  apart = apart || (e != 0u && most > e + (KIND == kE4m3 && (__float_as_uint(x) & 0x7fffffu) == 0u ? 20u : 13u));
   return most;
 }
 
@@ -362,8 +365,8 @@ __device__ __noinline__ bool scales_apart(const AttnParams& p, const Unit u, int
     const int tile = t0 + i / (TP / 32), x = (tile < u.st ? tile : tile + u.skip) * TP + i % (TP / 32) * 32 + lane;
     const int page = x < u.hi && (x >= u.lo || x < u.s_end) ? page_of(p.w, u.b, x) : -1;
     const size_t at = page >= 0 ? slot_row(p.w, page, u.h, x) : 0;
-    largest_exponent(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.k_scale + at), p.w.c.k, at, p.w.c.dh) : 0.f, 0u, apart);
-    largest_exponent(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.v_scale + at), p.w.c.v, at, p.w.c.dh) : 0.f, 0u, apart);
+    largest_exponent<KIND>(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.k_scale + at), p.w.c.k, at, p.w.c.dh) : 0.f, 0u, apart);
+    largest_exponent<KIND>(page >= 0 ? used_scale<KIND>(__ldg(p.w.c.v_scale + at), p.w.c.v, at, p.w.c.dh) : 0.f, 0u, apart);
   }
   return apart;
 }
@@ -686,7 +689,8 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
         for (int c = 0; c < kWords; ++c)
           raw[c] = r.on && kParts * c + part < ksteps ? __ldg(src + kParts * c) : make_uint4(0u, 0u, 0u, 0u);
       };
-      // codes * r as fp16, r in two parts: the product is rounded once
+      // codes * r as fp16, r in two parts, whose second one is a multiple of 2^-24: the product is rounded once, and r, of
+      // 2^-13 at least unless it is a power of two, by 2^-12 at most
       auto store = [&](const uint4 (&raw)[kWords], uint32_t tile, float r) {
         const __half hi = __float2half_rn(r), lo = __float2half_rn(r - __half2float(hi));
         const __half2 h2 = __half2half2(hi), l2 = __half2half2(lo);
@@ -723,7 +727,7 @@ __global__ void __launch_bounds__(kThreadsOf<KIND>, 1) paged_chunk_kernel(const 
           r.ks = used_scale<KIND>(r.ks, p.w.c.k, r.at, dh);
           r.vs = used_scale<KIND>(r.vs, p.w.c.v, r.at, dh);
         }
-        const uint32_t ek = largest_exponent(r.ks, 127u, apart), ev = largest_exponent(r.vs, 67u, apart);
+        const uint32_t ek = largest_exponent<KIND>(r.ks, 127u, apart), ev = largest_exponent<KIND>(r.vs, 67u, apart);
         if (apart) *static_cast<volatile int*>(&b.apart) = 1;
         // 2^(127 - e) as a float: e of 254 at most
         float rk = r.ks * __uint_as_float((254u - ek) << 23), rv = r.vs * __uint_as_float((254u - ev) << 23);

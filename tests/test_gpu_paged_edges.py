@@ -41,7 +41,10 @@ def smallest_weights(q, c, new, window=None, sinks=0):
     """What the fp16 weights of 8-bit pages may add to a result.  A weight goes to fp16 as p_j S_j, S_j being the power
     of two next to (in a chunk: at) the largest scale of the values among 32 positions, p_j the softmax; the
     row's largest, W, stands at 2^6 or more.  A weight below fp16's normal numbers is off by half of its smallest step,
-    2^-25, which is 2^-31 W: by sum_j 2^-31 W |v_j| / S_j in all, and S_j is more than half of the scale of j."""
+    2^-25, which is 2^-31 W: by sum_j 2^-31 W |v_j| / S_j in all, and S_j is more than half of the scale of j.  In a
+    chunk a value next to a larger scale is off by half of that step too, 2^-25 S_j (none where the scales of 32
+    positions are more than 2^20, for int8 2^13, apart: the work is done in fp32): by sum_j p_j 2^-25 S_j; and a key in the same way,
+    which moves a score by scale |q|_1 2^-25 S'_j, a weight by that and the sum of weights by as much again."""
     out = torch.zeros(q.shape, dtype=torch.double, device=q.device)
     if c["v_scale"] is None:
         return out
@@ -52,21 +55,33 @@ def smallest_weights(q, c, new, window=None, sinks=0):
         k, v = held64(c, b, length, "k"), held64(c, b, length, "v")
         pos = torch.arange(length, device=q.device)
         ids = c["table"][b].long()[pos // c["k_pages"].shape[2]]
-        s = c["v_scale"][ids, :, pos % c["k_pages"].shape[2]].double()              # [length, H]
-        s = torch.where((v == 0).all(-1) | ~s.isfinite(), torch.zeros_like(s), s)
-        group = torch.zeros_like(s)
-        for x in range(0, length, 32):
-            top, least = s[x: x + 32].amax(0), torch.where(s > 0, s, torch.full_like(s, math.inf))[x: x + 32].amin(0)
-            group[x: x + 32] = torch.where(top <= 2.0 ** 15 * least, top, s[x: x + 32])
+        groups = {}
+        for name, x64 in (("v", v), ("k", k)):
+            s = c[name + "_scale"][ids, :, pos % c["k_pages"].shape[2]].double()              # [length, H]
+            s = torch.where((x64 == 0).all(-1) | ~s.isfinite(), torch.zeros_like(s), s)
+            group = torch.zeros_like(s)
+            for x in range(0, length, 32):
+                top, least = s[x: x + 32].amax(0), torch.where(s > 0, s, torch.full_like(s, math.inf))[x: x + 32].amin(0)
+                near = top <= 2.0 ** (14 if c["k_pages"].dtype == torch.int8 else 21) * least
+                group[x: x + 32] = torch.where(near, top, s[x: x + 32])
+            groups[name] = s, group
+        (s, group), (_, kgroup) = groups["v"], groups["k"]
         codes = torch.where(s[..., None] > 0, v.abs() / s[..., None], torch.zeros_like(v)).nan_to_num(0.0)
         for i in range(n):
             p = length - n + i
-            j = torch.arange(p + 1, device=q.device)
+            j = torch.arange(max(p, -1) + 1, device=q.device)
             if window is not None:
                 j = j[(j > p - window) | (j < sinks)]
+            if not len(j):
+                continue
             a = torch.einsum("hgd,nhd->hgn", q[at + i].double().view(H, G, -1), k[j]) / math.sqrt(q.shape[2])
-            most = (torch.softmax(a, -1) * group[j].T[:, None]).amax(-1)                # [H, G]
-            out[at + i] = (2.0 ** -30 * most[..., None] * codes[j].sum(0)[:, None]).reshape(q.shape[1:])
+            w = torch.softmax(a, -1)
+            most = (w * group[j].T[:, None]).amax(-1)                                   # [H, G]
+            step = 2.0 ** -25 * (w * group[j].T[:, None]).sum(-1)
+            moved = 2.0 ** -24 / math.sqrt(q.shape[2]) * q[at + i].double().abs().sum(-1).view(H, G) * kgroup[j].amax(0)[:, None]
+            mag = torch.einsum("hgn,nhd->hgd", w, v[j].abs())
+            slack = 2.0 ** -30 * most[..., None] * codes[j].sum(0)[:, None] + step[..., None] + moved[..., None] * mag
+            out[at + i] = slack.reshape(q.shape[1:])
         at += n
     return out.nan_to_num(0.0)
 
@@ -177,10 +192,11 @@ def test_a_value_that_is_no_number_in_a_long_context(cb, be, kind, window, sinks
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
 @pytest.mark.parametrize("dh", [64, 128])
-@pytest.mark.parametrize("which,mag", [("v", 30), ("v", -40), ("k", 26), ("v zero", -40), ("k zero", -20)])
+@pytest.mark.parametrize("which,mag", [("v", 30), ("v", -40), ("v", 19), ("v", -12), ("k", 26), ("k", 18), ("k", -14),
+                                       ("v zero", -40), ("k zero", -20)])
 def test_neighbours_of_another_magnitude(cb, be, kind, dh, which, mag):
-    """Keys or values whose scales differ by more than fp16 numbers do, beside each other in a tile; rows before the
-    large one do not see it.  ``zero``: rows of zeros, which are stored under a scale of 1, among small ones."""
+    """Keys or values whose scales differ by much, some by more than fp16 numbers do, beside each other in a tile; rows
+    before the large one do not see it.  ``zero``: rows of zeros, which are stored under a scale of 1, among small ones."""
     for lengths, new, at in (([200, 30], [200, 30], 150), ([700, 30], [400, 30], 500), ([155, 30], [8, 3], 150)):
         c = make_cache(kind, lengths, 2, dh, 16, "cuda", seed=at)
         name = which[0]
