@@ -342,7 +342,8 @@ struct Segments {
 // ---- Units computed again.  Products of whole tiles hand a value that is no number on to rows that do not see it: a weight
 // of zero times NaN or inf is NaN.  It shows in an O that is not finite beside a finite sum of weights; then the positions
 // that only some of the unit's rows see are looked through, and if one holds such a value the work is done again row by row,
-// position by position, without touching what a row does not see.  Hundreds of times slower, and for diverged caches alone.
+// position by position, without touching what a row does not see.  Hundreds of times slower (ragged prompts with one NaN, 16 heads of
+// 128, 3.4 ms for 0.09; all 4099 x 6000 positions of an int8 chunk 39 ms for 0.19), and for diverged caches alone.
 
 // NaN if x, or a term before it, is not finite.
 __device__ __forceinline__ float track_odd(float odd, float x) { return fmaf(x, 0.f, odd); }

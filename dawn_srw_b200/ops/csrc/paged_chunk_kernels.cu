@@ -23,13 +23,13 @@
 // SMs idle; units that several blocks share are left in pieces for the merge kernel.
 //
 // What bounds it.  The products alone, at the rate of a large matrix product (1.66 PFLOP/s), are a third of the time:
-// five bf16 prompts of 301 to 2048 tokens, 16 heads of 128, 96 us for 31; 4099 tokens over 16000 int8 positions, 16
-// heads of 64 that share 4 and a window of 4096, 181 us for 61.  128 positions of a unit take about 4000 cycles.  By
+// five bf16 prompts of 301 to 2048 tokens, 16 heads of 128, 97 us for 31; 4099 tokens over 16000 int8 positions, 16
+// heads of 64 that share 4 and a window of 6000, 187 us for 61.  128 positions of a unit take about 4000 cycles.  By
 // arithmetic the exponential unit has 1700 of them to do, shared memory at 128 bytes a cycle 1800 (heads of 64) to 2800
 // (heads of 128) for the products' operands and 512 for the loads; the clock inside the kernel shows some 700 cycles
 // per tile and warp that are waits, and latencies of TMEM and shared memory, in the open: the two softmax warps of a
 // quarter of the SM run in step.  Starting one of them later changed nothing; exponentials on the FMA units help by 3 % at most (see kPoly).
-// A small call, 512 tokens over 2100 e4m3 positions, 16 heads of 80, takes 27 us for 3: its plan (2.5 us), two runs a
+// A small call, 512 tokens over 2100 e4m3 positions, 16 heads of 80, takes 28 us for 3: its plan (2.5 us), two runs a
 // block, the pieces and their merge (8 us).
 #include <type_traits>
 

@@ -10,6 +10,7 @@
 // lane's queries are those of the four neighbouring codes it gets.  Queries, bf16, become fp16 by a power of two for
 // each row that brings the largest to [128, 256): exact down to 2^-22 of it, off by 2^-33 of it below.  The keys'
 // scales go to the scores in fp32, the values' to the exponents (see below).  Running maximum and sum stay in registers.
+// Drafted tokens that do not all see a value that is no number have their rows done again (work_again).
 //
 // Two ways to share the work.  Where a warp has few tiles, a cluster of blocks takes a unit, its warps every n-th tile,
 // and merges in (distributed) shared memory: one launch.  For long caches as many warps as the GPU holds take equal
@@ -17,11 +18,11 @@
 // pieces, which a second kernel adds up in order.  The lengths are read on the device, so a captured call follows them.
 //
 // What bounds it.  Reading the keys and values once is the floor (6.5 TB/s).  Six e4m3 sequences of 2000 to 32000, 16
-// heads of 80: 53 us for 37, 4.6 TB/s: the rest is the plan, the merge of pieces (7 us together) and the conversion of
+// heads of 80: 54 us for 37, 4.6 TB/s: the rest is the plan, the merge of pieces (7 us together) and the conversion of
 // codes, half of the instructions issued.  32 bf16 sequences of 100 to 512, 16 heads of 128: 17 us for 10; one of 290,
 // 6 heads of 64: 6 us, a launch, three dependent loads (length, table, page) and a merge.  Four query heads or more per
 // head of the cache cost twice the instructions of one: 16 int8 sequences under a window of 4096, 32 query heads over
-// 4: 19 us for 9; five drafted tokens of 8 bf16 sequences, 16 over 8 heads of 64: 15 us for 3, the longest sequence
+// 4: 20 us for 9; five drafted tokens of 8 bf16 sequences, 16 over 8 heads of 64: 15 us for 3, the longest sequence
 // (6000) being 30 times the shortest in clusters of equal size.
 #include "common/paged_launch.h"
 #include "common/ptx.cuh"
@@ -672,7 +673,10 @@ int launch(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
   return launch_early(paged_merge_few_kernel<W::kRows>, dim3(p.workers), kMergeThreads, 0, p, stream);
 }
 
-// Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.
+// Sixteens of the head dimension that the registers are laid out for: 32, 64, 80 or 128.  Others use the next larger layout,
+// its words that they lack being zeros, and ask for each word of a copy whether it is there.  Microseconds of heads of
+// 64 / 80 / 96 / 112 / 128, 32 sequences of 100 to 512 (16 heads): bf16 10.0 / 13.2 / 17.6 / 19.2 / 16.8, e4m3 10.8 / 10.5 /
+// 18.2 / 19.0 / 15.5; 6 of 2000 to 32000: bf16 73 / 94 / 111 / 126 / 132, e4m3 52 / 55 / 71 / 74 / 82.
 template <int KIND, int NT>
 int launch_dim(AttnParams& p, int max_rt, const Sharing& how, cudaStream_t stream) {
   const int dh = p.w.c.dh;

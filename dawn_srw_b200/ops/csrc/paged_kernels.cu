@@ -83,10 +83,10 @@ __device__ __forceinline__ void store_row(void* pool, float* scales, size_t row,
   if (lane == 0) scales[row] = odd ? __uint_as_float(0x7fc00000u) : scale;
 }
 
-// A group of LPR lanes per (new token, head): its key and its value.  Bytes bound it: 24 prompts of 37 to 512 tokens, 16
-// heads of 128, fp32 to e4m3 (101 MB) take 23 us, 4.4 TB/s of 6.5; a token whose row, length and page are three loads one
-// behind the other has little else to wait behind, and two heads to a group were slower.  One token of 6 heads: 4 us, a
-// launch.
+// A group of LPR lanes per (new token, head): its key and its value.  Issue slots bound it more than bytes do: 24 prompts of
+// 37 to 512 tokens, 16 heads of 128, fp32 to e4m3 (101 MB) take 23 us, 4.4 TB/s of 6.5, with DRAM at 50 % and 68 % of the
+// slots taken, by the codes and by finding each row's sequence, length and page, loads that stand one behind the other.
+// Two heads to a group were slower.  One token of 6 heads: 4 us, a launch.
 template <int KIND, bool SRC_BF16, int LPR>
 __global__ void __launch_bounds__(kThreads) paged_write_kernel(const View w, const void* __restrict__ k,
                                                                const void* __restrict__ v, long long k_st, long long k_sh,
