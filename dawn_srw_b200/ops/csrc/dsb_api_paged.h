@@ -36,7 +36,8 @@ int dsb_paged_write(const struct DsbPaged* c, const void* k, const void* v, int 
 int dsb_paged_read(const struct DsbPaged* c, void* k, void* v, int dst_bf16, int max_len, cudaStream_t stream);
 // out [N, Hq, dh] bf16 = softmax(scale * q k^T) v over the keys at or before a row's position; with window > 0 only
 // the last `window` of them and the first `sinks` positions.  q bf16 [N, Hq, dh] (strides in elements), Hq a multiple
-// of H; B and H at most 65535.  A row without a key, or of no sequence, is zero.  max_new: the most new tokens a
+// of H; B and H at most 65535.  A row without a key, or of no sequence, is zero; what a row does not see never reaches it,
+// NaN and infinities included.  max_new: the most new tokens a
 // sequence has, as far as the caller knows (it chooses the kernel; a wrong one costs time only).  workspace:
 // dsb_paged_attention_workspace bytes of scratch, 16-byte aligned, this call's alone while it runs.
 long long dsb_paged_attention_workspace(const struct DsbPaged* c, int Hq, int max_new, int window, int sinks);

@@ -1020,7 +1020,7 @@ class CudaBackend:
         ``window`` of them and the first ``sinks`` positions only.  ``Hq`` is a multiple of the pages'
         heads; ``max_new``, the largest number of new tokens of a sequence if the caller knows it, only
         chooses the kernel.  Returns [N, Hq, dh] in bf16 (as ``attention``); zeros for a row that sees no
-        key or belongs to no sequence."""
+        key or belongs to no sequence.  NaN and infinities reach the rows that see them and no other."""
         count_launches(1)
         return ext().paged_attention(q, k_pages, v_pages, table, lengths, starts, k_scale, v_scale, max_new,
                                      window, sinks, scale, _paged_status(k_pages))

@@ -224,3 +224,43 @@ def test_nan_codes_read_back_as_nan(cb, be):
         assert int(want.isnan().sum()) == 4 and torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(), want.nan_to_num())
     cb.check_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[180, 40], [5, 3]])
+def test_captured_calls_follow_values_that_come_and_go(cb, be, kind, new):
+    """A call captured over an ordinary cache, replayed on two streams in turn while a value is no number, or a scale far
+    from the others, and when all is well again."""
+    lengths, at = [220, 40], 217
+    c = make_cache(kind, lengths, 2, 64, 16, "cuda", seed=3)
+    q, starts, page_slot = _rand(sum(new), 4, 64, seed=9), starts_of(new, "cuda"), _at(c, 0, at)
+    call = lambda: be.paged_attention(q, *args(c), starts, **scales(c))
+    first = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    page, slot = page_slot
+    keep = {n: None if c[n] is None else c[n].clone() for n in ("v_pages", "v_scale")}
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(6):
+        odd = i % 2 == 1
+        if odd and kind == "bf16":
+            c["v_pages"][page, 0, slot, 7] = math.inf
+        elif odd:
+            c["v_scale"][page, 0, slot] *= 2.0 ** 30
+        elif kind == "bf16":
+            c["v_pages"].copy_(keep["v_pages"])
+        else:
+            c["v_scale"].copy_(keep["v_scale"])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[i // 2 % 2]):
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = call()
+        assert torch.equal(out.nan_to_num(), eager.nan_to_num()) and torch.equal(out.isnan(), eager.isnan())
+        if odd:
+            _compare(cb, be, c, q, new)
+        else:
+            assert torch.equal(out, first)
+    cb.check_status()
